@@ -69,7 +69,9 @@ BOLT_API int bolt_set_launch_options(int pdl, int early_weights, int64_t smem_bu
  * Nonzero bits mean a kernel gave up a bounded wait (2 s) and returned without finishing
  * (bits 0-2, 4); bit 3 means a MoE expert id outside [0, E) was skipped; bit 5 means a
  * kernel found its shared-memory carve-out misaligned and returned without computing; bit 6
- * means a MambaVerify `sel` row lay outside its state buffers and nothing was written.
+ * means a MambaVerify `sel` row lay outside its state buffers and nothing was written; bit 7
+ * means a sequence's start or length did not fit its page table (the sequence was taken as
+ * empty); bit 8 means a page table named a page outside the cache (its tokens were left out).
  * No counterpart in the reference.
  */
 BOLT_API int bolt_get_device_status(unsigned* status);
@@ -256,6 +258,89 @@ BOLT_API int bolt_mamba_verify(const void* proj, const int64_t* proj_shape, int 
                                const void* sel, int64_t heads, int64_t head_dim, int64_t d_state, int64_t n_groups,
                                float epsilon, float time_step_min, void* y, void* conv_state_out,
                                void* ssm_state_out, void* xbc_act, void* ypre, void* stream);
+
+/*
+ * The paged 8-bit key/value cache (no counterpart in the reference, whose models leave attention to
+ * ONNX Runtime).  Five entry points share it:
+ *   k_cache, v_cache  u8  [pages, heads, T, D]   cache_shape; T in {16, 32, 64, 128, 256}, D in {64, 128}
+ *   k_scale, v_scale  f32 [pages, heads]         one scale (>= 0) per page and head
+ *   table             i32 [S, width]             table_shape; position j of sequence s is slot j % T of
+ *                                                page table[s][j / T]; entries past a sequence's end are not read
+ *   start, lens       i32 [S]                    row r of a call is position start[s] + r and exists while that
+ *                                                is below lens[s] (the length with the call's rows); a sequence
+ *                                                may be empty
+ *   fmt               0: value = scale * (code - 128), codes 1..255;  1: value = scale * e4m3(code)
+ * Rows (q, k, v) are bf16 [S, R, heads, D] with dense head and value axes; the sequence and row
+ * strides (elements, multiples of 8) are given, so parts of a fused projection can be passed as they
+ * are.  start, lens and table stay on the device, so a captured call follows them from step to step.
+ * A length, start or page that the tables cannot hold is left out and sets bit 7 or 8 of the device
+ * status word.
+ */
+
+/*
+ * KvAppend: quantise the rows k, v into the cache, in place.  For each page and head that takes rows,
+ * s' = max(s, max|x| / Q) over the new finite values x, where s is the page's scale if it holds
+ * positions before start[s] (0 otherwise) and Q is 127 (fmt 0) or 448 (fmt 1); the rows become
+ * round(x / s') and, where s' > s, the older codes round(c * (s / s')), ties to even.  Infinities are
+ * stored as +-Q * s' and NaN as 0.  Bytes of the page past the last row are left as they were.  A page
+ * must not take rows of two sequences in one call.
+ */
+BOLT_API int bolt_kv_append(const void* k, const int64_t* k_shape, const int64_t* k_strides, const void* v,
+                            const int64_t* v_strides, void* k_cache, const int64_t* cache_shape, void* v_cache,
+                            void* k_scale, void* v_scale, const void* table, const int64_t* table_shape,
+                            const void* start, const void* lens, int64_t fmt, void* stream);
+
+/*
+ * KvRead: k, v bf16 [S, rows, heads, D] = bf16(value) of the positions start[s] .. start[s] + rows - 1,
+ * 0 from lens[s] on.
+ */
+BOLT_API int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const void* v_cache, const void* k_scale,
+                          const void* v_scale, const void* table, const int64_t* table_shape, const void* start,
+                          const void* lens, int64_t rows, int64_t fmt, void* k, void* v, void* stream);
+
+/*
+ * KvAttention: attention of the rows q bf16 [S, R, Hq, D] (Hq a multiple of the cache's heads; query
+ * head i reads cache head i / (Hq / heads)) over the cached positions.  The row at position p sees
+ * the positions j <= p and, with window > 0, only those with j > p - window or j < sinks.
+ *   o    bf16 [S, R, Hq, D] = sum_j softmax_j(scale * q . k_j) v_j
+ *   lse  f32  [S, R, Hq]    = log sum_j exp(scale * q . k_j)
+ * Rows that do not exist give o = 0 and lse = -inf.
+ */
+BOLT_API int bolt_kv_attention(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,
+                               const int64_t* cache_shape, const void* v_cache, const void* k_scale,
+                               const void* v_scale, const void* table, const int64_t* table_shape, const void* start,
+                               const void* lens, float scale, int64_t window, int64_t sinks, int64_t fmt, void* o,
+                               void* lse, void* stream);
+
+/*
+ * KvScore: score f32 [S, heads, score_width] (score_width >= width * T) += each position's attention
+ * weight, sum over the rows and over the query heads of its cache head of exp(scale * q . k_j - lse),
+ * with q, the mask and lse as bolt_kv_attention took and gave them.  In place; positions that no row
+ * sees keep their sums.  The result does not depend on scheduling.
+ */
+BOLT_API int bolt_kv_score(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,
+                           const int64_t* cache_shape, const void* k_scale, const void* table,
+                           const int64_t* table_shape, const void* start, const void* lens, const void* lse,
+                           float scale, int64_t window, int64_t sinks, int64_t fmt, void* score, int64_t score_width,
+                           void* stream);
+
+/*
+ * KvEvict: cut every (sequence, head) to at most `keep` positions.  Of a sequence of more, each head keeps
+ * the first `sinks` positions, the last `recent` and of the others those of the largest score (equal
+ * ones: the lower position; NaN ranks highest), and lays their codes out in order in the pages of
+ * new_table i32 [S, new_width] (new_width * T >= keep; pages of the same cache that no table still in
+ * use names).  A new page's scale is the largest of its positions' scales s'; a code c of a position
+ * with scale s becomes round(c * (s / s')).
+ *   kept      i32 [S, heads, keep]  the kept positions, ascending; -1 past the end
+ *   new_lens  i32 [S]               min(lens[s], keep)
+ *   new_score f32 [S, heads, keep]  their scores; 0 past the end
+ * The old pages are not changed.  Heads keep different positions, so a window over the new cache
+ * counts kept positions.
+ */
+BOLT_API int bolt_kv_evict(void* k_cache, const int64_t* cache_shape, void* v_cache, void* k_scale, void* v_scale,
+                           const void* table, const int64_t* table_shape, const void* lens, const void* score,
+                           int64_t score_width, const void* new_table, int64_t new_width, int64_t keep, int64_t sinks,
+                           int64_t recent, int64_t fmt, void* kept, void* new_lens, void* new_score, void* stream);
 
 /*
  * Relu2 (replaces Relu2State::ComputeV2, src/bolt_ops.cu:630-646; kernel :624-629).

@@ -16,6 +16,7 @@
 #include "../../include/bolt_b200.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "kv.h"
 
 namespace bolt {
 
@@ -450,6 +451,181 @@ int bolt_mamba_verify(const void* proj, const int64_t* proj_shape, int proj_rank
   return mamba_impl(proj, proj_shape, proj_rank, conv_state, conv_shape, conv_rank, ssm_state, ssm_shape, ssm_rank,
                     conv_w, conv_b, dt_bias, a_neg, d_skip, norm_w, sel, heads, head_dim, d_state, n_groups, epsilon,
                     time_step_min, y, conv_state_out, ssm_state_out, xbc_act, ypre, stream);
+}
+
+namespace {
+// The arguments that the key/value cache entry points share.
+KvCache kv_cache(const std::string& op, const void* k, const int64_t* shape, const void* v, const void* ks,
+                 const void* vs, const void* table, const int64_t* table_shape, int64_t fmt) {
+  const auto need = [&](bool ok, const char* msg) {
+    if (!ok) throw std::invalid_argument(op + ": " + msg);
+  };
+  need(shape != nullptr && table_shape != nullptr, "null shape");
+  const int64_t pages = shape[0], heads = shape[1], T = shape[2], D = shape[3], S = table_shape[0], W = table_shape[1];
+  need(D == 64 || D == 128, "head size must be 64 or 128");
+  need(T >= 16 && T <= 256 && (T & (T - 1)) == 0, "a page must hold 16, 32, 64, 128 or 256 tokens");
+  need(pages >= 0 && pages <= INT32_MAX && heads >= 1 && heads <= 65535, "cache must be [pages, heads, tokens, head size]");
+  need(S >= 0 && S <= 65535 && W >= 0 && W * T <= (int64_t(1) << 30), "page table must be [sequences, pages of a sequence]");
+  need(fmt == kKvInt8 || fmt == kKvE4m3, "unknown cache format");
+  KvCache c{};
+  c.k = static_cast<uint8_t*>(const_cast<void*>(k));
+  c.v = static_cast<uint8_t*>(const_cast<void*>(v));
+  c.ks = static_cast<float*>(const_cast<void*>(ks));
+  c.vs = static_cast<float*>(const_cast<void*>(vs));
+  c.table = static_cast<const int*>(table);
+  c.pages = pages;
+  c.heads = static_cast<int>(heads);
+  c.T = static_cast<int>(T);
+  while ((int64_t(1) << c.tshift) < T) ++c.tshift;
+  c.D = static_cast<int>(D);
+  c.fmt = static_cast<int>(fmt);
+  c.S = static_cast<int>(S);
+  c.width = static_cast<int>(W);
+  return c;
+}
+
+// Rows [S, R, heads, D] whose head and value axes are dense: `strides` of the sequence and row axes in elements.
+int kv_row_shape(const std::string& op, const KvCache& c, const int64_t* shape, const int64_t* strides, int64_t heads) {
+  if (shape == nullptr) throw std::invalid_argument(op + ": null shape");
+  if (shape[0] != c.S || shape[2] != heads || shape[3] != c.D)
+    throw std::invalid_argument(op + ": rows must be [sequences, rows, heads, head size]");
+  if (shape[1] < 0 || shape[1] > (int64_t(1) << 30)) throw std::invalid_argument(op + ": bad row count");
+  if (strides && (strides[0] % 8 || strides[1] % 8 || strides[0] < 0 || strides[1] < 0))
+    throw std::invalid_argument(op + ": row strides must be multiples of 8");
+  return static_cast<int>(shape[1]);
+}
+
+void kv_pointers(const std::string& op, std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (p == nullptr) throw std::invalid_argument(op + ": null buffer");
+}
+
+// The arguments that KvAttention and KvScore share.
+KvAttnParams kv_attn(const std::string& op, const KvCache& c, const void* q, const int64_t* q_shape,
+                     const int64_t* q_strides, const void* start, const void* lens, float scale, int64_t window,
+                     int64_t sinks) {
+  KvAttnParams p{};
+  p.c = c;
+  if (q_shape == nullptr || q_strides == nullptr) throw std::invalid_argument(op + ": null shape");
+  const int64_t Hq = q_shape[2];
+  if (Hq < 1 || Hq > INT32_MAX || Hq % c.heads != 0)
+    throw std::invalid_argument(op + ": query heads must be a multiple of the cache's heads");
+  p.rows = KvRows{static_cast<const int*>(start), static_cast<const int*>(lens),
+                  kv_row_shape(op, c, q_shape, q_strides, Hq)};
+  if (window < 0 || sinks < 0) throw std::invalid_argument(op + ": window and sinks must not be negative");
+  const int64_t most = int64_t(1) << 30;  // no position is larger
+  p.mask = KvMask{static_cast<int>(std::min(window, most)), static_cast<int>(std::min(sinks, most))};
+  p.q = static_cast<const bf16*>(q);
+  p.qs = q_strides[0];
+  p.qr = q_strides[1];
+  p.Hq = static_cast<int>(Hq);
+  p.G = static_cast<int>(Hq / c.heads);
+  p.scale = scale;
+  return p;
+}
+}  // namespace
+
+int bolt_kv_append(const void* k, const int64_t* k_shape, const int64_t* k_strides, const void* v,
+                   const int64_t* v_strides, void* k_cache, const int64_t* cache_shape, void* v_cache, void* k_scale,
+                   void* v_scale, const void* table, const int64_t* table_shape, const void* start, const void* lens,
+                   int64_t fmt, void* stream) {
+  return guarded([&] {
+    const char* op = "KvAppend";
+    const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
+    require(k_strides != nullptr && v_strides != nullptr, "KvAppend: null shape");
+    const int R = kv_row_shape(op, c, k_shape, k_strides, c.heads);
+    kv_row_shape(op, c, k_shape, v_strides, c.heads);
+    if (c.S == 0 || R == 0 || c.width == 0) return;
+    kv_pointers(op, {k, v, k_cache, v_cache, k_scale, v_scale, table, start, lens});
+    require_aligned({k, v, k_cache, v_cache}, op);
+    check_launch(launch_kv_append(c, KvRows{static_cast<const int*>(start), static_cast<const int*>(lens), R},
+                                  static_cast<const bf16*>(k), k_strides[0], k_strides[1],
+                                  static_cast<const bf16*>(v), v_strides[0], v_strides[1], make_cfg(stream)));
+  });
+}
+
+int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const void* v_cache, const void* k_scale,
+                 const void* v_scale, const void* table, const int64_t* table_shape, const void* start,
+                 const void* lens, int64_t rows, int64_t fmt, void* k, void* v, void* stream) {
+  return guarded([&] {
+    const char* op = "KvRead";
+    const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
+    require(rows >= 0 && rows <= (int64_t(1) << 30), "KvRead: bad row count");
+    if (c.S == 0 || rows == 0) return;
+    kv_pointers(op, {k_cache, v_cache, k_scale, v_scale, table, start, lens, k, v});
+    require_aligned({k, v, k_cache, v_cache}, op);
+    check_launch(launch_kv_read(c, KvRows{static_cast<const int*>(start), static_cast<const int*>(lens),
+                                          static_cast<int>(rows)},
+                                static_cast<bf16*>(k), static_cast<bf16*>(v), make_cfg(stream)));
+  });
+}
+
+int bolt_kv_attention(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,
+                      const int64_t* cache_shape, const void* v_cache, const void* k_scale, const void* v_scale,
+                      const void* table, const int64_t* table_shape, const void* start, const void* lens, float scale,
+                      int64_t window, int64_t sinks, int64_t fmt, void* o, void* lse, void* stream) {
+  return guarded([&] {
+    const char* op = "KvAttention";
+    const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
+    KvAttnParams p = kv_attn(op, c, q, q_shape, q_strides, start, lens, scale, window, sinks);
+    if (c.S == 0 || p.rows.R == 0) return;
+    kv_pointers(op, {q, k_cache, v_cache, k_scale, v_scale, table, start, lens, o, lse});
+    require_aligned({q, k_cache, v_cache, o}, op);
+    p.o = static_cast<bf16*>(o);
+    p.lse = static_cast<float*>(lse);
+    check_launch(launch_kv_attention(p, make_cfg(stream)));
+  });
+}
+
+int bolt_kv_score(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,
+                  const int64_t* cache_shape, const void* k_scale, const void* table, const int64_t* table_shape,
+                  const void* start, const void* lens, const void* lse, float scale, int64_t window, int64_t sinks,
+                  int64_t fmt, void* score, int64_t score_width, void* stream) {
+  return guarded([&] {
+    const char* op = "KvScore";
+    const KvCache c = kv_cache(op, k_cache, cache_shape, nullptr, k_scale, nullptr, table, table_shape, fmt);
+    KvAttnParams p = kv_attn(op, c, q, q_shape, q_strides, start, lens, scale, window, sinks);
+    require(score_width >= static_cast<int64_t>(c.width) * c.T, "KvScore: score must cover the page table");
+    if (c.S == 0 || p.rows.R == 0 || c.width == 0) return;
+    kv_pointers(op, {q, k_cache, k_scale, table, start, lens, lse, score});
+    require_aligned({q, k_cache}, op);
+    p.lse = static_cast<float*>(const_cast<void*>(lse));
+    p.score = static_cast<float*>(score);
+    p.score_width = score_width;
+    check_launch(launch_kv_score(p, make_cfg(stream)));
+  });
+}
+
+int bolt_kv_evict(void* k_cache, const int64_t* cache_shape, void* v_cache, void* k_scale, void* v_scale,
+                  const void* table, const int64_t* table_shape, const void* lens, const void* score,
+                  int64_t score_width, const void* new_table, int64_t new_width, int64_t keep, int64_t sinks,
+                  int64_t recent, int64_t fmt, void* kept, void* new_lens, void* new_score, void* stream) {
+  return guarded([&] {
+    const char* op = "KvEvict";
+    const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
+    require(keep >= 1 && keep <= (int64_t(1) << 30), "KvEvict: keep must be at least 1");
+    require(sinks >= 0 && recent >= 0 && sinks <= keep && recent <= keep - sinks,
+            "KvEvict: sinks + recent must not exceed keep");
+    require(new_width * c.T >= keep && new_width <= INT32_MAX, "KvEvict: the new page table must hold keep positions");
+    require(score_width >= static_cast<int64_t>(c.width) * c.T, "KvEvict: score must cover the page table");
+    if (c.S == 0) return;
+    kv_pointers(op, {k_cache, v_cache, k_scale, v_scale, table, lens, score, new_table, kept, new_lens, new_score});
+    require_aligned({k_cache, v_cache}, op);
+    KvEvictParams p{};
+    p.c = c;
+    p.lens = static_cast<const int*>(lens);
+    p.score = static_cast<const float*>(score);
+    p.score_width = score_width;
+    p.new_table = static_cast<const int*>(new_table);
+    p.new_width = static_cast<int>(new_width);
+    p.keep = static_cast<int>(keep);
+    p.sinks = static_cast<int>(sinks);
+    p.recent = static_cast<int>(recent);
+    p.kept = static_cast<int*>(kept);
+    p.new_lens = static_cast<int*>(new_lens);
+    p.new_score = static_cast<float*>(new_score);
+    check_launch(launch_kv_evict(p, make_cfg(stream)));
+  });
 }
 
 int bolt_relu2(const void* x, const int64_t* x_shape, int x_rank, void* y, void* stream) {

@@ -32,6 +32,8 @@ enum StatusBits : unsigned {
   kStatusGridWait = 1u << 4,    // a cross-CTA wait timed out
   kStatusSmemAlign = 1u << 5,   // the shared-memory carve-out was not aligned as required
   kStatusBadRow = 1u << 6,      // a MambaVerify state row (sel) outside the state buffer: nothing written
+  kStatusKvRange = 1u << 7,     // a sequence's start or length outside its page table: taken as empty
+  kStatusKvPage = 1u << 8,      // a page table entry outside the cache: its tokens were left out
 };
 
 extern __device__ unsigned g_status;

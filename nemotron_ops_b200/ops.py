@@ -15,10 +15,12 @@ import torch
 from ._lib import last_error, lib, shape_arg
 
 __all__ = ["Nvfp4Gemv", "Q8Gemv", "Q4Gemv", "MoeRoute", "MoeDecode", "MoeVerify", "moe_verify_shard",
+           "KvAppend", "KvRead", "KvAttention", "KvScore", "KvEvict", "KV_INT8", "KV_E4M3",
            "f32_to_bf16", "copy_async", "dequant", "set_launch_options", "device_status", "FMT_Q8", "FMT_Q4", "FMT_NVFP4",
            "FMT_IQ2_LUT", "FMT_IQ2_NATIVE"]
 
 FMT_Q8, FMT_Q4, FMT_NVFP4, FMT_IQ2_LUT, FMT_IQ2_NATIVE = 0, 1, 2, 3, 4
+KV_INT8, KV_E4M3 = 0, 1
 
 
 def _ptr(t):
@@ -286,6 +288,145 @@ def Relu2(x):
     xs, _keep = shape_arg(x.shape)
     _check(lib().bolt_relu2(_ptr(x), xs, x.dim(), _ptr(y), _stream(x)))
     return y
+
+
+# ---------------------------------------------------------------------------------------------
+# paged 8-bit key/value cache (include/bolt_b200.h has the formulas)
+#   k_cache, v_cache u8 [pages, heads, T, D], k_scale, v_scale f32 [pages, heads]
+#   table i32 [S, width]: position j of sequence s is slot j % T of page table[s, j // T]
+#   start, lens i32 [S]: row r of a call is position start[s] + r, if that is below lens[s]
+# ---------------------------------------------------------------------------------------------
+def _kv_cache_args(op, k_cache, v_cache, k_scale, v_scale, table):
+    _need(k_cache, v_cache, k_scale, v_scale, table)
+    if not (k_cache.dtype == v_cache.dtype == torch.uint8 and k_scale.dtype == v_scale.dtype == torch.float32):
+        raise RuntimeError(f"{op}: caches are u8, scales f32")
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+        raise RuntimeError(f"{op}: cache must be [pages, heads, tokens, head size], scales [pages, heads]")
+    if table.dim() != 2:
+        raise RuntimeError(f"{op}: page table must be [sequences, pages of a sequence]")
+
+
+def _kv_indices(op, sequences, *tensors):
+    for t in tensors:
+        if t.dtype != torch.int32:
+            raise RuntimeError(f"{op}: page tables, starts and lengths are i32")
+    for t in tensors[1:]:
+        if t.shape != (sequences,):
+            raise RuntimeError(f"{op}: starts and lengths must be [sequences]")
+
+
+def _kv_rows(op, t, what):
+    """Strides of the sequence and row axes of rows [S, R, heads, D] whose last two axes are dense."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError("bolt ops take CUDA tensors (there is no CPU implementation)")
+    if t.dtype != torch.bfloat16 or t.dim() != 4:
+        raise RuntimeError(f"{op}: {what} must be bf16 [sequences, rows, heads, head size]")
+    seq, row, head, one = t.stride()
+    D = t.shape[3]
+    if (one != 1 and D != 1) or (head != D and t.shape[2] != 1):
+        raise RuntimeError(f"{op}: {what} must be dense over its heads and values")
+    # an axis of one entry has no step
+    return shape_arg((seq if t.shape[0] > 1 else 0, row if t.shape[1] > 1 else 0))
+
+
+def KvAppend(k, v, k_cache, v_cache, k_scale, v_scale, table, start, lens, fmt: int = KV_INT8):
+    """Quantise the rows k, v bf16 [S, R, heads, D] into their pages, in place: a page's scale grows to
+    max|x| / 127 (KV_INT8) or / 448 (KV_E4M3) where a row needs it, and its older codes with it."""
+    _kv_cache_args("KvAppend", k_cache, v_cache, k_scale, v_scale, table)
+    _need(start, lens)
+    _kv_indices("KvAppend", table.shape[0], table, start, lens)
+    ks, _k1 = _kv_rows("KvAppend", k, "k")
+    vs, _k2 = _kv_rows("KvAppend", v, "v")
+    if v.shape != k.shape:
+        raise RuntimeError("KvAppend: k and v must have the same shape")
+    shape, _k3 = shape_arg(k.shape)
+    cs, _k4 = shape_arg(k_cache.shape)
+    ts, _k5 = shape_arg(table.shape)
+    _check(lib().bolt_kv_append(_ptr(k), shape, ks, _ptr(v), vs, _ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale),
+                                _ptr(v_scale), _ptr(table), ts, _ptr(start), _ptr(lens), int(fmt), _stream(k_cache)))
+
+
+def KvRead(k_cache, v_cache, k_scale, v_scale, table, start, lens, rows: int, fmt: int = KV_INT8):
+    """Returns (k, v) bf16 [S, rows, heads, D]: what the cache holds of the positions from start on, 0 from
+    lens on."""
+    _kv_cache_args("KvRead", k_cache, v_cache, k_scale, v_scale, table)
+    _need(start, lens)
+    S = table.shape[0]
+    _kv_indices("KvRead", S, table, start, lens)
+    k = torch.empty(S, rows, k_cache.shape[1], k_cache.shape[3], dtype=torch.bfloat16, device=k_cache.device)
+    v = torch.empty_like(k)
+    cs, _k1 = shape_arg(k_cache.shape)
+    ts, _k2 = shape_arg(table.shape)
+    _check(lib().bolt_kv_read(_ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(table), ts,
+                              _ptr(start), _ptr(lens), int(rows), int(fmt), _ptr(k), _ptr(v), _stream(k_cache)))
+    return k, v
+
+
+def KvAttention(q, k_cache, v_cache, k_scale, v_scale, table, start, lens, scale: float, window: int = 0,
+                sinks: int = 0, fmt: int = KV_INT8):
+    """Returns (o bf16 [S, R, Hq, D], lse f32 [S, R, Hq]) of the rows q bf16 [S, R, Hq, D]: the row at
+    position p sees the positions j <= p and, with a window, only j > p - window or j < sinks."""
+    _kv_cache_args("KvAttention", k_cache, v_cache, k_scale, v_scale, table)
+    _need(start, lens)
+    _kv_indices("KvAttention", table.shape[0], table, start, lens)
+    st, _k1 = _kv_rows("KvAttention", q, "q")
+    o = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    shape, _k2 = shape_arg(q.shape)
+    cs, _k3 = shape_arg(k_cache.shape)
+    ts, _k4 = shape_arg(table.shape)
+    _check(lib().bolt_kv_attention(_ptr(q), shape, st, _ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+                                   _ptr(table), ts, _ptr(start), _ptr(lens), float(scale), int(window), int(sinks),
+                                   int(fmt), _ptr(o), _ptr(lse), _stream(k_cache)))
+    return o, lse
+
+
+def KvScore(q, k_cache, k_scale, table, start, lens, lse, score, scale: float, window: int = 0, sinks: int = 0,
+            fmt: int = KV_INT8):
+    """Adds every cached position's attention weight to score f32 [S, heads, >= width * T], in place (and
+    returns it); q, the mask and lse as in the KvAttention call whose weights are taken."""
+    _kv_cache_args("KvScore", k_cache, k_cache, k_scale, k_scale, table)
+    _need(start, lens, lse, score)
+    S, heads = table.shape[0], k_cache.shape[1]
+    _kv_indices("KvScore", S, table, start, lens)
+    st, _k1 = _kv_rows("KvScore", q, "q")
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:3]:
+        raise RuntimeError("KvScore: lse must be f32 [sequences, rows, query heads]")
+    if score.dtype != torch.float32 or score.dim() != 3 or score.shape[:2] != (S, heads):
+        raise RuntimeError("KvScore: score must be f32 [sequences, heads, positions]")
+    shape, _k2 = shape_arg(q.shape)
+    cs, _k3 = shape_arg(k_cache.shape)
+    ts, _k4 = shape_arg(table.shape)
+    _check(lib().bolt_kv_score(_ptr(q), shape, st, _ptr(k_cache), cs, _ptr(k_scale), _ptr(table), ts, _ptr(start),
+                               _ptr(lens), _ptr(lse), float(scale), int(window), int(sinks), int(fmt), _ptr(score),
+                               score.shape[2], _stream(k_cache)))
+    return score
+
+
+def KvEvict(k_cache, v_cache, k_scale, v_scale, table, lens, score, new_table, keep: int, sinks: int = 0,
+            recent: int = 0, fmt: int = KV_INT8):
+    """Cuts every (sequence, head) to its first `sinks` positions, its last `recent` and those of the largest
+    score, `keep` in all, laid out in order in the pages of new_table i32 [S, >= keep / T].  Returns
+    (kept i32 [S, heads, keep], new_lens i32 [S], new_score f32 [S, heads, keep])."""
+    _kv_cache_args("KvEvict", k_cache, v_cache, k_scale, v_scale, table)
+    _need(lens, score, new_table)
+    S, heads = table.shape[0], k_cache.shape[1]
+    _kv_indices("KvEvict", S, table, lens)
+    if new_table.dtype != torch.int32 or new_table.dim() != 2 or new_table.shape[0] != S:
+        raise RuntimeError("KvEvict: the new page table must be i32 [sequences, pages of a sequence]")
+    if score.dtype != torch.float32 or score.dim() != 3 or score.shape[:2] != (S, heads):
+        raise RuntimeError("KvEvict: score must be f32 [sequences, heads, positions]")
+    kept = torch.empty(S, heads, keep, dtype=torch.int32, device=score.device)
+    new_lens = torch.empty(S, dtype=torch.int32, device=score.device)
+    new_score = torch.empty(S, heads, keep, dtype=torch.float32, device=score.device)
+    cs, _k1 = shape_arg(k_cache.shape)
+    ts, _k2 = shape_arg(table.shape)
+    _check(lib().bolt_kv_evict(_ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(table), ts,
+                               _ptr(lens), _ptr(score), score.shape[2], _ptr(new_table), new_table.shape[1],
+                               int(keep), int(sinks), int(recent), int(fmt), _ptr(kept), _ptr(new_lens),
+                               _ptr(new_score), _stream(k_cache)))
+    return kept, new_lens, new_score
 
 
 def f32_to_bf16(t, out=None):

@@ -1,0 +1,497 @@
+"""The paged 8-bit key/value cache ops (CUDA path through the C ABI) against plain 64-bit forms.
+
+Bounds, with u = 2^-24 the unit of fp32 rounding:
+  logits   a dot product of D terms in fp32, summed in any order and truncated by the matrix unit:
+           2 D u sum|q k| scale, plus a few roundings of the product with the scales: (2 D + 16) u ql
+  lse      the logits' bound, and 2^-20 for exp, log and the sums over at most 2^20 terms' pairwise blocks
+  weights  a relative error of the logits' bound plus 2^-18
+  o        bf16's half step 2^-9 of the value (2^-8 taken), and a relative error of each weight of
+           2^-11 (weights may pass through a 16-bit product) + the logits' bound, times sum p|v|
+  codes    the exact quotient is within half a step (+ 2^-20 of it, for the fp32 quotient) of the code's value
+"""
+import numpy as np
+import pytest
+import torch
+
+import oracle as O
+from nemotron_ops_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+
+
+class Cache:
+    """A pool of pages in which `lens` positions of each sequence lie, scattered; random codes."""
+
+    def __init__(self, lens, H, D, T, fmt, seed=0, width=None, spare=2):
+        g = torch.Generator().manual_seed(seed)
+        need = [-(-n // T) for n in lens]
+        self.width = width or max(1, max(need))
+        pool = sum(need) + spare
+        perm = torch.randperm(pool, generator=g).int()
+        self.table = torch.full((len(lens), self.width), -1, dtype=torch.int32)  # unused entries name no page
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = perm[at:at + n]
+            at += n
+        self.free = perm[at:]
+        x = torch.randn(2, pool, H, T, D, generator=g) * (O.KV_QMAX[fmt] / 3)
+        x = x.clamp(-O.KV_QMAX[fmt], O.KV_QMAX[fmt])
+        codes = (x.round() + 128).to(torch.uint8) if fmt == 0 else x.to(torch.float8_e4m3fn).view(torch.uint8)
+        self.k, self.v = codes[0].contiguous(), codes[1].contiguous()
+        self.ks, self.vs = ((torch.rand(pool, H, generator=g) + 0.2) * 3 / O.KV_QMAX[fmt] for _ in range(2))
+        self.lens = torch.tensor(lens, dtype=torch.int32)
+        self.fmt, self.T = fmt, T
+
+    def dev(self):
+        return [t.to(DEV) for t in (self.k, self.v, self.ks, self.vs)]
+
+    def host(self):
+        return self.k, self.v, self.ks, self.vs
+
+
+def _rows(S, R, Hq, D, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(S, R, Hq, D, generator=g) * scale).bfloat16()
+
+
+def _check_attention(o, lse, ref, D):
+    o, lse = o.double().cpu().numpy(), lse.double().cpu().numpy()
+    dl = (2 * D + 16) * U * ref["ql"]
+    none = np.isneginf(ref["lse"])
+    assert np.array_equal(none, np.isneginf(lse))
+    lim = dl + 2.0 ** -20 * (1 + np.abs(np.where(none, 0, ref["lse"])))
+    assert (np.abs(np.where(none, 0, lse) - np.where(none, 0, ref["lse"])) <= lim).all()
+    bound = 2.0 ** -8 * np.abs(ref["o"]) + (2.0 ** -11 + 2.0 ** -18 + 2 * dl[..., None]) * ref["av"]
+    assert (np.abs(o - ref["o"]) <= bound).all(), float((np.abs(o - ref["o"]) - bound).max())
+
+
+def _attention(c, q, start, scale, **kw):
+    args = c.dev()
+    return ops.KvAttention(q.to(DEV), *args, c.table.to(DEV), start.to(DEV), c.lens.to(DEV), scale, fmt=c.fmt, **kw)
+
+
+CASES = [
+    # lens, R, Hq, Hkv, D, T, fmt, window, sinks
+    ([1], 1, 1, 1, 64, 16, 0, 0, 0),
+    ([1, 2, 0, 17], 1, 4, 2, 128, 16, 0, 0, 0),
+    ([15, 16, 17, 31, 32, 33], 1, 8, 2, 128, 16, 1, 0, 0),
+    ([127, 128, 129], 2, 16, 1, 64, 64, 0, 0, 0),
+    ([300, 0, 5], 5, 15, 3, 128, 32, 0, 0, 0),
+    ([777], 8, 32, 2, 128, 64, 1, 0, 0),
+    ([1000, 63], 8, 40, 8, 64, 128, 1, 0, 0),
+    ([2500], 1, 16, 1, 128, 256, 0, 0, 0),
+    ([511, 40, 3], 3, 6, 2, 128, 16, 0, 32, 4),
+    ([511, 40, 3], 3, 6, 2, 64, 32, 1, 1, 0),
+    ([700], 16, 2, 2, 128, 16, 0, 100, 40),
+    ([257, 300], 65, 8, 4, 128, 16, 0, 0, 0),
+    ([401], 130, 10, 2, 64, 32, 0, 64, 20),
+    ([140], 140, 17, 1, 128, 16, 1, 0, 0),
+]
+
+
+@pytest.mark.parametrize("lens,R,Hq,Hkv,D,T,fmt,window,sinks", CASES)
+def test_attention_matches_64_bits(lens, R, Hq, Hkv, D, T, fmt, window, sinks):
+    c = Cache(lens, Hkv, D, T, fmt, seed=len(lens) + R)
+    q = _rows(len(lens), R, Hq, D, seed=R)
+    start = (c.lens - R).clamp(min=0)
+    o, lse = _attention(c, q, start, D ** -0.5, window=window, sinks=sinks)
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, D ** -0.5, window, sinks, fmt)
+    _check_attention(o, lse, ref, D)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_peaked_logits_and_uneven_scales(D, fmt):
+    # one page's values are 10^4 times the others', and rows whose weights all lie elsewhere
+    lens = [400, 90]
+    c = Cache(lens, 2, D, 16, fmt, seed=9)
+    c.vs[c.table[0, 3].long()] *= 1e4
+    c.vs[c.table[1, 1].long()] = 0.0
+    c.ks[c.table[0, 5].long()] = 0.0
+    q = _rows(2, 2, 6, D, seed=4, scale=8.0)
+    start = c.lens - 2
+    o, lse = _attention(c, q, start, D ** -0.5)
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, D ** -0.5, fmt=fmt)
+    _check_attention(o, lse, ref, D)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e30])
+def test_attention_tiny_and_huge_query_values(scale):
+    # values that a 16-bit float cannot hold: the logits' scale brings them back
+    c = Cache([100], 1, 128, 32, 0, seed=2)
+    q = _rows(1, 2, 4, 128, seed=3, scale=scale)
+    start = c.lens - 2
+    o, lse = _attention(c, q, start, 128 ** -0.5 / scale)
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, 128 ** -0.5 / scale)
+    _check_attention(o, lse, ref, 128)
+
+
+def test_attention_rows_that_do_not_exist_and_stale_bytes():
+    # sequence 0 has 2 of 4 rows, sequence 1 none; bytes past a sequence's end are NaN codes
+    c = Cache([37, 20, 16], 2, 128, 32, 1, seed=5)
+    for s, n in enumerate([37, 20, 16]):
+        for cache in (c.k, c.v):
+            page = int(c.table[s, (n - 1) // 32])
+            cache[page, :, (n - 1) % 32 + 1:] = 0x7F
+    q = _rows(3, 4, 4, 128, seed=6)
+    start = torch.tensor([35, 20, 12], dtype=torch.int32)
+    o, lse = _attention(c, q, start, 0.1)
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, 0.1, fmt=1)
+    _check_attention(o, lse, ref, 128)
+    assert not o[0, 2:].any() and not o[1].any() and bool(torch.isneginf(lse[1]).all())
+
+
+def test_attention_takes_parts_of_a_projection():
+    c = Cache([50, 61], 2, 64, 16, 0, seed=7)
+    x = _rows(2, 3, 4 + 2 + 2, 64, seed=8).flatten(2)
+    q = x[..., :256].unflatten(-1, (4, 64))
+    start = c.lens - 3
+    dq = x.to(DEV)[..., :256].unflatten(-1, (4, 64))
+    o, lse = ops.KvAttention(dq, *c.dev(), c.table.to(DEV), start.to(DEV), c.lens.to(DEV), 0.125)
+    _check_attention(o, lse, O.kv_attention(q, *c.host(), c.table, start, c.lens, 0.125), 64)
+
+
+def test_attention_offsets_past_32_bits():
+    # a pool of 4.6 GB of codes a cache, whose last pages are used
+    T, H, D = 256, 2, 128
+    pool = (9 << 29) // (T * H * D)
+    c = Cache([600], H, D, T, 0, seed=11)
+    k, v = (torch.zeros(pool, H, T, D, dtype=torch.uint8, device=DEV) for _ in range(2))
+    ks, vs = (torch.zeros(pool, H, device=DEV) for _ in range(2))
+    table = torch.tensor([[pool - 1, pool - 3, pool - 2]], dtype=torch.int32, device=DEV)
+    old = c.table[0, :3].long()
+    for dst, src in ((k, c.k), (v, c.v), (ks, c.ks), (vs, c.vs)):
+        dst[table[0].long()] = src[old].to(DEV)
+    q = _rows(1, 1, 4, D, seed=12)
+    start = c.lens - 1
+    o, lse = ops.KvAttention(q.to(DEV), k, v, ks, vs, table, start.to(DEV), c.lens.to(DEV), 0.1)
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, 0.1)
+    _check_attention(o, lse, ref, D)
+    # and scored, written and read there (in this order: a write may requantise the page)
+    score = torch.zeros(1, H, 768, device=DEV)
+    ops.KvScore(q.to(DEV), k, ks, table, start.to(DEV), c.lens.to(DEV), lse, score, 0.1)
+    assert abs(float(score.sum()) - 4.0) < 1e-4
+    rows = _rows(1, 5, H, D, seed=13)
+    lens = torch.tensor([605], dtype=torch.int32, device=DEV)
+    at = torch.tensor([600], dtype=torch.int32, device=DEV)
+    ops.KvAppend(rows.to(DEV), rows.to(DEV), k, v, ks, vs, table, at, lens)
+    rk, rv = ops.KvRead(k, v, ks, vs, table, at, lens, 5)
+    step = torch.maximum(ks[pool - 2], vs[pool - 2]).cpu()[:, None]
+    assert bool(((rk.cpu().float() - rows.float()).abs() <= step * 0.502 + rows.float().abs() * 2 ** -8).all())
+    assert torch.equal(rk, rv) or not torch.equal(ks[pool - 2], vs[pool - 2])
+    assert ops.device_status() == 0
+
+
+def test_bad_lengths_and_pages_are_left_out():
+    c = Cache([40, 40, 40], 1, 64, 16, 0, seed=14)
+    q = _rows(3, 1, 2, 64, seed=15)
+    lens = torch.tensor([40, 49, -3], dtype=torch.int32)  # the table holds 48
+    start = torch.tensor([39, 48, 0], dtype=torch.int32)
+    assert ops.device_status() == 0
+    o, lse = ops.KvAttention(q.to(DEV), *c.dev(), c.table.to(DEV), start.to(DEV), lens.to(DEV), 0.1)
+    assert ops.device_status() == 1 << 7
+    ok = torch.tensor([40, 0, 0], dtype=torch.int32)
+    _check_attention(o, lse, O.kv_attention(q, *c.host(), c.table, start, ok, 0.1), 64)
+    # a page that the cache does not have: its 16 positions are not seen
+    bad = c.table.clone()
+    bad[0, 1] = c.k.shape[0]
+    o, lse = ops.KvAttention(q.to(DEV), *c.dev(), bad.to(DEV), start.to(DEV), ok.to(DEV), 0.1)
+    assert ops.device_status() == 1 << 8
+    k = O.kv_tokens(c.k, c.ks, c.table, 0, np.r_[0:16, 32:40], 0)[:, 0]
+    x = k @ q[0, 0].double().numpy().T * 0.1
+    assert np.allclose(np.log(np.exp(x).sum(0)), lse[0, 0].double().cpu().numpy(), atol=1e-4)
+
+
+@pytest.mark.parametrize("lens,R,Hq,Hkv,D,T,fmt,window,sinks", CASES)
+def test_score_matches_64_bits(lens, R, Hq, Hkv, D, T, fmt, window, sinks):
+    c = Cache(lens, Hkv, D, T, fmt, seed=len(lens) + R)
+    q = _rows(len(lens), R, Hq, D, seed=R)
+    start = (c.lens - R).clamp(min=0)
+    scale = D ** -0.5
+    att = O.kv_attention(q, *c.host(), c.table, start, c.lens, scale, window, sinks, fmt)
+    lse = torch.from_numpy(att["lse"]).float()
+    score = torch.rand(len(lens), Hkv, c.width * T + 3)
+    want, added = O.kv_score(q, c.k, c.ks, c.table, start, c.lens, lse, score, scale, window, sinks, fmt)
+    got = ops.KvScore(q.to(DEV), c.k.to(DEV), c.ks.to(DEV), c.table.to(DEV), start.to(DEV), c.lens.to(DEV),
+                      lse.to(DEV), score.to(DEV), scale, window=window, sinks=sinks, fmt=fmt)
+    got = got.double().cpu().numpy()
+    live = np.where(np.isneginf(att["lse"]), 0, np.abs(att["lse"]))
+    dl = (2 * D + 16) * U * att["ql"].max() + 4 * U * live.max() + 2.0 ** -18
+    assert (np.abs(got - want) <= 2 * dl * added + 2 * U * np.abs(want)).all()
+    assert ops.device_status() == 0
+
+
+def test_score_and_attention_are_the_same_from_call_to_call():
+    c = Cache([3000, 1700], 2, 128, 32, 0, seed=21)
+    q = _rows(2, 2, 16, 128, seed=22).to(DEV)
+    start = (c.lens - 2).to(DEV)
+    args, table, lens = c.dev(), c.table.to(DEV), c.lens.to(DEV)
+    first = None
+    for _ in range(5):
+        o, lse = ops.KvAttention(q, *args, table, start, lens, 0.1)
+        score = ops.KvScore(q, args[0], args[2], table, start, lens, lse, torch.zeros(2, 2, 94 * 32, device=DEV), 0.1)
+        if first is None:
+            first = o, lse, score
+        assert all(torch.equal(a, b) for a, b in zip(first, (o, lse, score)))
+
+
+# ---------------------------------------------------------------------------------------------
+# KvAppend, KvRead
+# ---------------------------------------------------------------------------------------------
+def _step(x, fmt):
+    """Size of the code grid at |x| (in units of the scale)."""
+    if fmt == 0:
+        return np.ones_like(x)
+    return 2.0 ** (np.floor(np.log2(np.maximum(np.abs(x), 2.0 ** -6))) - 3)
+
+
+def _check_codes(got, want, fmt):
+    """got: values of the codes; want: exact quotients."""
+    want = np.clip(want, -O.KV_QMAX[fmt], O.KV_QMAX[fmt])
+    lim = 0.5 * np.maximum(_step(want, fmt), _step(got, fmt)) + 2.0 ** -20 * np.abs(want) + 1e-30
+    assert (np.abs(got - want) <= lim).all()
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("lens,start,R,H,D,T", [
+    ([1], [0], 1, 1, 64, 16),
+    ([17, 16, 40, 0], [16, 15, 39, 0], 1, 3, 128, 16),
+    ([100, 33, 70], [63, 33, 0], 70, 2, 128, 32),
+    ([300, 261], [5, 250], 295, 2, 64, 256),
+    ([64, 130], [0, 127], 64, 1, 128, 64),
+])
+def test_append_matches_64_bits(lens, start, R, H, D, T, fmt):
+    c = Cache(lens, H, D, T, fmt, seed=31)
+    S = len(lens)
+    k, v = _rows(S, R, H, D, seed=32), _rows(S, R, H, D, seed=33, scale=4.0)
+    st = torch.tensor(start, dtype=torch.int32)
+    dev = c.dev()
+    ops.KvAppend(k.to(DEV), v.to(DEV), *dev, c.table.to(DEV), st.to(DEV), c.lens.to(DEV), fmt=fmt)
+    after = [t.cpu() for t in dev]
+    touched = torch.zeros(2, *c.ks.shape[:1], T, dtype=torch.bool)
+    for x, old, new, olds, news in ((k, c.k, after[0], c.ks, after[2]), (v, c.v, after[1], c.vs, after[3])):
+        seen = torch.zeros(old.shape[0], T, dtype=torch.bool)  # slots that may have changed
+        for s in range(S):
+            for lo in range(start[s] // T * T, lens[s] if lens[s] > start[s] else 0, T):
+                page, hi, first = int(c.table[s, lo // T]), min(lo + T, lens[s]), max(lo, start[s])
+                seen[page, :hi - lo] = True
+                for h in range(H):
+                    rows = x[s, first - start[s]:hi - start[s], h].double().numpy()
+                    unit = np.float32(np.abs(rows).max()) / np.float32(O.KV_QMAX[fmt])
+                    before = olds[page, h].numpy() if first > lo else np.float32(0)
+                    unit = max(unit, before)
+                    assert news[page, h].numpy() == unit
+                    got = O.kv_values(new[page, h], fmt)
+                    _check_codes(got[first - lo:hi - lo], rows / unit, fmt)
+                    if first > lo:
+                        held = O.kv_values(old[page, h, :first - lo], fmt)
+                        if unit == before:
+                            assert np.array_equal(got[:first - lo], held)
+                        else:
+                            _check_codes(got[:first - lo], held * (np.float64(before) / unit), fmt)
+        assert torch.equal(new[~seen[:, None].expand(-1, H, -1)], old[~seen[:, None].expand(-1, H, -1)])
+    # KvRead gives bf16(scale * value), and 0 past the end
+    rows = R + 3
+    rk, rv = ops.KvRead(*dev, c.table.to(DEV), st.to(DEV), c.lens.to(DEV), rows, fmt=fmt)
+    for got, cache, scale in ((rk, after[0], after[2]), (rv, after[1], after[3])):
+        for s in range(S):
+            n = max(0, min(rows, lens[s] - start[s]))
+            want = O.kv_tokens(cache, scale, c.table, s, np.arange(start[s], start[s] + n), fmt)
+            assert torch.equal(got[s, :n].cpu(), torch.from_numpy(want).float().bfloat16())
+            assert not got[s, n:].any()
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_append_special_values(fmt):
+    # zeros, an infinity, NaN, the smallest and the largest finite values
+    c = Cache([16, 16, 16, 16], 1, 64, 16, fmt, seed=41)
+    x = torch.zeros(4, 16, 1, 64)
+    x[1, 3, 0, :4] = torch.tensor([float("inf"), -float("inf"), float("nan"), 2.0])
+    x[2, 0, 0, 0] = 3.3e38
+    x[3, 0, 0, :2] = torch.tensor([1e-40, -1e-40])
+    x = x.bfloat16()
+    dev = c.dev()
+    zero = torch.zeros(4, dtype=torch.int32, device=DEV)
+    ops.KvAppend(x.to(DEV), x.to(DEV), *dev, c.table.to(DEV), zero, c.lens.to(DEV), fmt=fmt)
+    k, _ = ops.KvRead(*dev, c.table.to(DEV), zero, c.lens.to(DEV), 16, fmt=fmt)
+    k = k.cpu().float()
+    assert not k[0].any()
+    q = O.KV_QMAX[fmt]
+    unit = np.float32(2.0) / np.float32(q)
+    want = torch.tensor([q * unit, -q * unit, 0.0, q * unit]).bfloat16().float()
+    assert torch.equal(k[1, 3, 0, :4], want) and not k[1, :3].any()
+    assert abs(k[2, 0, 0, 0] / 3.3e38 - 1) < 0.01
+    assert bool((k[3].abs() <= 2e-40).all())
+    assert ops.device_status() == 0
+
+
+def test_append_step_by_step_holds_a_page_to_its_largest_value():
+    # one token at a time with growing values: every step requantises the page
+    H, D, T, n = 2, 64, 16, 40
+    c = Cache([n], H, D, T, 0, seed=51)
+    x = _rows(1, n, H, D, seed=52) * torch.linspace(0.1, 3.0, n)[None, :, None, None].bfloat16()
+    dev, table = c.dev(), c.table.to(DEV)
+    for i in range(n):
+        at = torch.tensor([i], dtype=torch.int32, device=DEV)
+        ops.KvAppend(x[:, i:i + 1].to(DEV), x[:, i:i + 1].to(DEV), *dev, table, at, at + 1)
+    k, _ = ops.KvRead(*dev, table, torch.zeros(1, dtype=torch.int32, device=DEV), c.lens.to(DEV), n)
+    unit = dev[2].cpu()[c.table[0].long()].repeat_interleave(T, 0)[:n]  # [n, H]
+    # a rounding a step: at most 16 half steps of at most the last scale
+    assert bool(((k.cpu()[0].float() - x[0].float()).abs() <= unit[..., None] * 8 + 0.02).all())
+
+
+# ---------------------------------------------------------------------------------------------
+# KvEvict
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("lens,keep,sinks,recent,H,D,T,kind", [
+    ([100], 40, 4, 8, 2, 128, 16, "even"),
+    ([1, 0, 33, 200], 33, 0, 0, 3, 64, 32, "even"),
+    ([5000, 33], 1000, 1, 999, 1, 64, 64, "even"),      # nothing but sinks and recent
+    ([3000, 2047], 700, 4, 128, 2, 128, 16, "ties"),
+    ([500], 123, 2, 3, 2, 64, 256, "same"),
+    ([400], 77, 0, 0, 1, 64, 16, "special"),
+    ([1500], 1499, 0, 1, 1, 128, 128, "even"),
+    ([40], 1, 0, 0, 1, 64, 16, "even"),
+])
+def test_evict_matches_the_definition(lens, keep, sinks, recent, H, D, T, kind, fmt):
+    S = len(lens)
+    blocks = -(-keep // T)
+    c = Cache(lens, H, D, T, fmt, seed=61, spare=S * blocks)
+    g = torch.Generator().manual_seed(62)
+    score = torch.rand(S, H, c.width * T + 5, generator=g)
+    if kind == "ties":
+        score = (score * 8).floor()
+    elif kind == "same":
+        score = torch.full_like(score, 0.25)
+    elif kind == "special":
+        score = torch.tensor([float("nan"), 0.0, -0.0, float("inf"), -float("inf"), -1.0, 1e-42, 3.0])[
+            torch.randint(0, 8, score.shape, generator=g)]
+    new_table = c.free[:S * blocks].view(S, blocks).contiguous()
+    dev = c.dev()
+    kept, new_lens, new_score = ops.KvEvict(*dev, c.table.to(DEV), c.lens.to(DEV), score.to(DEV), new_table.to(DEV),
+                                            keep, sinks=sinks, recent=recent, fmt=fmt)
+    after = [t.cpu() for t in dev]
+    kept, new_score = kept.cpu(), new_score.cpu()
+    assert new_lens.tolist() == [min(n, keep) for n in lens]
+    for s, n in enumerate(lens):
+        m = min(n, keep)
+        for h in range(H):
+            want = O.kv_evict_keep(score[s, h].numpy(), n, keep, sinks, recent)
+            assert np.array_equal(kept[s, h, :m].numpy(), want) and bool((kept[s, h, m:] == -1).all())
+            assert np.array_equal(new_score[s, h, :m].numpy(), score[s, h, torch.from_numpy(want)].numpy(),
+                                  equal_nan=True)
+            assert not new_score[s, h, m:].any()
+            for old, new, olds, news in ((c.k, after[0], c.ks, after[2]), (c.v, after[1], c.vs, after[3])):
+                for b in range(0, m, T):
+                    idx = want[b:b + T]
+                    src = c.table[s].long()[torch.from_numpy(idx) // T]
+                    units = olds[src, h].numpy()
+                    to = int(new_table[s, b // T])
+                    assert news[to, h].numpy() == units.max()
+                    held = O.kv_values(old[src, h, torch.from_numpy(idx) % T], fmt)
+                    got = O.kv_values(new[to, h, :len(idx)], fmt)
+                    _check_codes(got, held * (units.astype(np.float64) / units.max())[:, None], fmt)
+                    same = units == units.max()
+                    assert np.array_equal(got[same], held[same])
+    # the old pages are as they were
+    used = c.table[c.table >= 0].long()
+    for a, b in zip(after, c.host()):
+        assert torch.equal(a[used], b[used])
+    assert ops.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# a whole step, captured; streams
+# ---------------------------------------------------------------------------------------------
+def test_step_in_a_graph_follows_the_lengths():
+    # append, attention and score captured once; replays at other lengths read them from the device
+    H, Hq, D, T, S = 2, 8, 128, 16, 2
+    c = Cache([70, 70], H, D, T, 0, seed=71)
+    dev, table = c.dev(), c.table.to(DEV)
+    x = _rows(S, 1, Hq + 2 * H, D, seed=72).to(DEV)
+    q, k, v = x[:, :, :Hq], x[:, :, Hq:Hq + H], x[:, :, Hq + H:]
+    start = torch.tensor([40, 11], dtype=torch.int32, device=DEV)
+    lens = start + 1
+    score = torch.zeros(S, H, c.width * T, device=DEV)
+
+    def step():
+        ops.KvAppend(k, v, *dev, table, start, lens)
+        o, lse = ops.KvAttention(q, *dev, table, start, lens, 0.1)
+        return o, lse, ops.KvScore(q, dev[0], dev[2], table, start, lens, lse, score, 0.1)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse, _ = step()
+    for i in range(3):
+        start.copy_(torch.tensor([50 + 5 * i, 20 * i], dtype=torch.int32))
+        lens.copy_(start + 1)
+        score.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        host = [t.cpu() for t in dev]
+        ref = O.kv_attention(q.cpu(), host[0], host[1], host[2], host[3], c.table, start.cpu(), lens.cpu(), 0.1)
+        _check_attention(o, lse, ref, D)
+        for s in range(S):
+            n = int(lens[s])
+            assert abs(float(score[s].sum()) - Hq) < 1e-3 and not score[s, :, n:].any()
+    assert ops.device_status() == 0
+
+
+def test_refusals():
+    c = Cache([20, 20], 2, 64, 16, 0, seed=81)
+    dev, table, lens = c.dev(), c.table.to(DEV), c.lens.to(DEV)
+    start = lens - 1
+    q = _rows(2, 1, 4, 64, seed=82).to(DEV)
+    row = _rows(2, 1, 2, 64, seed=83).to(DEV)
+
+    def att(**kw):
+        a = dict(q=q, k_cache=dev[0], v_cache=dev[1], k_scale=dev[2], v_scale=dev[3], table=table, start=start,
+                 lens=lens, scale=0.1)
+        a.update(kw)
+        return ops.KvAttention(**a)
+
+    for kw, msg in [
+        (dict(q=q.float()), "bf16"),
+        (dict(q=q[:, :, :3]), "multiple of the cache's heads"),
+        (dict(q=q[:1]), "rows must be"),
+        (dict(q=q.transpose(2, 3)), "dense"),
+        (dict(q=torch.empty(2, 1, 4 * 64 + 4, dtype=torch.bfloat16, device=DEV)[..., :256].unflatten(-1, (4, 64))),
+         "multiples of 8"),
+        (dict(q=q.cpu()), "CUDA tensors"),
+        (dict(k_cache=dev[0][..., :32].contiguous(), v_cache=dev[1][..., :32].contiguous()), "head size"),
+        (dict(k_cache=dev[0][:, :, :8].contiguous(), v_cache=dev[1][:, :, :8].contiguous()), "a page must hold"),
+        (dict(k_scale=dev[2][:, :1].contiguous()), "scales"),
+        (dict(v_scale=dev[3].double()), "f32"),
+        (dict(table=table.long()), "i32"),
+        (dict(lens=lens[:1]), "starts and lengths"),
+        (dict(window=-1), "must not be negative"),
+        (dict(fmt=2), "unknown cache format"),
+    ]:
+        with pytest.raises(RuntimeError, match=msg):
+            att(**kw)
+    with pytest.raises(RuntimeError, match="same shape"):
+        ops.KvAppend(row, row[:, :, :1], *dev, table, start, lens)
+    score = torch.zeros(2, 2, 32, device=DEV)
+    lse = torch.zeros(2, 1, 4, device=DEV)
+    with pytest.raises(RuntimeError, match="score must cover"):
+        ops.KvScore(q, dev[0], dev[2], table, start, lens, lse, score[:, :, :31].contiguous(), 0.1)
+    with pytest.raises(RuntimeError, match="lse must be"):
+        ops.KvScore(q, dev[0], dev[2], table, start, lens, lse[..., :2].contiguous(), score, 0.1)
+    new = torch.zeros(2, 1, dtype=torch.int32, device=DEV)
+    for kw, msg in [(dict(keep=17), "must hold keep"), (dict(keep=0), "at least 1"),
+                    (dict(keep=8, sinks=5, recent=4), "must not exceed keep")]:
+        with pytest.raises(RuntimeError, match=msg):
+            ops.KvEvict(*dev, table, lens, score, new, **kw)
+    # nothing to do
+    o, lse = att(q=q[:, :0])
+    assert o.shape == (2, 0, 4, 64) and lse.shape == (2, 0, 4)
+    assert ops.device_status() == 0
