@@ -305,12 +305,16 @@ BOLT_API int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const
  *   o    bf16 [S, R, Hq, D] = sum_j softmax_j(scale * q . k_j) v_j
  *   lse  f32  [S, R, Hq]    = log sum_j exp(scale * q . k_j)
  * Rows that do not exist give o = 0 and lse = -inf.
+ *   workspace  scratch device memory of bolt_kv_attention_workspace(q_shape, cache_shape) bytes on the
+ *              current device (-1: bad shapes), 16-byte aligned; nothing has to be in it, and nothing
+ *              of it is read by a later call
  */
+BOLT_API int64_t bolt_kv_attention_workspace(const int64_t* q_shape, const int64_t* cache_shape);
 BOLT_API int bolt_kv_attention(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,
                                const int64_t* cache_shape, const void* v_cache, const void* k_scale,
                                const void* v_scale, const void* table, const int64_t* table_shape, const void* start,
                                const void* lens, float scale, int64_t window, int64_t sinks, int64_t fmt, void* o,
-                               void* lse, void* stream);
+                               void* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * KvScore: score f32 [S, heads, score_width] (score_width >= width * T) += each position's attention

@@ -36,7 +36,8 @@ SIGNATURES = {
                                _F, _P, _P, _P, _P, _P, _P]),
     "bolt_kv_append": (_I, [_P, _S, _S, _P, _S, _P, _S, _P, _P, _P, _P, _S, _P, _P, _L, _P]),
     "bolt_kv_read": (_I, [_P, _S, _P, _P, _P, _P, _S, _P, _P, _L, _L, _P, _P, _P]),
-    "bolt_kv_attention": (_I, [_P, _S, _S, _P, _S, _P, _P, _P, _P, _S, _P, _P, _F, _L, _L, _L, _P, _P, _P]),
+    "bolt_kv_attention_workspace": (_L, [_S, _S]),
+    "bolt_kv_attention": (_I, [_P, _S, _S, _P, _S, _P, _P, _P, _P, _S, _P, _P, _F, _L, _L, _L, _P, _P, _P, _L, _P]),
     "bolt_kv_score": (_I, [_P, _S, _S, _P, _S, _P, _P, _S, _P, _P, _P, _F, _L, _L, _L, _P, _L, _P]),
     "bolt_kv_evict": (_I, [_P, _S, _P, _P, _P, _P, _S, _P, _P, _L, _P, _L, _L, _L, _L, _L, _P, _P, _P, _P]),
     "bolt_relu2": (_I, [_P, _S, _I, _P, _P]),

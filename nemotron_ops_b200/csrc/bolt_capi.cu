@@ -560,20 +560,35 @@ int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const void* v_
   });
 }
 
+int64_t bolt_kv_attention_workspace(const int64_t* q_shape, const int64_t* cache_shape) {
+  int64_t n = -1;
+  guarded([&] {
+    require(q_shape != nullptr && cache_shape != nullptr, "KvAttention: null shape");
+    require(cache_shape[1] >= 1 && q_shape[2] >= 1 && q_shape[2] % cache_shape[1] == 0 && q_shape[1] >= 0,
+            "KvAttention: query heads must be a multiple of the cache's heads");
+    n = kv_attention_workspace(q_shape[1] * (q_shape[2] / cache_shape[1]), static_cast<int>(cache_shape[3]), sm_count());
+  });
+  return n;
+}
+
 int bolt_kv_attention(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,
                       const int64_t* cache_shape, const void* v_cache, const void* k_scale, const void* v_scale,
                       const void* table, const int64_t* table_shape, const void* start, const void* lens, float scale,
-                      int64_t window, int64_t sinks, int64_t fmt, void* o, void* lse, void* stream) {
+                      int64_t window, int64_t sinks, int64_t fmt, void* o, void* lse, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
   return guarded([&] {
     const char* op = "KvAttention";
     const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
     KvAttnParams p = kv_attn(op, c, q, q_shape, q_strides, start, lens, scale, window, sinks);
     if (c.S == 0 || p.rows.R == 0) return;
-    kv_pointers(op, {q, k_cache, v_cache, k_scale, v_scale, table, start, lens, o, lse});
-    require_aligned({q, k_cache, v_cache, o}, op);
+    kv_pointers(op, {q, k_cache, v_cache, k_scale, v_scale, table, start, lens, o, lse, workspace});
+    require_aligned({q, k_cache, v_cache, o, workspace}, op);
     p.o = static_cast<bf16*>(o);
     p.lse = static_cast<float*>(lse);
-    check_launch(launch_kv_attention(p, make_cfg(stream)));
+    const LaunchCfg cfg = make_cfg(stream);
+    require(workspace_bytes >= kv_attention_workspace(static_cast<int64_t>(p.rows.R) * p.G, c.D, cfg.sms),
+            "KvAttention: the workspace is too small (bolt_kv_attention_workspace)");
+    check_launch(launch_kv_attention(p, workspace, cfg));
   });
 }
 

@@ -50,7 +50,10 @@ struct KvAttnParams {
 cudaError_t launch_kv_append(const KvCache& c, const KvRows& rows, const bf16* k, int64_t k_seq, int64_t k_row,
                              const bf16* v, int64_t v_seq, int64_t v_row, const LaunchCfg& cfg);
 cudaError_t launch_kv_read(const KvCache& c, const KvRows& rows, bf16* k, bf16* v, const LaunchCfg& cfg);
-cudaError_t launch_kv_attention(const KvAttnParams& p, const LaunchCfg& cfg);
+// Bytes of the scratch memory that launch_kv_attention takes (16-byte aligned).
+// `rows`: R * G, the rows that read one head of the cache.
+int64_t kv_attention_workspace(int64_t rows, int D, int sms);
+cudaError_t launch_kv_attention(const KvAttnParams& p, void* workspace, const LaunchCfg& cfg);
 cudaError_t launch_kv_score(const KvAttnParams& p, const LaunchCfg& cfg);
 
 struct KvEvictParams {

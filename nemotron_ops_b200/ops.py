@@ -376,9 +376,10 @@ def KvAttention(q, k_cache, v_cache, k_scale, v_scale, table, start, lens, scale
     shape, _k2 = shape_arg(q.shape)
     cs, _k3 = shape_arg(k_cache.shape)
     ts, _k4 = shape_arg(table.shape)
+    ws = torch.empty(max(0, lib().bolt_kv_attention_workspace(shape, cs)), dtype=torch.uint8, device=q.device)
     _check(lib().bolt_kv_attention(_ptr(q), shape, st, _ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
                                    _ptr(table), ts, _ptr(start), _ptr(lens), float(scale), int(window), int(sinks),
-                                   int(fmt), _ptr(o), _ptr(lse), _stream(k_cache)))
+                                   int(fmt), _ptr(o), _ptr(lse), _ptr(ws), ws.numel(), _stream(k_cache)))
     return o, lse
 
 
