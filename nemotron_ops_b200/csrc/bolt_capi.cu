@@ -489,7 +489,7 @@ int kv_row_shape(const std::string& op, const KvCache& c, const int64_t* shape, 
   if (shape == nullptr) throw std::invalid_argument(op + ": null shape");
   if (shape[0] != c.S || shape[2] != heads || shape[3] != c.D)
     throw std::invalid_argument(op + ": rows must be [sequences, rows, heads, head size]");
-  if (shape[1] < 0 || shape[1] > (int64_t(1) << 30)) throw std::invalid_argument(op + ": bad row count");
+  if (shape[1] < 0 || shape[1] > (int64_t(1) << 29)) throw std::invalid_argument(op + ": bad row count");
   if (strides && (strides[0] % 8 || strides[1] % 8 || strides[0] < 0 || strides[1] < 0))
     throw std::invalid_argument(op + ": row strides must be multiples of 8");
   return static_cast<int>(shape[1]);
@@ -550,7 +550,7 @@ int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const void* v_
   return guarded([&] {
     const char* op = "KvRead";
     const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
-    require(rows >= 0 && rows <= (int64_t(1) << 30), "KvRead: bad row count");
+    require(rows >= 0 && rows <= (int64_t(1) << 29), "KvRead: bad row count");
     if (c.S == 0 || rows == 0) return;
     kv_pointers(op, {k_cache, v_cache, k_scale, v_scale, table, start, lens, k, v});
     require_aligned({k, v, k_cache, v_cache}, op);

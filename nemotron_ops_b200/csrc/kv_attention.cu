@@ -35,11 +35,14 @@ struct Work {
   int row_blocks;
 };
 
-template <int D, int MR, int MW, int TW>
+template <int D, int MR, int MW, int TW, int STAGES>
 struct Tile {
   static constexpr int kRows = MR * MW * 16, kThreads = MW * TW * 32;
-  static constexpr int kQ = MR * MW * (D / 16) * 32;  // uint4
-  static constexpr size_t kSmem = kQ * 16 + kRows * 4 + TW * kRows * 8 + static_cast<size_t>(TW) * kRows * D * 4;
+  static constexpr int kQ = MR * MW * (D / 16) * 32;      // uint4 of query operands
+  static constexpr int kStep = D * 2;                     // uint4 of a warp's step: 16 positions, K and V
+  static constexpr int kRing = MW * TW * STAGES * kStep;  // uint4
+  static constexpr int kJoin = TW * kRows * D / 4;        // uint4, in the ring's place
+  static constexpr size_t kSmem = (kQ + (kRing > kJoin ? kRing : kJoin)) * 16 + kRows * 4 + TW * kRows * 8;
 };
 
 // float4 index f of a row's values in the joining buffer, spread over the banks
@@ -48,113 +51,135 @@ __device__ __forceinline__ int swizzle(int row, int f) {
   return f ^ ((f >> 3) | ((row & 1) << (D == 128 ? 2 : 1)));
 }
 
-template <int D, bool KEEP>
-struct VRaw;
-template <bool KEEP>
-struct VRaw<128, KEEP> {
-  uint4 x[4];
-  __device__ __forceinline__ void load(const uint8_t* v, int64_t at) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+// A warp's step in its ring: every lane copies the bytes that it will use itself, so that no other
+// lane waits for them.  K: lane (g, c) takes the codes 64 i + 16 c .. + 15 of the positions g and 8 + g.
+// V: the codes (D / 8) g .. of the positions 2 c, 2 c + 1, 8 + 2 c and 8 + 2 c + 1.
+template <int D>
+__device__ __forceinline__ void copy_step(uint4* to, const uint8_t* k, const uint8_t* v) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = ld128<KEEP>(v + (at + (i >> 1) * 8 + 2 * c + (i & 1)) * 128 + 16 * g);
-  }
-  __device__ __forceinline__ uint32_t word(int i, int w) const { return word_of(x[i], w); }
-  __device__ __forceinline__ void clear(int i) { x[i] = make_uint4(0, 0, 0, 0); }
-};
-template <bool KEEP>
-struct VRaw<64, KEEP> {
-  uint2 x[4];
-  __device__ __forceinline__ void load(const uint8_t* v, int64_t at) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = ld64<KEEP>(v + (at + (i >> 1) * 8 + 2 * c + (i & 1)) * 64 + 8 * g);
+    for (int i = 0; i < D / 64; ++i) cp_async16(to + (t * (D / 64) + i) * 32 + lane, k + (8 * t + g) * D + 64 * i + 16 * c);
+  to += D / 32 * 32;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint8_t* from = v + ((i >> 1) * 8 + 2 * c + (i & 1)) * D + D / 8 * g;
+    if constexpr (D == 128)
+      cp_async16(to + i * 32 + lane, from);
+    else
+      cp_async8(reinterpret_cast<uint2*>(to) + i * 32 + lane, from);
   }
-  __device__ __forceinline__ uint32_t word(int i, int w) const { return w == 0 ? x[i].x : x[i].y; }
-  __device__ __forceinline__ void clear(int i) { x[i] = make_uint2(0, 0); }
+}
+
+template <int D>
+struct VCodes {
+  uint32_t w[4][D / 32];  // position, word
+  __device__ __forceinline__ void load(const uint4* from) {
+    const int lane = threadIdx.x & 31;
+    from += D / 32 * 32;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (D == 128) {
+        const uint4 x = from[i * 32 + lane];
+        w[i][0] = x.x;
+        w[i][1] = x.y;
+        w[i][2] = x.z;
+        w[i][3] = x.w;
+      } else {
+        const uint2 x = reinterpret_cast<const uint2*>(from)[i * 32 + lane];
+        w[i][0] = x.x;
+        w[i][1] = x.y;
+      }
+    }
+  }
 };
 
-template <int D, bool KEEP>
-struct Step {
-  uint4 k[2][D / 64];
-  VRaw<D, KEEP> v;
-};
-
-template <int D, int FMT, int MR, int MW, int TW, int CPS>
+template <int D, int FMT, int MR, int MW, int TW, int STAGES, int CPS>
 __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const KvAttnParams p, const Work w) {
-  using L = Tile<D, MR, MW, TW>;
-  constexpr bool kKeep = MW > 1;  // the MW warps of a step read the same lines
+  using L = Tile<D, MR, MW, TW, STAGES>;
   extern __shared__ uint4 smem[];
-  uint4* sq = smem;                                      // [MW * MR][D / 16][32]
-  float* sf = reinterpret_cast<float*>(smem + L::kQ);    // [rows]
-  float* sm = sf + L::kRows;                             // [TW][rows]
-  float* sl = sm + TW * L::kRows;                        // [TW][rows]
-  float4* so = reinterpret_cast<float4*>(sl + TW * L::kRows);  // [TW][rows][D / 4]
+  uint4* sq = smem;                                                                  // [MW * MR][D / 16][32]
+  float4* so = reinterpret_cast<float4*>(smem + L::kQ);                              // [TW][rows][D / 4]
+  float* sf = reinterpret_cast<float*>(smem + L::kSmem / 16) - L::kRows * (1 + 2 * TW);  // [rows]
+  float* sm = sf + L::kRows;                                                         // [TW][rows]
+  float* sl = sm + TW * L::kRows;                                                    // [TW][rows]
   pdl_wait();
   pdl_trigger();
   const KvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
   const int mw = warp % MW, tk = warp / MW;
-  const int64_t M = static_cast<int64_t>(p.rows.R) * p.G;
-  const int64_t pairs = static_cast<int64_t>(c.S) * w.row_blocks;
-  const bool by_item = pairs * c.heads == w.splits;
-  KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW);
+  uint4* ring = smem + L::kQ + warp * STAGES * L::kStep;
+  const unsigned M = static_cast<unsigned>(p.rows.R) * p.G, G = p.G;
+  const int pairs = c.S * w.row_blocks;
+  const bool by_item = static_cast<int64_t>(pairs) * c.heads == w.splits;
+  const KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW);
 
   if (!by_item && tid == 0) w.split[blockIdx.x].parts = 0;
   // items without steps: their rows see nothing
-  for (int64_t i = blockIdx.x; i < pairs; i += gridDim.x) {
-    const int s = static_cast<int>(i / w.row_blocks);
-    const int64_t m0 = (i % w.row_blocks) * L::kRows;
-    const KvSeq seq = kv_seq(c, p.rows.start, p.rows.lens, s);
-    if (kv_span(p, seq, m0, L::kRows).n > 0) continue;
-    const int64_t rows = min(M - m0, static_cast<int64_t>(L::kRows)) * c.heads;
-    for (int64_t e = tid; e < rows * (D / 8); e += L::kThreads) {
-      const int64_t row = e / (D / 8), m = m0 + row / c.heads;
-      const int64_t out = (static_cast<int64_t>(s) * p.rows.R + m / p.G) * p.Hq + (row % c.heads) * p.G + m % p.G;
+  for (int i = blockIdx.x; i < pairs; i += gridDim.x) {
+    const int s = i / w.row_blocks;
+    const unsigned m0 = (i - s * w.row_blocks) * L::kRows;
+    if (kv_span(p, kv_seq(c, p.rows.start, p.rows.lens, s), m0, L::kRows).n > 0) continue;
+    const unsigned rows = min(M - m0, static_cast<unsigned>(L::kRows)) * c.heads;
+    for (unsigned e = tid; e < rows * (D / 8); e += L::kThreads) {
+      const unsigned row = e / (D / 8), h = row % c.heads, m = m0 + row / c.heads, r = m / G;
+      const int64_t out = (static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * G + (m - r * G);
       reinterpret_cast<uint4*>(p.o + out * D)[e % (D / 8)] = make_uint4(0, 0, 0, 0);
       if (e % (D / 8) == 0) p.lse[out] = -INFINITY;
     }
     if (by_item)
-      for (int h = tid; h < c.heads; h += L::kThreads) w.split[i * c.heads + h].parts = 0;
+      for (int h = tid; h < c.heads; h += L::kThreads) w.split[static_cast<int64_t>(i) * c.heads + h].parts = 0;
   }
 
-  const int64_t begin = blockIdx.x * share.per, end = min(begin + share.per, share.total);
-  int64_t pair = share.pair, off = share.off;
-  for (int64_t at = begin; at < end;) {
-    const int s = static_cast<int>(pair / w.row_blocks), mb = static_cast<int>(pair % w.row_blocks);
-    const int64_t m0 = static_cast<int64_t>(mb) * L::kRows;
+  int64_t left = share.left, off = share.off, at = share.at;
+  for (int pair = share.pair; left > 0;) {
+    const int s = pair / w.row_blocks, mb = pair - s * w.row_blocks;
+    const unsigned m0 = static_cast<unsigned>(mb) * L::kRows;
     const KvSeq seq = kv_seq(c, p.rows.start, p.rows.lens, s);
     const KvSpan span = kv_span(p, seq, m0, L::kRows);
     if (span.n == 0) {
       ++pair;
       continue;
     }
-    const int h = static_cast<int>(off / span.n), i0 = static_cast<int>(off % span.n);
-    const int i1 = static_cast<int>(min(static_cast<int64_t>(span.n), i0 + end - at));
+    const int h = static_cast<int>(kv_div(off, span.n)), i0 = static_cast<int>(off - static_cast<int64_t>(h) * span.n);
+    const int i1 = static_cast<int>(min(static_cast<int64_t>(span.n), i0 + left));
 
     // ---- the segment: steps i0 .. i1 - 1, this warp's are i0 + tk, + TW, ...
-    if (tk == 0)
-#pragma unroll
-      for (int r = 0; r < MR; ++r)
-        kv_load_q<D>(p, seq, s, h, m0 + (mw * MR + r) * 16, sq + (mw * MR + r) * (D / 16) * 32, sf + (mw * MR + r) * 16);
-    int pos[MR][2];
-#pragma unroll
-    for (int r = 0; r < MR; ++r)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int64_t m = m0 + (mw * MR + r) * 16 + 8 * e + g;
-        const int64_t at_row = seq.start + m / p.G;
-        pos[r][e] = m < M && at_row < seq.len ? static_cast<int>(at_row) : -1;
-      }
     const KvSpan mine = kv_span(p, seq, min(m0 + mw * MR * 16, M), MR * 16);
     const int steps = mine.n > 0 ? max(0, (i1 - i0 - tk + TW - 1) / TW) : 0;
     const auto base_of = [&](int n) { return span.base(i0 + tk + n * TW); };
     const uint8_t* kc = c.k + static_cast<int64_t>(h) * c.T * D;
     const uint8_t* vc = c.v + static_cast<int64_t>(h) * c.T * D;
     const int64_t page_codes = static_cast<int64_t>(c.heads) * c.T * D;
-
+    KvPages meta = kv_pages(c, s, lane < steps, base_of(lane)), next{-1};
+    const auto fetch = [&](int n, int page) {  // step n into its slot of the ring; an empty group where there is none
+      if (page >= 0) {
+        const int64_t from = page * page_codes + (base_of(n) & (c.T - 1)) * D;
+        copy_step<D>(ring + n % STAGES * L::kStep, kc + from, vc + from);
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int n = 0; n < STAGES - 1; ++n) {
+      const int page = __shfl_sync(0xffffffffu, meta.page, n);
+      fetch(n, n < steps ? page : -1);
+    }
+    kv_scales<true>(c, h, meta);
+    if (tk == 0)
+#pragma unroll
+      for (int r = 0; r < MR; ++r)
+        kv_load_q<D>(p, seq, s, h, m0 + (mw * MR + r) * 16, sq + (mw * MR + r) * (D / 16) * 32, sf + (mw * MR + r) * 16);
+    int pos[MR][2];
     float o[MR][D / 8][4], m_run[MR][2], l_run[MR][2];
 #pragma unroll
     for (int r = 0; r < MR; ++r) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const unsigned m = m0 + (mw * MR + r) * 16 + 8 * e + g;
+        const int row = seq.start + static_cast<int>(m / G);
+        pos[r][e] = m < M && row < seq.len ? row : -1;
+      }
 #pragma unroll
       for (int t = 0; t < D / 8; ++t)
 #pragma unroll
@@ -162,16 +187,6 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
       m_run[r][0] = m_run[r][1] = -INFINITY;
       l_run[r][0] = l_run[r][1] = 0.f;
     }
-    KvMeta meta = kv_meta<true>(c, s, h, lane < steps, base_of(lane)), next{};
-    Step<D, kKeep> buf[2];
-    const auto fetch = [&](int n, const KvMeta& from, Step<D, kKeep>& to) {
-      const int page = __shfl_sync(0xffffffffu, from.page, n & 31);
-      if (page < 0) return;
-      const int64_t row = base_of(n) & (c.T - 1);
-      kv_load_k<D, kKeep>(kc + page * page_codes, row, to.k);
-      to.v.load(vc + page * page_codes, row);
-    };
-    if (steps > 0) fetch(0, meta, buf[0]);
     __syncthreads();  // the query operands
     float qf[MR][2];
 #pragma unroll
@@ -181,7 +196,8 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
     }
     const uint4* q = sq + mw * MR * (D / 16) * 32 + lane;
 
-    const auto compute = [&](int n, Step<D, kKeep>& b) {
+    const auto compute = [&](int n) {
+      const uint4* b = ring + n % STAGES * L::kStep;
       const int page = __shfl_sync(0xffffffffu, meta.page, n & 31);
       const float ks = __shfl_sync(0xffffffffu, meta.ks, n & 31);
       const float vlog = __shfl_sync(0xffffffffu, meta.vlog, n & 31);
@@ -190,6 +206,7 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
       if (page < 0 || j0 > mine.last) return;
       // logits of 16 positions, in units of log 2, with the value scale's logarithm added
       float x[MR][2][4];
+      uint4 kw[2];
 #pragma unroll
       for (int r = 0; r < MR; ++r)
 #pragma unroll
@@ -198,9 +215,12 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
           for (int e = 0; e < 4; ++e) x[r][t][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
+        if ((kk & 3) == 0)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) kw[t] = b[(t * (D / 64) + (kk >> 2)) * 32 + lane];
         uint32_t b0[2], b1[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) codes_to_half<FMT>(word_of(b.k[t][kk >> 2], kk & 3), b0[t], b1[t]);
+        for (int t = 0; t < 2; ++t) codes_to_half<FMT>(word_of(kw[t], kk & 3), b0[t], b1[t]);
 #pragma unroll
         for (int r = 0; r < MR; ++r) {
           const uint4 a = q[(r * (D / 16) + kk) * 32];
@@ -224,14 +244,6 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (!kv_sees(p.mask, pos[r][e >> 1], j0 + 8 * t + 2 * q4 + (e & 1))) x[r][t][e] = -INFINITY;
-        if constexpr (FMT == kKvE4m3) {
-          // what no row of the warp sees may be a NaN code
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = j0 + (i >> 1) * 8 + 2 * q4 + (i & 1);
-            if (j > mine.last || (p.mask.window && j <= mine.first - p.mask.window && j >= p.mask.sinks)) b.v.clear(i);
-          }
-        }
       }
       uint4 a[MR];
 #pragma unroll
@@ -271,19 +283,31 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
         a[r] = make_uint4(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1),
                           *reinterpret_cast<const uint32_t*>(&h2), *reinterpret_cast<const uint32_t*>(&h3));
       }
+      VCodes<D> v;
+      v.load(b);
+      if (FMT == kKvE4m3 && !whole) {
+        // what no row of the warp sees may be a NaN code
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = j0 + (i >> 1) * 8 + 2 * q4 + (i & 1);
+          if (j > mine.last || (p.mask.window && j <= mine.first - p.mask.window && j >= p.mask.sinks))
+#pragma unroll
+            for (int wd = 0; wd < D / 32; ++wd) v.w[i][wd] = 0;
+        }
+      }
       // values: column g of tile t is value (D / 8) g + t; a word holds 4 tiles of one position
 #pragma unroll
       for (int wd = 0; wd < D / 32; ++wd) {
         uint32_t b0[4], b1[4];
         {
-          const uint32_t lo = prmt(b.v.word(0, wd), b.v.word(1, wd), 0x5140u);
-          const uint32_t hi = prmt(b.v.word(0, wd), b.v.word(1, wd), 0x7362u);
+          const uint32_t lo = prmt(v.w[0][wd], v.w[1][wd], 0x5140u);
+          const uint32_t hi = prmt(v.w[0][wd], v.w[1][wd], 0x7362u);
           codes_to_half<FMT>(lo, b0[0], b0[1]);
           codes_to_half<FMT>(hi, b0[2], b0[3]);
         }
         {
-          const uint32_t lo = prmt(b.v.word(2, wd), b.v.word(3, wd), 0x5140u);
-          const uint32_t hi = prmt(b.v.word(2, wd), b.v.word(3, wd), 0x7362u);
+          const uint32_t lo = prmt(v.w[2][wd], v.w[3][wd], 0x5140u);
+          const uint32_t hi = prmt(v.w[2][wd], v.w[3][wd], 0x7362u);
           codes_to_half<FMT>(lo, b1[0], b1[1]);
           codes_to_half<FMT>(hi, b1[2], b1[3]);
         }
@@ -294,17 +318,18 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
       }
     };
     for (int n = 0; n < steps; ++n) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (half == 1 && ++n >= steps) break;
-        if ((n & 31) == 0) {
-          if (n > 0) meta = next;
-          next = kv_meta<true>(c, s, h, n + 32 + lane < steps, base_of(min(n + 32 + lane, steps)));
-        }
-        if (n + 1 < steps) fetch(n + 1, ((n + 1) & 31) == 0 ? next : meta, buf[half ^ 1]);
-        compute(n, buf[half]);
+      if ((n & 31) == 0) {
+        if (n > 0) meta = next;
+        next = kv_pages(c, s, n + 32 + lane < steps, base_of(min(n + 32 + lane, steps)));
       }
+      if ((n & 31) == 16) kv_scales<true>(c, h, next);
+      const int ahead = n + STAGES - 1;
+      const int page = __shfl_sync(0xffffffffu, (ahead ^ n) < 32 ? meta.page : next.page, ahead & 31);
+      fetch(ahead, ahead < steps ? page : -1);
+      cp_async_wait<STAGES - 1>();
+      compute(n);
     }
+    cp_async_wait<0>();
 
     // ---- join the TW warps of each row
 #pragma unroll
@@ -349,14 +374,15 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
     const bool item = i0 == 0 && i1 == span.n;
     const int slot = 2 * blockIdx.x + (i0 == 0);
     if (!item && i0 == 0 && tid == 0) {
-      const int64_t last = (at + span.n - 1) / share.per;
-      w.split[by_item ? pair * c.heads + h : blockIdx.x] =
-          Split{s, mb, h, static_cast<int>(blockIdx.x), static_cast<int>(last - blockIdx.x) + 1};
+      const int parts = share.cross ? static_cast<int>((at + span.n - 1) / share.per) - static_cast<int>(blockIdx.x) + 1
+                                    : static_cast<int>((span.n + share.per - 1) / share.per);
+      w.split[by_item ? static_cast<int64_t>(pair) * c.heads + h : blockIdx.x] =
+          Split{s, mb, h, static_cast<int>(blockIdx.x), parts};
     }
-    if (item && by_item && tid == 0) w.split[pair * c.heads + h].parts = 0;
+    if (item && by_item && tid == 0) w.split[static_cast<int64_t>(pair) * c.heads + h].parts = 0;
     for (int e = tid; e < L::kRows * (D / 8); e += L::kThreads) {
       const int row = e / (D / 8), f = 2 * (e % (D / 8));
-      const int64_t m = m0 + row;
+      const unsigned m = m0 + row;
       if (m >= M) break;
       float top = sm[row];
 #pragma unroll
@@ -378,7 +404,8 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
       }
       if (item) {
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        const int64_t out = (static_cast<int64_t>(s) * p.rows.R + m / p.G) * p.Hq + h * p.G + m % p.G;
+        const unsigned r = m / G;
+        const int64_t out = (static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * G + (m - r * G);
         uint4 u;
         __nv_bfloat162 y0 = __floats2bfloat162_rn(v[0].x * inv, v[0].y * inv);
         __nv_bfloat162 y1 = __floats2bfloat162_rn(v[0].z * inv, v[0].w * inv);
@@ -398,6 +425,7 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
       }
     }
     __syncthreads();  // the next segment writes the shared buffers
+    left -= i1 - i0;
     at += i1 - i0;
     off += i1 - i0;
     if (off == static_cast<int64_t>(span.n) * c.heads) {
@@ -488,11 +516,11 @@ Plan plan_of(int64_t M) {
   return Plan{128, 2, 1};
 }
 
-template <int D, int FMT, int MR, int MW, int TW, int CPS>
+template <int D, int FMT, int MR, int MW, int TW, int STAGES, int CPS>
 cudaError_t launch(const KvAttnParams& p, const Work& w, unsigned blocks, const LaunchCfg& cfg) {
-  using L = Tile<D, MR, MW, TW>;
+  using L = Tile<D, MR, MW, TW, STAGES>;
   static SmemOptIn opt;
-  auto kern = kv_attention_kernel<D, FMT, MR, MW, TW, CPS>;
+  auto kern = kv_attention_kernel<D, FMT, MR, MW, TW, STAGES, CPS>;
   const cudaError_t e = allow_smem(kern, L::kSmem, opt);
   if (e != cudaSuccess) return e;
   return launch_kernel(kern, dim3(blocks), dim3(L::kThreads), L::kSmem, cfg, p, w);
@@ -501,10 +529,10 @@ cudaError_t launch(const KvAttnParams& p, const Work& w, unsigned blocks, const 
 template <int D, int FMT>
 cudaError_t launch_rows(const KvAttnParams& p, const Work& w, int rows, unsigned blocks, const LaunchCfg& cfg) {
   switch (rows) {
-    case 16: return launch<D, FMT, 1, 1, 4, 3>(p, w, blocks, cfg);
-    case 32: return launch<D, FMT, 2, 1, 8, 1>(p, w, blocks, cfg);
-    case 64: return launch<D, FMT, 2, 2, 4, 1>(p, w, blocks, cfg);
-    default: return launch<D, FMT, 2, 4, 2, 1>(p, w, blocks, cfg);
+    case 16: return launch<D, FMT, 1, 1, 4, 4, 3>(p, w, blocks, cfg);
+    case 32: return launch<D, FMT, 2, 1, 8, 4, 1>(p, w, blocks, cfg);
+    case 64: return launch<D, FMT, 2, 2, 4, 4, 1>(p, w, blocks, cfg);
+    default: return launch<D, FMT, 2, 4, 2, 4, 1>(p, w, blocks, cfg);
   }
 }
 
@@ -522,7 +550,7 @@ cudaError_t launch_kv_attention(const KvAttnParams& p, void* workspace, const La
   const int64_t M = static_cast<int64_t>(p.rows.R) * p.G;
   const Plan t = plan_of(M);
   const int64_t row_blocks = (M + t.rows - 1) / t.rows, items = p.c.S * row_blocks * p.c.heads;
-  if (p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (M > 0x7fffffff || p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   // no more blocks than the longest sequences could fill
   const int64_t steps = std::max<int64_t>(items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16), 1);
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(cfg.sms) * t.per_sm, (steps + t.tw - 1) / t.tw);

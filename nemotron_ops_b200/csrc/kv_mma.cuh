@@ -16,20 +16,21 @@ namespace bolt {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// The rows m0 .. m0 + rows - 1 of a sequence (row m = r * G + head of the group) and the steps that
-// they see: `sink` steps from position 0 on, then the steps lo ..; `n` in all.
+// The rows m0 .. m0 + rows - 1 of a sequence (row m = r * G + head of the group; R * G < 2^31) and the
+// steps that they see: `sink` steps from position 0 on, then the steps lo ..; `n` in all.
 struct KvSpan {
   int first, last;  // positions of the first and the last row that exist; last < first: none
   int sink, lo, n;
   __device__ __forceinline__ int base(int i) const { return (i < sink ? i : lo + i - sink) << 4; }
 };
 
-__device__ __forceinline__ KvSpan kv_span(const KvAttnParams& p, const KvSeq& q, int64_t m0, int rows) {
-  const int r0 = static_cast<int>(m0 / p.G);
-  const int64_t r1 = min((m0 + rows - 1) / p.G, static_cast<int64_t>(p.rows.R) - 1);
+__device__ __forceinline__ KvSpan kv_span(const KvAttnParams& p, const KvSeq& q, unsigned m0, unsigned rows) {
+  const unsigned G = p.G, most = static_cast<unsigned>(p.rows.R) - 1;
+  const unsigned r0 = m0 / G, r1 = min((m0 + rows - 1) / G, most);
   KvSpan t;
-  t.first = static_cast<int>(min(static_cast<int64_t>(q.start) + r0, static_cast<int64_t>(q.len)));
-  t.last = static_cast<int>(min(q.start + r1, static_cast<int64_t>(q.len) - 1));
+  // start <= 2^30 and R <= 2^30
+  t.first = min(q.start + static_cast<int>(min(r0, most + 1)), q.len);
+  t.last = min(q.start + static_cast<int>(r1), q.len - 1);
   t.sink = t.lo = t.n = 0;
   if (t.last < t.first) return t;
   if (p.mask.window) {
@@ -40,79 +41,113 @@ __device__ __forceinline__ KvSpan kv_span(const KvAttnParams& p, const KvSeq& q,
   return t;
 }
 
-// The blocks share the steps of all (sequence, row block, head) items evenly: the items lie one after
-// another on one axis (head fastest within a (sequence, row block) pair), and block i takes the i-th
-// piece of `per` steps of it.  Lengths are only known on the device, so every block adds them up itself.
+// a / b of non-negative numbers; 64-bit division costs several times the 32-bit one's instructions
+__device__ __forceinline__ int64_t kv_div(int64_t a, int b) {
+  if (a <= 0xFFFFFFFFll) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// The blocks share the steps of all (sequence, row block, head) items evenly.  The items lie one after
+// another on one axis (head fastest within a (sequence, row block) pair), and each block takes a piece
+// of `per` consecutive steps of it.  Where there are few items (at most a quarter of the blocks), pieces
+// do not cross from one item to the next: a piece of two items costs its block a second set-up, which
+// takes longer than the few steps that the last pieces of the items leave idle.  Lengths are only known
+// on the device, so every block adds them up itself.
 struct KvShare {
-  int64_t total;  // steps on the axis
-  int64_t per;    // steps of a block
-  int64_t off;    // of this block's first step within its pair
-  int pair;       // of this block's first step
+  int64_t per;   // steps of a piece
+  int64_t left;  // steps of this block's piece, from here on:
+  int64_t off;   // of its first step within its pair
+  int64_t at;    // of its first step on the axis (pieces that cross items)
+  int pair;
+  bool cross;
 };
 
 template <int THREADS>
-__device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_blocks, int block_rows, int round) {
-  __shared__ int64_t s_sum[THREADS / 32];
-  __shared__ int64_t s_off;
+__device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_blocks, unsigned block_rows, int round) {
+  __shared__ int64_t s_sum[THREADS / 32], s_off;
   __shared__ int s_pair;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t pairs = static_cast<int64_t>(p.c.S) * row_blocks, q = (pairs + THREADS - 1) / THREADS;
-  const auto steps = [&](int64_t i) -> int64_t {
-    const int s = static_cast<int>(i / row_blocks);
-    const int64_t m0 = (i % row_blocks) * block_rows;
-    return static_cast<int64_t>(kv_span(p, kv_seq(p.c, p.rows.start, p.rows.lens, s), m0, block_rows).n) * p.c.heads;
+  const unsigned pairs = static_cast<unsigned>(p.c.S) * row_blocks, q = (pairs + THREADS - 1) / THREADS;
+  const auto steps = [&](unsigned i) -> int {
+    const unsigned s = row_blocks == 1 ? i : i / row_blocks, m0 = (i - s * row_blocks) * block_rows;
+    return kv_span(p, kv_seq(p.c, p.rows.start, p.rows.lens, s), m0, block_rows).n;
   };
-  const int64_t i0 = min(tid * q, pairs), i1 = min(i0 + q, pairs);
-  int64_t mine = 0;
-  for (int64_t i = i0; i < i1; ++i) mine += steps(i);
-  int64_t pre = mine;
+  const unsigned i0 = min(tid * q, pairs), i1 = min(i0 + q, pairs);
+  // the sum over this thread's pairs, the sum over those of the threads before it, and over all
+  const auto scan = [&](auto&& of, int64_t& mine, int64_t& before, int64_t& all) {
+    mine = 0;
+    for (unsigned i = i0; i < i1; ++i) mine += of(i);
+    int64_t pre = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, pre, o);
-    if (lane >= o) pre += up;
-  }
-  if (lane == 31) s_sum[warp] = pre;
-  __syncthreads();
-  KvShare w{0, 0, 0, 0};
-  int64_t before = 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += up;
+    }
+    __syncthreads();  // s_sum may hold another scan's
+    if (lane == 31) s_sum[warp] = pre;
+    __syncthreads();
+    before = pre - mine;
+    all = 0;
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) {
-    if (i < warp) before += s_sum[i];
-    w.total += s_sum[i];
-  }
-  pre += before - mine;
-  w.per = (w.total + gridDim.x - 1) / gridDim.x;
-  w.per = max((w.per + round - 1) / round, static_cast<int64_t>(1)) * round;
-  const int64_t a = blockIdx.x * w.per;
-  if (mine > 0 && a >= pre && a < pre + mine) {
-    int64_t i = i0, n;
-    while (a >= pre + (n = steps(i))) {
-      pre += n;
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < warp) before += s_sum[i];
+      all += s_sum[i];
+    }
+  };
+  int64_t mine, before, total;
+  scan([&](unsigned i) { return static_cast<int64_t>(steps(i)) * p.c.heads; }, mine, before, total);
+  const int64_t items = static_cast<int64_t>(pairs) * p.c.heads;
+  const int blocks = static_cast<int>(gridDim.x);
+  KvShare w{0, 0, 0, 0, 0, items * 4 > blocks};
+  if (total == 0) return w;
+  const int pieces = w.cross ? blocks : blocks - static_cast<int>(items);  // each item may leave a piece unfilled
+  w.per = kv_div(total + pieces - 1, pieces);
+  w.per = kv_div(w.per + round - 1, round) * round;
+  // this block's place: on the axis, or among the pieces
+  w.at = w.cross ? blockIdx.x * w.per : blockIdx.x;
+  const auto pieces_of = [&](unsigned i) { return kv_div(steps(i) + w.per - 1, static_cast<int>(w.per)) * p.c.heads; };
+  if (!w.cross) scan([&](unsigned i) { return pieces_of(i); }, mine, before, total);
+  if (w.at >= total) return w;
+  if (w.at >= before && w.at < before + mine) {
+    unsigned i = i0;
+    int64_t n;
+    while (w.at >= before + (n = w.cross ? static_cast<int64_t>(steps(i)) * p.c.heads : pieces_of(i))) {
+      before += n;
       ++i;
     }
     s_pair = static_cast<int>(i);
-    s_off = a - pre;
+    s_off = w.at - before;
   }
   __syncthreads();
   w.pair = s_pair;
   w.off = s_off;
+  if (w.cross) {
+    w.left = min(w.per, total - w.at);
+  } else {
+    const int n = steps(w.pair), parts = static_cast<int>(kv_div(n + w.per - 1, static_cast<int>(w.per)));
+    const int h = static_cast<int>(w.off) / parts, part = static_cast<int>(w.off) % parts;
+    w.off = static_cast<int64_t>(h) * n + part * w.per;
+    w.left = min(w.per, n - part * w.per);
+  }
   return w;
 }
 
-// Page and scales of 32 of a warp's steps, one a lane.
-struct KvMeta {
+// Page and scales of 32 of a warp's steps, one a lane.  The pages come first: the copies of the codes
+// wait for them alone.
+struct KvPages {
   int page;
   float ks, vlog, vinv;
 };
 
+__device__ __forceinline__ KvPages kv_pages(const KvCache& c, int s, bool live, int base) {
+  return KvPages{live ? kv_page(c.table, c.width, c.pages, s, base >> c.tshift) : -1, 0.f, 0.f, 0.f};
+}
+
 // The value scale enters the logits as a power of two (vlog), so that the weights of every page share
 // one reference whatever its scale; a scale of 0 (a page of zeros) is taken as 2^-96.
 template <bool V>
-__device__ __forceinline__ KvMeta kv_meta(const KvCache& c, int s, int h, bool live, int base) {
-  KvMeta m{-1, 0.f, 0.f, 0.f};
-  if (!live) return m;
-  m.page = kv_page(c.table, c.width, c.pages, s, base >> c.tshift);
-  if (m.page < 0) return m;
+__device__ __forceinline__ void kv_scales(const KvCache& c, int h, KvPages& m) {
+  if (m.page < 0) return;
   const int64_t unit = static_cast<int64_t>(m.page) * c.heads + h;
   m.ks = c.ks[unit];
   if constexpr (V) {
@@ -120,7 +155,6 @@ __device__ __forceinline__ KvMeta kv_meta(const KvCache& c, int s, int h, bool l
     m.vlog = log2f(vs);
     m.vinv = 1.f / vs;
   }
-  return m;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -129,25 +163,25 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Plain loads: an earlier kernel of the stream may have written the codes while this one was starting.
-template <bool KEEP>
+// Asynchronous copies to shared memory, and plain loads: an earlier kernel of the stream may have written
+// the codes while this one was starting.
+__device__ __forceinline__ void cp_async16(void* dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(void* dst, const uint8_t* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 __device__ __forceinline__ uint4 ld128(const uint8_t* p) {
   uint4 v;
-  if constexpr (KEEP)
-    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  else
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-  return v;
-}
-template <bool KEEP>
-__device__ __forceinline__ uint2 ld64(const uint8_t* p) {
-  uint2 v;
-  if constexpr (KEEP)
-    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  else
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
   return v;
 }
 
@@ -181,15 +215,15 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t
 // rows' logit factors (the power of two taken out, times scale * log2 e) to `sf`.  Rows that do not
 // exist are 0.
 template <int D>
-__device__ __forceinline__ void kv_load_q(const KvAttnParams& p, const KvSeq& seq, int s, int h, int64_t m0, uint4* sq,
+__device__ __forceinline__ void kv_load_q(const KvAttnParams& p, const KvSeq& seq, int s, int h, unsigned m0, uint4* sq,
                                           float* sf) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   uint32_t half[2][D / 64][8];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const int64_t m = m0 + g + 8 * e;
-    const int64_t r = m / p.G;
-    const bool live = r < p.rows.R && seq.start + r < seq.len;
+    const unsigned m = m0 + g + 8 * e, r = m / static_cast<unsigned>(p.G);
+    const bool live = r < static_cast<unsigned>(p.rows.R) && seq.start + static_cast<int>(r) < seq.len;
+    const bf16* from = p.q + s * p.qs + r * p.qr + (h * static_cast<int64_t>(p.G) + (m - r * p.G)) * D + 16 * c;
     uint4 raw[D / 64][2];
     float amax = 0.f;
 #pragma unroll
@@ -198,8 +232,7 @@ __device__ __forceinline__ void kv_load_q(const KvAttnParams& p, const KvSeq& se
       for (int k = 0; k < 2; ++k) {
         raw[i][k] = make_uint4(0, 0, 0, 0);
         if (live)
-          raw[i][k] = *reinterpret_cast<const uint4*>(p.q + s * p.qs + r * p.qr + (h * p.G + m % p.G) * D + 64 * i +
-                                                      16 * c + 8 * k);
+          raw[i][k] = *reinterpret_cast<const uint4*>(from + 64 * i + 8 * k);
         const uint32_t w[4] = {raw[i][k].x, raw[i][k].y, raw[i][k].z, raw[i][k].w};
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -231,16 +264,6 @@ __device__ __forceinline__ void kv_load_q(const KvAttnParams& p, const KvSeq& se
     for (int w = 0; w < 4; ++w)
       sq[(4 * i + w) * 32 + lane] =
           make_uint4(half[0][i][2 * w], half[1][i][2 * w], half[0][i][2 * w + 1], half[1][i][2 * w + 1]);
-}
-
-// A step's K codes: lane (g, c) holds the codes 64 i + 16 c .. + 15 of the positions g and 8 + g.
-template <int D, bool KEEP>
-__device__ __forceinline__ void kv_load_k(const uint8_t* k, int64_t at, uint4 (&raw)[2][D / 64]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) raw[t][i] = ld128<KEEP>(k + (at + 8 * t + g) * D + 64 * i + 16 * c);
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }

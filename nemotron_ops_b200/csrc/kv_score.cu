@@ -23,52 +23,57 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv_score_kernel(const KvAttnPa
   pdl_trigger();
   const KvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
-  const int64_t M = static_cast<int64_t>(p.rows.R) * p.G;
-  const int all = static_cast<int>(min(M, static_cast<int64_t>(0x7fffffff)));
-  const KvShare share = kv_share<kWarps * 32>(p, 1, all, kWarps);
-  const int64_t begin = blockIdx.x * share.per, end = min(begin + share.per, share.total);
-  int64_t s64 = share.pair, off = share.off;
-  for (int64_t at = begin; at < end;) {
-    const int s = static_cast<int>(s64);
+  const unsigned M = static_cast<unsigned>(p.rows.R) * p.G;
+  const KvShare share = kv_share<kWarps * 32>(p, 1, M, kWarps);
+  int64_t left = share.left, off = share.off;
+  for (int s = share.pair; left > 0;) {
     const KvSeq seq = kv_seq(c, p.rows.start, p.rows.lens, s);
-    const KvSpan span = kv_span(p, seq, 0, all);
+    const KvSpan span = kv_span(p, seq, 0, M);
     if (span.n == 0) {
-      ++s64;
+      ++s;
       continue;
     }
-    const int h = static_cast<int>(off / span.n), i0 = static_cast<int>(off % span.n);
-    const int i1 = static_cast<int>(min(static_cast<int64_t>(span.n), i0 + end - at));
+    const int h = static_cast<int>(kv_div(off, span.n)), i0 = static_cast<int>(off - static_cast<int64_t>(h) * span.n);
+    const int i1 = static_cast<int>(min(static_cast<int64_t>(span.n), i0 + left));
     float* score = p.score + (static_cast<int64_t>(s) * c.heads + h) * p.score_width;
     const int steps = max(0, (i1 - i0 - warp + kWarps - 1) / kWarps);
     const auto base_of = [&](int n) { return span.base(i0 + warp + n * kWarps); };
     const uint8_t* kc = c.k + static_cast<int64_t>(h) * c.T * D;
     const int64_t page_codes = static_cast<int64_t>(c.heads) * c.T * D;
-    for (int64_t m0 = 0; m0 < M; m0 += kRowTiles * 16) {
-      const int tiles = static_cast<int>(min((M - m0 + 15) / 16, static_cast<int64_t>(kRowTiles)));
+    for (unsigned m0 = 0; m0 < M; m0 += kRowTiles * 16) {
+      const int tiles = min((M - m0 + 15) / 16, static_cast<unsigned>(kRowTiles));
       const KvSpan chunk = kv_span(p, seq, m0, kRowTiles * 16);
       if (chunk.n == 0) break;  // rows past the sequence's end, here and in every later chunk
       __syncthreads();          // the previous chunk's operands are still read
       for (int t = warp; t < tiles; t += kWarps)
         kv_load_q<D>(p, seq, s, h, m0 + t * 16, sq + t * (D / 16) * 32, sf + t * 16);
       for (int i = tid; i < tiles * 16; i += kWarps * 32) {
-        const int64_t m = m0 + i, r = m / p.G;
-        const bool live = m < M && seq.start + r < seq.len;
-        spos[i] = live ? static_cast<int>(seq.start + r) : -1;
-        sz[i] = live ? p.lse[(static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * p.G + m % p.G] * kLog2e : 0.f;
+        const unsigned m = m0 + i, r = m / static_cast<unsigned>(p.G);
+        const bool live = m < M && seq.start + static_cast<int>(r) < seq.len;
+        spos[i] = live ? seq.start + static_cast<int>(r) : -1;
+        sz[i] = live ? p.lse[(static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * p.G + (m - r * p.G)] * kLog2e : 0.f;
       }
-      KvMeta meta{}, next = kv_meta<false>(c, s, h, lane < steps, base_of(lane));
+      KvPages meta{-1}, next = kv_pages(c, s, lane < steps, base_of(lane));
       uint4 raw[2][D / 64], ahead[2][D / 64];
-      const auto fetch = [&](int n, const KvMeta& from) {
-        const int page = __shfl_sync(0xffffffffu, from.page, n & 31);
-        if (page >= 0) kv_load_k<D, false>(kc + page * page_codes, base_of(n) & (c.T - 1), ahead);
+      const auto fetch = [&](int n, const KvPages& of) {
+        const int page = __shfl_sync(0xffffffffu, of.page, n & 31);
+        if (page < 0) return;
+        // lane (g, q4) takes the codes 64 i + 16 q4 .. + 15 of the positions g and 8 + g
+        const uint8_t* from = kc + page * page_codes + ((base_of(n) & (c.T - 1)) + g) * D + 16 * q4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) ahead[t][i] = ld128(from + 8 * t * D + 64 * i);
       };
       if (steps > 0) fetch(0, next);
       __syncthreads();
       for (int n = 0; n < steps; ++n) {
         if ((n & 31) == 0) {
           meta = next;
-          next = kv_meta<false>(c, s, h, n + 32 + lane < steps, base_of(min(n + 32 + lane, steps)));
+          if (n == 0) kv_scales<false>(c, h, meta);
+          next = kv_pages(c, s, n + 32 + lane < steps, base_of(min(n + 32 + lane, steps)));
         }
+        if ((n & 31) == 16) kv_scales<false>(c, h, next);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -118,10 +123,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv_score_kernel(const KvAttnPa
           }
       }
     }
-    at += i1 - i0;
+    left -= i1 - i0;
     off += i1 - i0;
     if (off == static_cast<int64_t>(span.n) * c.heads) {
-      ++s64;
+      ++s;
       off = 0;
     }
   }
