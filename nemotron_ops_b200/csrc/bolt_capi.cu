@@ -464,7 +464,8 @@ KvCache kv_cache(const std::string& op, const void* k, const int64_t* shape, con
   const int64_t pages = shape[0], heads = shape[1], T = shape[2], D = shape[3], S = table_shape[0], W = table_shape[1];
   need(D == 64 || D == 128, "head size must be 64 or 128");
   need(T >= 16 && T <= 256 && (T & (T - 1)) == 0, "a page must hold 16, 32, 64, 128 or 256 tokens");
-  need(pages >= 0 && pages <= INT32_MAX && heads >= 1 && heads <= 65535, "cache must be [pages, heads, tokens, head size]");
+  need(pages >= 1 && pages <= INT32_MAX && heads >= 1 && heads <= 65535, "cache must be [pages, heads, tokens, head size]");
+  need(pages * heads * T <= INT32_MAX, "cache must have fewer than 2^31 rows (pages * heads * tokens)");
   need(S >= 0 && S <= 65535 && W >= 0 && W * T <= (int64_t(1) << 30), "page table must be [sequences, pages of a sequence]");
   need(fmt == kKvInt8 || fmt == kKvE4m3, "unknown cache format");
   KvCache c{};

@@ -45,6 +45,7 @@ struct KvAttnParams {
   float* lse;               // [S, R, Hq]; KvScore reads it
   float* score;             // [S, heads, score_width] (KvScore)
   int64_t score_width;
+  bool few_steps;           // the 16-position steps of all items are fewer than 2^31 whatever the lengths
 };
 
 cudaError_t launch_kv_append(const KvCache& c, const KvRows& rows, const bf16* k, int64_t k_seq, int64_t k_row,

@@ -13,15 +13,18 @@
 // results do not depend on scheduling.
 //
 // Rounding: logits, maxima, sums and values are fp32; a weight is rounded to fp16 (11 bits) once, as
-// the second product's operand.  Weights are kept as 2^15 times their share of the row's largest, so
-// that those down to 2^-29 of it have all 11 bits.
+// the second product's operand.  A row's weights are 2^(x - m + 8) for its logits x (in units of log 2)
+// and a reference m that is raised to the row's maximum only when some x passes m + 7: weights stay
+// below 2^15, those down to 2^-22 of the reference keep all 11 bits, and most steps need neither the
+// maximum over the row's lanes nor a rescaling.
 #include "kv_mma.cuh"
+#include "tensor_map.h"
 
 namespace bolt {
 
 namespace {
 
-constexpr float kWeightLog = 15.f;
+constexpr float kWeightLog = 8.f, kWeightTop = 15.f;
 
 struct Split {   // segments of one item: the first in block `block`'s slot 2 block + 1, the i-th in 2 (block + i)
   int s, mb, h, block, parts;
@@ -35,59 +38,59 @@ struct Work {
   int row_blocks;
 };
 
-template <int D, int MR, int MW, int TW, int STAGES>
+// NT tiles of 8 rows a warp, MW warps along the rows, TW along the steps; a warp takes NP steps at a
+// time, from a ring of STAGES steps.
+template <int D, int NT, int MW, int TW, int NP, int STAGES>
 struct Tile {
-  static constexpr int kRows = MR * MW * 16, kThreads = MW * TW * 32;
-  static constexpr int kQ = MR * MW * (D / 16) * 32;      // uint4 of query operands
-  static constexpr int kStep = D * 2;                     // uint4 of a warp's step: 16 positions, K and V
-  static constexpr int kRing = MW * TW * STAGES * kStep;  // uint4
-  static constexpr int kJoin = TW * kRows * D / 4;        // uint4, in the ring's place
-  static constexpr size_t kSmem = (kQ + (kRing > kJoin ? kRing : kJoin)) * 16 + kRows * 4 + TW * kRows * 8;
+  static constexpr int kRows = NT * MW * 8, kWarps = MW * TW, kThreads = kWarps * 32;
+  static constexpr int kStep = D * 2;                    // uint4 of a warp's step: 16 positions, K and V
+  static constexpr int kRing = kWarps * STAGES * kStep;  // uint4
+  static constexpr int kJoin = TW * kRows * D / 4;       // uint4, in the ring's place
+  static constexpr bool kQRegs = NT <= 2;                // query operands in registers, else in shared memory
+  static constexpr int kQ = kQRegs ? 0 : MW * NT * (D / 16) * 32;  // uint2
+  static constexpr size_t kSmem = (kRing > kJoin ? kRing : kJoin) * 16 + kQ * 8 + kWarps * (64 * 20 + STAGES * 8) +
+                                  TW * kRows * 8 + 1024;  // the ring starts on a 1,024-byte boundary
 };
 
 // float4 index f of a row's values in the joining buffer, spread over the banks
 template <int D>
 __device__ __forceinline__ int swizzle(int row, int f) {
-  return f ^ ((f >> 3) | ((row & 1) << (D == 128 ? 2 : 1)));
+  const int c = (row >> 1) & 3;
+  return f ^ (D == 128 ? c : (c & 1) | (c >> 1) << 2);
 }
 
-// A warp's step in its ring: every lane copies the bytes that it will use itself, so that no other
-// lane waits for them.  K: lane (g, c) takes the codes 64 i + 16 c .. + 15 of the positions g and 8 + g.
-// V: the codes (D / 8) g .. of the positions 2 c, 2 c + 1, 8 + 2 c and 8 + 2 c + 1.
+// A step's codes lie in the ring as the tensor copy writes them: 16 rows of D bytes of K, then of V, the
+// 16-byte chunks of row r exchanged by XOR with r % 8 (D = 128) or r / 2 % 4 (D = 64).  Row index i of a
+// tile of 8 positions stands for position place<D>(i): with this order the 8 lanes of a shared-memory phase
+// fall into different banks both when they read K (rows i = lane / 4) and V (rows i = 2 (lane % 4) and + 1).
 template <int D>
-__device__ __forceinline__ void copy_step(uint4* to, const uint8_t* k, const uint8_t* v) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) cp_async16(to + (t * (D / 64) + i) * 32 + lane, k + (8 * t + g) * D + 64 * i + 16 * c);
-  to += D / 32 * 32;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint8_t* from = v + ((i >> 1) * 8 + 2 * c + (i & 1)) * D + D / 8 * g;
-    if constexpr (D == 128)
-      cp_async16(to + i * 32 + lane, from);
-    else
-      cp_async8(reinterpret_cast<uint2*>(to) + i * 32 + lane, from);
-  }
+__device__ __forceinline__ int place(int i) {
+  return D == 128 ? i ^ ((i & 1) << 2) : (i & 4) | ((i & 1) << 1) | (((i >> 1) ^ i) & 1);
+}
+
+// An 8 x 8 matrix of halves, two neighbours of a row a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(__half2 x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(*reinterpret_cast<const uint32_t*>(&x)));
+  return y;
 }
 
 template <int D>
 struct VCodes {
   uint32_t w[4][D / 32];  // position, word
-  __device__ __forceinline__ void load(const uint4* from) {
-    const int lane = threadIdx.x & 31;
-    from += D / 32 * 32;
+  // `at`: this lane's places of the positions 2 c and 2 c + 1 in the step's V rows; the others are 8 rows on
+  __device__ __forceinline__ void load(const uint8_t* v, const int (&at)[2]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const uint8_t* from = v + at[i & 1] + (i >> 1) * 8 * D;
       if constexpr (D == 128) {
-        const uint4 x = from[i * 32 + lane];
+        const uint4 x = lds128(from);
         w[i][0] = x.x;
         w[i][1] = x.y;
         w[i][2] = x.z;
         w[i][3] = x.w;
       } else {
-        const uint2 x = reinterpret_cast<const uint2*>(from)[i * 32 + lane];
+        const uint2 x = *reinterpret_cast<const uint2*>(from);
         w[i][0] = x.x;
         w[i][1] = x.y;
       }
@@ -95,25 +98,48 @@ struct VCodes {
   }
 };
 
-template <int D, int FMT, int MR, int MW, int TW, int STAGES, int CPS>
-__global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const KvAttnParams p, const Work w) {
-  using L = Tile<D, MR, MW, TW, STAGES>;
-  extern __shared__ uint4 smem[];
-  uint4* sq = smem;                                                                  // [MW * MR][D / 16][32]
-  float4* so = reinterpret_cast<float4*>(smem + L::kQ);                              // [TW][rows][D / 4]
-  float* sf = reinterpret_cast<float*>(smem + L::kSmem / 16) - L::kRows * (1 + 2 * TW);  // [rows]
-  float* sm = sf + L::kRows;                                                         // [TW][rows]
-  float* sl = sm + TW * L::kRows;                                                    // [TW][rows]
+template <int D, int FMT, int NT, int MW, int TW, int NP, int STAGES, int CPS>
+__global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
+    const KvAttnParams p, const Work w, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  using L = Tile<D, NT, MW, TW, NP, STAGES>;
+  extern __shared__ uint4 smem_raw[];
+  uint4* smem = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float4* so = reinterpret_cast<float4*>(smem);                            // [TW][rows][D / 4]
+  uint4* tail = smem + (L::kRing > L::kJoin ? L::kRing : L::kJoin);
+  uint2* sq = reinterpret_cast<uint2*>(tail);                              // [MW * NT][D / 16][32]
+  float4* s_scale = reinterpret_cast<float4*>(sq + L::kQ);                 // [warps][64]: K scale, log2 and 1 / V scale, position and flags
+  int* s_row = reinterpret_cast<int*>(s_scale + L::kWarps * 64);           // [warps][64]: first row of the codes, or -1
+  uint64_t* s_full = reinterpret_cast<uint64_t*>(s_row + L::kWarps * 64);  // [warps][STAGES]: barriers of the ring
+  float* sm = reinterpret_cast<float*>(s_full + L::kWarps * STAGES);       // [TW][rows]
+  float* sl = sm + TW * L::kRows;                                          // [TW][rows]
   pdl_wait();
   pdl_trigger();
   const KvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
   const int mw = warp % MW, tk = warp / MW;
-  uint4* ring = smem + L::kQ + warp * STAGES * L::kStep;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(smem + warp * STAGES * L::kStep);
   const unsigned M = static_cast<unsigned>(p.rows.R) * p.G, G = p.G;
   const int pairs = c.S * w.row_blocks;
   const bool by_item = static_cast<int64_t>(pairs) * c.heads == w.splits;
-  const KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW);
+  s_scale += warp * 64;
+  s_row += warp * 64;
+  s_full += warp * STAGES;
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(s_full + i), 1);
+    fence_barrier_init();
+    asm volatile("fence.proxy.async;" ::: "memory");
+  }
+  __syncwarp();
+  unsigned taken = 0;   // steps that this warp has put into its ring, of all segments
+  bool stuck = false;   // a copy did not arrive in time: the rest of the work is left
+  const int k_at = place<D>(g) * D + (D == 128 ? q4 ^ (place<D>(g) & 7) : q4 ^ ((place<D>(g) >> 1) & 3)) * 16;
+  int v_at[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = place<D>(2 * q4 + i);
+    v_at[i] = t * D + (D == 128 ? (g ^ t) * 16 : ((g >> 1) ^ ((t >> 1) & 3)) * 16 + (g & 1) * 8);
+  }
+  const KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW * NP);
 
   if (!by_item && tid == 0) w.split[blockIdx.x].parts = 0;
   // items without steps: their rows see nothing
@@ -142,244 +168,314 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
       ++pair;
       continue;
     }
-    const int h = static_cast<int>(kv_div(off, span.n)), i0 = static_cast<int>(off - static_cast<int64_t>(h) * span.n);
-    const int i1 = static_cast<int>(min(static_cast<int64_t>(span.n), i0 + left));
-
-    // ---- the segment: steps i0 .. i1 - 1, this warp's are i0 + tk, + TW, ...
-    const KvSpan mine = kv_span(p, seq, min(m0 + mw * MR * 16, M), MR * 16);
-    const int steps = mine.n > 0 ? max(0, (i1 - i0 - tk + TW - 1) / TW) : 0;
-    const auto base_of = [&](int n) { return span.base(i0 + tk + n * TW); };
-    const uint8_t* kc = c.k + static_cast<int64_t>(h) * c.T * D;
-    const uint8_t* vc = c.v + static_cast<int64_t>(h) * c.T * D;
-    const int64_t page_codes = static_cast<int64_t>(c.heads) * c.T * D;
-    KvPages meta = kv_pages(c, s, lane < steps, base_of(lane)), next{-1};
-    const auto fetch = [&](int n, int page) {  // step n into its slot of the ring; an empty group where there is none
-      if (page >= 0) {
-        const int64_t from = page * page_codes + (base_of(n) & (c.T - 1)) * D;
-        copy_step<D>(ring + n % STAGES * L::kStep, kc + from, vc + from);
-      }
-      cp_async_commit();
-    };
-#pragma unroll
-    for (int n = 0; n < STAGES - 1; ++n) {
-      const int page = __shfl_sync(0xffffffffu, meta.page, n);
-      fetch(n, n < steps ? page : -1);
+    // units u0 .. u1 - 1 of the item, of which those from share.cost on are its steps
+    const int size = span.n + share.cost;
+    const int h = static_cast<int>(kv_div(off, size)), u0 = static_cast<int>(off - static_cast<int64_t>(h) * size);
+    const int u1 = static_cast<int>(min(static_cast<int64_t>(size), u0 + left));
+    const int i0 = max(0, u0 - share.cost), i1 = max(0, u1 - share.cost);
+    const int64_t end = at - u0 + size;  // on the axis, behind this item
+    left -= u1 - u0;
+    at += u1 - u0;
+    off += u1 - u0;
+    const int item_pair = pair;
+    if (off == static_cast<int64_t>(size) * c.heads) {
+      ++pair;
+      off = 0;
     }
-    kv_scales<true>(c, h, meta);
-    if (tk == 0)
+    if (i0 == i1) continue;
+
+    // ---- the segment: steps i0 .. i1 - 1; this warp's k-th is the k % NP-th of the group k / NP * TW + tk
+    const unsigned m1 = m0 + mw * NT * 8;  // this warp's first row
+    const KvSpan mine = kv_span(p, seq, min(m1, M), NT * 8);
+    const int rounds = mine.n > 0 && !stuck ? max(0, (i1 - i0 - tk * NP + TW * NP - 1) / (TW * NP)) : 0;
+    const auto step_of = [&](int k) { return i0 + (k / NP * TW + tk) * NP + k % NP; };
+    uint4 raw_q[NT][D / 64][2];
 #pragma unroll
-      for (int r = 0; r < MR; ++r)
-        kv_load_q<D>(p, seq, s, h, m0 + (mw * MR + r) * 16, sq + (mw * MR + r) * (D / 16) * 32, sf + (mw * MR + r) * 16);
-    int pos[MR][2];
-    float o[MR][D / 8][4], m_run[MR][2], l_run[MR][2];
+    for (int r = 0; r < NT; ++r) kv_fetch_q<D>(p, seq, s, h, m1 + r * 8, raw_q[r]);
+    // offsets and scales of 32 steps, one a lane, made in three stages so that the loads of one are under way
+    // while steps are computed
+    KvPages meta;
+    const auto look_up_page = [&](int k) {
+      const int i = step_of(k);
+      meta.load_page(c, s, k < rounds * NP && i < i1, span.base(min(i, i1 - 1)));
+    };
+    const auto look_up_scales = [&](int k) {
+      meta.check_page(c);
+      meta.load_scales<true>(c, h);
+      s_row[k & 63] = meta.page < 0 ? -1 : (meta.page * c.heads + h) * c.T + (span.base(step_of(k)) & (c.T - 1));
+    };
+    constexpr int kDead = 1, kWhole = 2;  // none of the warp's rows sees the step, or all see all of it
+    const auto keep = [&](int k) {
+      const int j0 = span.base(min(step_of(k), i1 - 1));
+      int flags = 0;
+      if (meta.page < 0 || j0 > mine.last)
+        flags = kDead;
+      else if (j0 + 15 <= mine.first &&
+               (p.mask.window == 0 || j0 > mine.last - p.mask.window || j0 + 15 < p.mask.sinks))
+        flags = kWhole;
+      const float vs = fmaxf(meta.vs, 0x1p-96f);
+      s_scale[k & 63] = make_float4(meta.ks, log2f(vs), 1.f / vs, __int_as_float(j0 | flags));
+    };
+    const auto fetch = [&](int n) {  // round n into its places in the ring
+      __syncwarp();  // which no lane reads any more
+      if (lane != 0 || n >= rounds) return;
 #pragma unroll
-    for (int r = 0; r < MR; ++r) {
+      for (int u = 0; u < NP; ++u) {
+        const unsigned slot = (taken + n * NP + u) % STAGES;
+        const int row = s_row[(n * NP + u) & 63];
+        const uint32_t bar = smem_u32(s_full + slot), to = smem_u32(ring + slot * L::kStep * 16);
+        if (row >= 0) {
+          mbar_arrive_expect_tx(bar, 32 * D);
+          tma_load_3d(to, &map_k, 0, row, 0, bar);
+          tma_load_3d(to + 16 * D, &map_v, 0, row, 0, bar);
+        } else {
+          mbar_arrive(bar);
+        }
+      }
+    };
+    constexpr int kAhead = STAGES / NP - 1;
+    look_up_page(lane);
+    look_up_scales(lane);
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) fetch(n);
+    keep(lane);
+    uint2 q[L::kQRegs ? NT : 1][D / 16];
+    float qf[NT][2], qt[NT][2];  // of the rows 2 q4 and 2 q4 + 1 of each tile, as all that follow
+    int pos[NT][2];
+    float o[NT][D / 16][4], l_run[NT][2];
+    float m_ref[NT][2], m_top[NT][2];  // the reference m - 8, and how far a logit may pass it: not at all until there is one
+#pragma unroll
+    for (int r = 0; r < NT; ++r) {
+      float f, t;
+      kv_make_q<D, FMT>(p, raw_q[r], q[L::kQRegs ? r : 0], f, t);
+      if (!L::kQRegs && tk == 0)
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) sq[((mw * NT + r) * (D / 16) + kk) * 32 + lane] = q[0][kk];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const unsigned m = m0 + (mw * MR + r) * 16 + 8 * e + g;
+        qf[r][e] = __shfl_sync(0xffffffffu, f, (2 * q4 + e) * 4);
+        qt[r][e] = __shfl_sync(0xffffffffu, t, (2 * q4 + e) * 4);
+        const unsigned m = m1 + r * 8 + 2 * q4 + e;
         const int row = seq.start + static_cast<int>(m / G);
         pos[r][e] = m < M && row < seq.len ? row : -1;
+        m_ref[r][e] = 0.f;
+        m_top[r][e] = -INFINITY;
+        l_run[r][e] = 0.f;
       }
 #pragma unroll
-      for (int t = 0; t < D / 8; ++t)
+      for (int t2 = 0; t2 < D / 16; ++t2)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[r][t][x] = 0.f;
-      m_run[r][0] = m_run[r][1] = -INFINITY;
-      l_run[r][0] = l_run[r][1] = 0.f;
+        for (int x = 0; x < 4; ++x) o[r][t2][x] = 0.f;
     }
-    __syncthreads();  // the query operands
-    float qf[MR][2];
-#pragma unroll
-    for (int r = 0; r < MR; ++r) {
-      qf[r][0] = sf[(mw * MR + r) * 16 + g];
-      qf[r][1] = sf[(mw * MR + r) * 16 + 8 + g];
-    }
-    const uint4* q = sq + mw * MR * (D / 16) * 32 + lane;
+    if constexpr (L::kQRegs)
+      __syncwarp();
+    else
+      __syncthreads();
+    const auto q_of = [&](int r, int kk) {
+      return L::kQRegs ? q[L::kQRegs ? r : 0][kk] : sq[((mw * NT + r) * (D / 16) + kk) * 32 + lane];
+    };
 
-    const auto compute = [&](int n) {
-      const uint4* b = ring + n % STAGES * L::kStep;
-      const int page = __shfl_sync(0xffffffffu, meta.page, n & 31);
-      const float ks = __shfl_sync(0xffffffffu, meta.ks, n & 31);
-      const float vlog = __shfl_sync(0xffffffffu, meta.vlog, n & 31);
-      const float vinv = __shfl_sync(0xffffffffu, meta.vinv, n & 31);
-      const int j0 = base_of(n);
-      if (page < 0 || j0 > mine.last) return;
-      // logits of 16 positions, in units of log 2, with the value scale's logarithm added
-      float x[MR][2][4];
-      uint4 kw[2];
+    for (int n = 0; n < rounds; ++n) {
+      const int k0 = n * NP;
+      if ((k0 & 7) == 0) {
+        const int later = (k0 & ~31) + 32 + lane;
+        __syncwarp();  // no lane reads the entries of 32 steps ago any more
+        if ((k0 & 31) == 0) look_up_page(later);
+        if ((k0 & 31) == 8) look_up_scales(later);
+        if ((k0 & 31) == 16) keep(later);
+        __syncwarp();
+      }
+      fetch(n + kAhead);
 #pragma unroll
-      for (int r = 0; r < MR; ++r)
+      for (int u = 0; u < NP; ++u) {
+        const unsigned i = taken + k0 + u;
+        stuck |= !mbar_wait(smem_u32(s_full + i % STAGES), (i / STAGES) & 1, kStatusFullWait);
+      }
+      if (__any_sync(0xffffffffu, stuck)) {
+        // wait, within limits, for what else is on its way into the ring
+        for (int k = k0; k < min(n + kAhead + 1, rounds) * NP; ++k)
+          mbar_wait(smem_u32(s_full + (taken + k) % STAGES), ((taken + k) / STAGES) & 1, kStatusDrainWait);
+        stuck = true;
+        break;
+      }
+
+      const uint8_t* b[NP];
+      float4 sc[NP];
+      int j0[NP];
+      int all = kDead | kWhole;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int u = 0; u < NP; ++u) {
+        b[u] = ring + (taken + k0 + u) % STAGES * L::kStep * 16;
+        sc[u] = s_scale[(k0 + u) & 63];
+        j0[u] = __float_as_int(sc[u].w);
+        all &= j0[u];
+      }
+      if (all & kDead) continue;
+      const bool whole = all & kWhole;
+      // logits in units of log 2, with the value scale's logarithm added, less the reference: lane (g, q4) has
+      // the positions place(g) and 8 + place(g) (index 2 i) and the rows 2 q4 and 2 q4 + 1 (index e)
+      float x[NT][NP][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[r][t][e] = 0.f;
+      for (int u = 0; u < NP; ++u)
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        if ((kk & 3) == 0)
+        for (int i = 0; i < D / 64; ++i) {
+          const uint4 lo = lds128(b[u] + (k_at ^ (64 * i))), hi = lds128(b[u] + 8 * D + (k_at ^ (64 * i)));
 #pragma unroll
-          for (int t = 0; t < 2; ++t) kw[t] = b[(t * (D / 64) + (kk >> 2)) * 32 + lane];
-        uint32_t b0[2], b1[2];
+          for (int y = 0; y < 4; ++y) {
+            uint32_t a0, a1, a2, a3;
+            k_to_half<FMT>(word_of(lo, y), a0, a2);
+            k_to_half<FMT>(word_of(hi, y), a1, a3);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) codes_to_half<FMT>(word_of(kw[t], kk & 3), b0[t], b1[t]);
-#pragma unroll
-        for (int r = 0; r < MR; ++r) {
-          const uint4 a = q[(r * (D / 16) + kk) * 32];
-          mma16816(x[r][0], a, b0[0], b1[0]);
-          mma16816(x[r][1], a, b0[1], b1[1]);
+            for (int r = 0; r < NT; ++r) {
+              const uint2 qb = q_of(r, 4 * i + y);
+              if (i + y == 0)
+                mma16816_first(x[r][u], a0, a1, a2, a3, qb.x, qb.y);
+              else
+                mma16816(x[r][u], a0, a1, a2, a3, qb.x, qb.y);
+            }
+          }
         }
-      }
-      const bool whole = j0 + 15 <= mine.first && (p.mask.window == 0 || j0 > mine.last - p.mask.window ||
-                                                   j0 + 15 < p.mask.sinks);
+      bool over = false;
 #pragma unroll
-      for (int r = 0; r < MR; ++r)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[r][t][e] = x[r][t][e] * (qf[r][e >> 1] * ks) + vlog;
-      if (!whole) {
-#pragma unroll
-        for (int r = 0; r < MR; ++r)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!kv_sees(p.mask, pos[r][e >> 1], j0 + 8 * t + 2 * q4 + (e & 1))) x[r][t][e] = -INFINITY;
-      }
-      uint4 a[MR];
-#pragma unroll
-      for (int r = 0; r < MR; ++r) {
-        float top[2], ref[2];
+      for (int r = 0; r < NT; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float y = fmaxf(fmaxf(x[r][0][2 * e], x[r][0][2 * e + 1]), fmaxf(x[r][1][2 * e], x[r][1][2 * e + 1]));
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-          top[e] = fmaxf(m_run[r][e], y);
-          ref[e] = top[e] == -INFINITY ? 0.f : top[e];
-        }
-        if (__any_sync(0xffffffffu, top[0] > m_run[r][0] || top[1] > m_run[r][1])) {
-          const float f0 = ex2(m_run[r][0] - ref[0]), f1 = ex2(m_run[r][1] - ref[1]);
+          float top = -INFINITY;
 #pragma unroll
-          for (int t = 0; t < D / 8; ++t) {
-            o[r][t][0] *= f0;
-            o[r][t][1] *= f0;
-            o[r][t][2] *= f1;
-            o[r][t][3] *= f1;
+          for (int u = 0; u < NP; ++u) {
+            const float f = qf[r][e] * sc[u].x, d = sc[u].y - m_ref[r][e] - qt[r][e] * sc[u].x;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float& z = x[r][u][2 * i + e];
+              z = z * f + d;
+              if (!whole && ((j0[u] & kDead) || !kv_sees(p.mask, pos[r][e], (j0[u] & ~15) + 8 * i + place<D>(g)))) z = -INFINITY;
+              top = fmaxf(top, z);
+            }
           }
-          l_run[r][0] *= f0;
-          l_run[r][1] *= f1;
-          m_run[r][0] = top[0];
-          m_run[r][1] = top[1];
+          over |= top > m_top[r][e];
+        }
+      if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+        for (int r = 0; r < NT; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < NP; ++u) top = fmaxf(top, fmaxf(x[r][u][e], x[r][u][2 + e]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const bool fresh = m_top[r][e] == -INFINITY;
+            // a row that sees nothing new keeps its reference
+            if (top == -INFINITY) continue;
+            const float up = fresh ? top - kWeightLog : fmaxf(0.f, top - kWeightLog), f = fresh ? 0.f : ex2(-up);
+#pragma unroll
+            for (int u = 0; u < NP; ++u) {
+              x[r][u][e] -= up;
+              x[r][u][2 + e] -= up;
+            }
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+              o[r][t][e] *= f;
+              o[r][t][2 + e] *= f;
+            }
+            l_run[r][e] *= f;
+            m_ref[r][e] += up;
+            m_top[r][e] = kWeightTop;
+          }
+      }
+      // weights, as the second product's B operand: positions and rows change places
+      uint32_t w0[NT][NP], w1[NT][NP];
+#pragma unroll
+      for (int r = 0; r < NT; ++r)
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = ex2(x[r][u][e]);
+          l_run[r][0] += (y[0] + y[2]) * sc[u].z;
+          l_run[r][1] += (y[1] + y[3]) * sc[u].z;
+          w0[r][u] = transpose8(__floats2half2_rn(y[0], y[1]));
+          w1[r][u] = transpose8(__floats2half2_rn(y[2], y[3]));
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int u = 0; u < NP; ++u) {
+        VCodes<D> v;
+        v.load(b[u] + 16 * D, v_at);
+        if (!whole) {
+          // weights of 0 must not meet NaN: a step that was not copied, or a stale e4m3 code that no row of the warp sees
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[r][t][e] = ex2(x[r][t][e] - (ref[e >> 1] - kWeightLog));
+          for (int i = 0; i < 4; ++i) {
+            const int j = (j0[u] & ~15) + (i >> 1) * 8 + place<D>(2 * q4 + (i & 1));
+            if ((j0[u] & kDead) || (FMT == kKvE4m3 && (j > mine.last || (p.mask.window && j <= mine.first - p.mask.window &&
+                                                                 j >= p.mask.sinks))))
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          l_run[r][e] += (x[r][0][2 * e] + x[r][0][2 * e + 1] + (x[r][1][2 * e] + x[r][1][2 * e + 1])) * vinv;
-        const __half2 h0 = __floats2half2_rn(x[r][0][0], x[r][0][1]), h1 = __floats2half2_rn(x[r][0][2], x[r][0][3]);
-        const __half2 h2 = __floats2half2_rn(x[r][1][0], x[r][1][1]), h3 = __floats2half2_rn(x[r][1][2], x[r][1][3]);
-        a[r] = make_uint4(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1),
-                          *reinterpret_cast<const uint32_t*>(&h2), *reinterpret_cast<const uint32_t*>(&h3));
-      }
-      VCodes<D> v;
-      v.load(b);
-      if (FMT == kKvE4m3 && !whole) {
-        // what no row of the warp sees may be a NaN code
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = j0 + (i >> 1) * 8 + 2 * q4 + (i & 1);
-          if (j > mine.last || (p.mask.window && j <= mine.first - p.mask.window && j >= p.mask.sinks))
-#pragma unroll
-            for (int wd = 0; wd < D / 32; ++wd) v.w[i][wd] = 0;
+              for (int wd = 0; wd < D / 32; ++wd) v.w[i][wd] = 0;
+          }
         }
-      }
-      // values: column g of tile t is value (D / 8) g + t; a word holds 4 tiles of one position
+        // the value axis: rows g and 8 + g of tile t are the values (D / 8) g + 2 t and + 1.  Lifted int8 codes
+        // are the subnormals 2^-24 code; a second product with -2^-17 takes their offset of 128 off in every step
 #pragma unroll
-      for (int wd = 0; wd < D / 32; ++wd) {
-        uint32_t b0[4], b1[4];
-        {
-          const uint32_t lo = prmt(v.w[0][wd], v.w[1][wd], 0x5140u);
-          const uint32_t hi = prmt(v.w[0][wd], v.w[1][wd], 0x7362u);
-          codes_to_half<FMT>(lo, b0[0], b0[1]);
-          codes_to_half<FMT>(hi, b0[2], b0[3]);
-        }
-        {
-          const uint32_t lo = prmt(v.w[2][wd], v.w[3][wd], 0x5140u);
-          const uint32_t hi = prmt(v.w[2][wd], v.w[3][wd], 0x7362u);
-          codes_to_half<FMT>(lo, b1[0], b1[1]);
-          codes_to_half<FMT>(hi, b1[2], b1[3]);
-        }
+        for (int wd = 0; wd < D / 32; ++wd)
 #pragma unroll
-        for (int x4 = 0; x4 < 4; ++x4)
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t sel = i ? 0x7362u : 0x5140u;
+            uint32_t a0, a1, a2, a3;
+            codes_to_half<FMT>(prmt(v.w[0][wd], v.w[1][wd], sel), a0, a1);
+            codes_to_half<FMT>(prmt(v.w[2][wd], v.w[3][wd], sel), a2, a3);
 #pragma unroll
-          for (int r = 0; r < MR; ++r) mma16816(o[r][4 * wd + x4], a[r], b0[x4], b1[x4]);
+            for (int r = 0; r < NT; ++r) mma16816(o[r][2 * wd + i], a0, a1, a2, a3, w0[r][u], w1[r][u]);
+          }
       }
-    };
-    for (int n = 0; n < steps; ++n) {
-      if ((n & 31) == 0) {
-        if (n > 0) meta = next;
-        next = kv_pages(c, s, n + 32 + lane < steps, base_of(min(n + 32 + lane, steps)));
-      }
-      if ((n & 31) == 16) kv_scales<true>(c, h, next);
-      const int ahead = n + STAGES - 1;
-      const int page = __shfl_sync(0xffffffffu, (ahead ^ n) < 32 ? meta.page : next.page, ahead & 31);
-      fetch(ahead, ahead < steps ? page : -1);
-      cp_async_wait<STAGES - 1>();
-      compute(n);
     }
-    cp_async_wait<0>();
+    taken += rounds * NP;
 
     // ---- join the TW warps of each row
 #pragma unroll
-    for (int r = 0; r < MR; ++r)
+    for (int r = 0; r < NT; ++r)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float l = l_run[r][e];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (pos[r][e] < 0) m_run[r][e] = -INFINITY;  // rows that do not exist
-        if (q4 == 0) {
-          const int row = (mw * MR + r) * 16 + 8 * e + g;
-          sm[tk * L::kRows + row] = m_run[r][e];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        // the maximum's place takes the reference; none for rows that do not exist
+        m_ref[r][e] = pos[r][e] < 0 || m_top[r][e] == -INFINITY ? -INFINITY : m_ref[r][e] + kWeightLog;
+        if (g == 0) {
+          const int row = (mw * NT + r) * 8 + 2 * q4 + e;
+          sm[tk * L::kRows + row] = m_ref[r][e];
           sl[tk * L::kRows + row] = l;
         }
       }
-    __syncthreads();
+    __syncthreads();  // and all rings are idle
 #pragma unroll
-    for (int r = 0; r < MR; ++r)
+    for (int r = 0; r < NT; ++r)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = (mw * MR + r) * 16 + 8 * e + g;
+        const int row = (mw * NT + r) * 8 + 2 * q4 + e;
         float top = sm[row];
 #pragma unroll
         for (int k = 1; k < TW; ++k) top = fmaxf(top, sm[k * L::kRows + row]);
-        const float f = m_run[r][e] == -INFINITY ? 0.f : ex2(m_run[r][e] - top);
+        const float f = m_ref[r][e] == -INFINITY ? 0.f : ex2(m_ref[r][e] - top);
         float4* to = so + (tk * L::kRows + row) * (D / 4);
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int t = 0; t < D / 32; ++t) {
-            float4 v;
-            v.x = o[r][4 * t][2 * e + y] * f;
-            v.y = o[r][4 * t + 1][2 * e + y] * f;
-            v.z = o[r][4 * t + 2][2 * e + y] * f;
-            v.w = o[r][4 * t + 3][2 * e + y] * f;
-            if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-            to[swizzle<D>(row, (D / 32) * (2 * q4 + y) + t)] = v;
-          }
+        for (int t = 0; t < D / 16; t += 2) {
+          float4 v = make_float4(o[r][t][e] * f, o[r][t][2 + e] * f, o[r][t + 1][e] * f, o[r][t + 1][2 + e] * f);
+          if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+          to[swizzle<D>(row, D / 32 * g + t / 2)] = v;
+        }
       }
     __syncthreads();
     const bool item = i0 == 0 && i1 == span.n;
     const int slot = 2 * blockIdx.x + (i0 == 0);
     if (!item && i0 == 0 && tid == 0) {
-      const int parts = share.cross ? static_cast<int>((at + span.n - 1) / share.per) - static_cast<int>(blockIdx.x) + 1
+      const int parts = share.cross ? static_cast<int>((end - 1) / share.per) - static_cast<int>(blockIdx.x) + 1
                                     : static_cast<int>((span.n + share.per - 1) / share.per);
-      w.split[by_item ? static_cast<int64_t>(pair) * c.heads + h : blockIdx.x] =
+      w.split[by_item ? static_cast<int64_t>(item_pair) * c.heads + h : blockIdx.x] =
           Split{s, mb, h, static_cast<int>(blockIdx.x), parts};
     }
-    if (item && by_item && tid == 0) w.split[static_cast<int64_t>(pair) * c.heads + h].parts = 0;
+    if (item && by_item && tid == 0) w.split[static_cast<int64_t>(item_pair) * c.heads + h].parts = 0;
     for (int e = tid; e < L::kRows * (D / 8); e += L::kThreads) {
       const int row = e / (D / 8), f = 2 * (e % (D / 8));
       const unsigned m = m0 + row;
@@ -424,22 +520,16 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(const K
         if (f == 0) w.ml[static_cast<int64_t>(slot) * L::kRows + row] = make_float2(top, l);
       }
     }
-    __syncthreads();  // the next segment writes the shared buffers
-    left -= i1 - i0;
-    at += i1 - i0;
-    off += i1 - i0;
-    if (off == static_cast<int64_t>(span.n) * c.heads) {
-      ++pair;
-      off = 0;
-    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next segment's copies come after these reads and writes
+    __syncthreads();
   }
 }
 
 // Joins the parts of the items that lie in several blocks: WPR warps a row, a lane D / 32 values.
 template <int D, int WPR>
-__global__ void __launch_bounds__(256) kv_combine_kernel(const KvAttnParams p, const Work w, int rows) {
-  constexpr int E = D / 32, RPB = 8 / WPR;
-  __shared__ float s_l[8], s_o[8][D];
+__global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(const KvAttnParams p, const Work w, int rows) {
+  constexpr int E = D / 32, W = WPR > 8 ? WPR : 8, RPB = W / WPR;
+  __shared__ float s_l[W], s_o[W][D];
   pdl_wait();
   pdl_trigger();
   const Split t = w.split[blockIdx.x];
@@ -504,35 +594,43 @@ __global__ void __launch_bounds__(256) kv_combine_kernel(const KvAttnParams p, c
   if (lane == 0) p.lse[out] = l > 0.f ? (top - kWeightLog + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// The tiling for M = R * G rows a kv head: at most 16 rows: one tile whose steps four warps share, three
-// blocks an SM; more: two tiles a warp, so that a converted operand serves both, one block an SM.
+// The tiling for M = R * G rows a kv head.  Up to 16 rows: tiles of 8 or 16 rows whose steps four warps
+// share, several blocks an SM.  More: 32 rows a warp, so that a converted operand serves four tiles, one
+// block an SM.
 struct Plan {
-  int rows, tw, per_sm;
+  int rows, round, per_sm;
 };
 Plan plan_of(int64_t M) {
-  if (M <= 16) return Plan{16, 4, 3};
+  if (M <= 8) return Plan{8, 4, 3};
+  if (M <= 16) return Plan{16, 4, 2};
   if (M <= 32) return Plan{32, 8, 1};
   if (M <= 64) return Plan{64, 4, 1};
   return Plan{128, 2, 1};
 }
 
-template <int D, int FMT, int MR, int MW, int TW, int STAGES, int CPS>
+template <int D, int FMT, int NT, int MW, int TW, int NP, int STAGES, int CPS>
 cudaError_t launch(const KvAttnParams& p, const Work& w, unsigned blocks, const LaunchCfg& cfg) {
-  using L = Tile<D, MR, MW, TW, STAGES>;
+  using L = Tile<D, NT, MW, TW, NP, STAGES>;
   static SmemOptIn opt;
-  auto kern = kv_attention_kernel<D, FMT, MR, MW, TW, STAGES, CPS>;
+  auto kern = kv_attention_kernel<D, FMT, NT, MW, TW, NP, STAGES, CPS>;
   const cudaError_t e = allow_smem(kern, L::kSmem, opt);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kern, dim3(blocks), dim3(L::kThreads), L::kSmem, cfg, p, w);
+  // a step's rows of K and of V, as the ring holds them
+  const int64_t rows = p.c.pages * p.c.heads * p.c.T;
+  CUtensorMap map_k, map_v;
+  if (!encode_row_tile_map(&map_k, p.c.k, rows, D, 1, D, 16) || !encode_row_tile_map(&map_v, p.c.v, rows, D, 1, D, 16))
+    return cudaErrorInvalidValue;
+  return launch_kernel(kern, dim3(blocks), dim3(L::kThreads), L::kSmem, cfg, p, w, map_k, map_v);
 }
 
 template <int D, int FMT>
 cudaError_t launch_rows(const KvAttnParams& p, const Work& w, int rows, unsigned blocks, const LaunchCfg& cfg) {
   switch (rows) {
-    case 16: return launch<D, FMT, 1, 1, 4, 4, 3>(p, w, blocks, cfg);
-    case 32: return launch<D, FMT, 2, 1, 8, 4, 1>(p, w, blocks, cfg);
-    case 64: return launch<D, FMT, 2, 2, 4, 4, 1>(p, w, blocks, cfg);
-    default: return launch<D, FMT, 2, 4, 2, 4, 1>(p, w, blocks, cfg);
+    case 8: return launch<D, FMT, 1, 1, 4, 1, 4, 3>(p, w, blocks, cfg);
+    case 16: return launch<D, FMT, 2, 1, 4, 1, 4, 2>(p, w, blocks, cfg);
+    case 32: return launch<D, FMT, 4, 1, 8, 1, 4, 1>(p, w, blocks, cfg);
+    case 64: return launch<D, FMT, 4, 2, 4, 1, 4, 1>(p, w, blocks, cfg);
+    default: return launch<D, FMT, 4, 4, 2, 1, 4, 1>(p, w, blocks, cfg);
   }
 }
 
@@ -546,14 +644,16 @@ int64_t kv_attention_workspace(int64_t rows, int D, int sms) {
   return align16(blocks * 2 * t.rows * D * 4) + align16(blocks * 2 * t.rows * 8) + blocks * static_cast<int64_t>(sizeof(Split));
 }
 
-cudaError_t launch_kv_attention(const KvAttnParams& p, void* workspace, const LaunchCfg& cfg) {
+cudaError_t launch_kv_attention(const KvAttnParams& params, void* workspace, const LaunchCfg& cfg) {
+  KvAttnParams p = params;
   const int64_t M = static_cast<int64_t>(p.rows.R) * p.G;
   const Plan t = plan_of(M);
   const int64_t row_blocks = (M + t.rows - 1) / t.rows, items = p.c.S * row_blocks * p.c.heads;
   if (M > 0x7fffffff || p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  p.few_steps = items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16 + kItemCost) <= 0x7fffffff;
   // no more blocks than the longest sequences could fill
   const int64_t steps = std::max<int64_t>(items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16), 1);
-  const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(cfg.sms) * t.per_sm, (steps + t.tw - 1) / t.tw);
+  const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(cfg.sms) * t.per_sm, (steps + t.round - 1) / t.round);
   Work w{};
   w.row_blocks = static_cast<int>(row_blocks);
   w.splits = static_cast<int>(std::min(items, blocks));
@@ -571,12 +671,12 @@ cudaError_t launch_kv_attention(const KvAttnParams& p, void* workspace, const La
   LaunchCfg c2 = cfg;
   c2.pdl = true;  // same op: the kernel waits for its predecessor with griddepcontrol.wait
   const int64_t rows = std::min<int64_t>(M, t.rows);
-  // few rows to join: eight warps a row, since each may have many parts
-  const bool few = w.splits * rows <= 8 * cfg.sms;
+  // few rows to join: 32 warps a row, since each may have many parts
+  const bool few = w.splits * rows <= 2 * cfg.sms;
   const dim3 grid(static_cast<unsigned>(w.splits), static_cast<unsigned>(few ? rows : (rows + 7) / 8));
-  auto kern = p.c.D == 128 ? (few ? kv_combine_kernel<128, 8> : kv_combine_kernel<128, 1>)
-                           : (few ? kv_combine_kernel<64, 8> : kv_combine_kernel<64, 1>);
-  return launch_kernel(kern, grid, dim3(256), 0, c2, p, w, t.rows);
+  auto kern = p.c.D == 128 ? (few ? kv_combine_kernel<128, 32> : kv_combine_kernel<128, 1>)
+                           : (few ? kv_combine_kernel<64, 32> : kv_combine_kernel<64, 1>);
+  return launch_kernel(kern, grid, dim3(few ? 1024 : 256), 0, c2, p, w, t.rows);
 }
 
 }  // namespace bolt

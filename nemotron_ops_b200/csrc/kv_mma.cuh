@@ -2,11 +2,12 @@
 // codes as matrix-unit operands.
 //
 // Both read the cache in steps of 16 positions (16-position steps never straddle a page).  A step's
-// codes go from global memory to the registers of one warp and become fp16 operands of
-// mma.m16n8k16 there: fp16 holds every int8 and e4m3 value exactly, and a permutation of the
-// contraction index, applied to both operands, lets every lane load 16 consecutive bytes.  Query rows
-// are scaled by a power of two into fp16's range (their 8 significant bits fit) and the power goes
-// into the row's logit factor.
+// codes go to the registers of one warp and become fp16 operands of mma.m16n8k16 there, with the
+// positions (for logits) or the value axis (for outputs) as the 16 and the query rows as the 8: a
+// sequence's rows that share a head are few, and tiles of 8 leave the least of the unit idle.  fp16
+// holds every int8 and e4m3 value exactly, and a permutation of the contraction index, applied to both
+// operands, lets every lane load 16 consecutive bytes.  Query rows are scaled by a power of two into
+// fp16's range (their 8 significant bits fit) and the power goes into the row's logit factor.
 #pragma once
 
 #include "kv.cuh"
@@ -48,17 +49,21 @@ __device__ __forceinline__ int64_t kv_div(int64_t a, int b) {
 }
 
 // The blocks share the steps of all (sequence, row block, head) items evenly.  The items lie one after
-// another on one axis (head fastest within a (sequence, row block) pair), and each block takes a piece
-// of `per` consecutive steps of it.  Where there are few items (at most a quarter of the blocks), pieces
-// do not cross from one item to the next: a piece of two items costs its block a second set-up, which
-// takes longer than the few steps that the last pieces of the items leave idle.  Lengths are only known
-// on the device, so every block adds them up itself.
+// another on one axis (head fastest within a (sequence, row block) pair), each behind kItemCost units that
+// stand for a block's set-up of an item, and each block takes a piece of `per` consecutive units of it.
+// Where there are few items (at most a quarter of the blocks), pieces do not cross from one item to the
+// next and there is nothing to level: a piece of two items costs its block a second set-up, which takes
+// longer than the few steps that the last pieces of the items leave idle.  Lengths are only known on the
+// device, so every block adds them up itself.
+constexpr int kItemCost = 16;  // about 6 us, measured in a batch of 64 sequences: the steps that a block takes in that time
+
 struct KvShare {
-  int64_t per;   // steps of a piece
-  int64_t left;  // steps of this block's piece, from here on:
-  int64_t off;   // of its first step within its pair
-  int64_t at;    // of its first step on the axis (pieces that cross items)
+  int64_t per;   // units of a piece
+  int64_t left;  // units of this block's piece, from here on:
+  int64_t off;   // of its first unit within its pair
+  int64_t at;    // of its first unit on the axis (pieces that cross items)
   int pair;
+  int cost;      // units in front of an item's steps: kItemCost, or 0 where pieces do not cross items
   bool cross;
 };
 
@@ -71,6 +76,14 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_block
   const auto steps = [&](unsigned i) -> int {
     const unsigned s = row_blocks == 1 ? i : i / row_blocks, m0 = (i - s * row_blocks) * block_rows;
     return kv_span(p, kv_seq(p.c, p.rows.start, p.rows.lens, s), m0, block_rows).n;
+  };
+  const int64_t items = static_cast<int64_t>(pairs) * p.c.heads;
+  const int blocks = static_cast<int>(gridDim.x);
+  KvShare w{0, 0, 0, 0, 0, 0, items * 4 > blocks};
+  w.cost = w.cross ? kItemCost : 0;
+  const auto units = [&](unsigned i) {
+    const int n = steps(i);
+    return n > 0 ? n + w.cost : 0;
   };
   const unsigned i0 = min(tid * q, pairs), i1 = min(i0 + q, pairs);
   // the sum over this thread's pairs, the sum over those of the threads before it, and over all
@@ -94,11 +107,40 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_block
       all += s_sum[i];
     }
   };
+  if (p.few_steps && pairs <= 32) {
+    // the same in each warp by itself: no barriers, 32-bit sums
+    const int n = lane < static_cast<int>(pairs) ? units(lane) : 0, heads = p.c.heads;
+    const int all = __reduce_add_sync(0xffffffffu, n * heads);
+    if (all == 0) return w;
+    const int pieces = w.cross ? blocks : blocks - static_cast<int>(items);
+    const int per = ((all + pieces - 1) / pieces + round - 1) / round * round;
+    const int parts = (n + per - 1) / per;  // of this lane's pair
+    int pre = w.cross ? n * heads : parts * heads;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += up;
+    }
+    const int64_t at = w.cross ? static_cast<int64_t>(blockIdx.x) * per : blockIdx.x;
+    const unsigned past = __ballot_sync(0xffffffffu, at < pre);
+    w.per = per;
+    w.at = at;
+    if (past == 0) return w;
+    w.pair = __ffs(past) - 1;
+    const int size = __shfl_sync(0xffffffffu, n, w.pair), ps = __shfl_sync(0xffffffffu, parts, w.pair);
+    const int off = static_cast<int>(at) - (__shfl_sync(0xffffffffu, pre, w.pair) - (w.cross ? size : ps) * heads);
+    if (w.cross) {
+      w.off = off;
+      w.left = min(per, all - static_cast<int>(at));
+    } else {
+      const int h = off / ps, part = off - h * ps;
+      w.off = static_cast<int64_t>(h) * size + part * per;
+      w.left = min(per, size - part * per);
+    }
+    return w;
+  }
   int64_t mine, before, total;
-  scan([&](unsigned i) { return static_cast<int64_t>(steps(i)) * p.c.heads; }, mine, before, total);
-  const int64_t items = static_cast<int64_t>(pairs) * p.c.heads;
-  const int blocks = static_cast<int>(gridDim.x);
-  KvShare w{0, 0, 0, 0, 0, items * 4 > blocks};
+  scan([&](unsigned i) { return static_cast<int64_t>(units(i)) * p.c.heads; }, mine, before, total);
   if (total == 0) return w;
   const int pieces = w.cross ? blocks : blocks - static_cast<int>(items);  // each item may leave a piece unfilled
   w.per = kv_div(total + pieces - 1, pieces);
@@ -111,7 +153,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_block
   if (w.at >= before && w.at < before + mine) {
     unsigned i = i0;
     int64_t n;
-    while (w.at >= before + (n = w.cross ? static_cast<int64_t>(steps(i)) * p.c.heads : pieces_of(i))) {
+    while (w.at >= before + (n = w.cross ? static_cast<int64_t>(units(i)) * p.c.heads : pieces_of(i))) {
       before += n;
       ++i;
     }
@@ -132,30 +174,29 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_block
   return w;
 }
 
-// Page and scales of 32 of a warp's steps, one a lane.  The pages come first: the copies of the codes
-// wait for them alone.
+// Page and scales of 32 of a warp's steps, one a lane.
 struct KvPages {
   int page;
-  float ks, vlog, vinv;
-};
-
-__device__ __forceinline__ KvPages kv_pages(const KvCache& c, int s, bool live, int base) {
-  return KvPages{live ? kv_page(c.table, c.width, c.pages, s, base >> c.tshift) : -1, 0.f, 0.f, 0.f};
-}
-
-// The value scale enters the logits as a power of two (vlog), so that the weights of every page share
-// one reference whatever its scale; a scale of 0 (a page of zeros) is taken as 2^-96.
-template <bool V>
-__device__ __forceinline__ void kv_scales(const KvCache& c, int h, KvPages& m) {
-  if (m.page < 0) return;
-  const int64_t unit = static_cast<int64_t>(m.page) * c.heads + h;
-  m.ks = c.ks[unit];
-  if constexpr (V) {
-    const float vs = fmaxf(c.vs[unit], 0x1p-96f);
-    m.vlog = log2f(vs);
-    m.vinv = 1.f / vs;
+  float ks, vs;
+  __device__ __forceinline__ void load_page(const KvCache& c, int s, bool live, int base) {
+    page = -1;
+    if (live) page = c.table[static_cast<int64_t>(s) * c.width + (base >> c.tshift)] & 0x7fffffff;
   }
-}
+  __device__ __forceinline__ void check_page(const KvCache& c) {
+    if (page >= c.pages) {
+      set_status(kStatusKvPage);
+      page = -1;
+    }
+  }
+  template <bool V>
+  __device__ __forceinline__ void load_scales(const KvCache& c, int h) {
+    ks = vs = 0.f;
+    if (page < 0) return;
+    const int64_t unit = static_cast<int64_t>(page) * c.heads + h;
+    ks = c.ks[unit];
+    if (V) vs = c.vs[unit];
+  }
+};
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -163,20 +204,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Asynchronous copies to shared memory, and plain loads: an earlier kernel of the stream may have written
-// the codes while this one was starting.
-__device__ __forceinline__ void cp_async16(void* dst, const uint8_t* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async8(void* dst, const uint8_t* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
+// A plain load: an earlier kernel of the stream may have written the codes while this one was starting.
 __device__ __forceinline__ uint4 ld128(const uint8_t* p) {
   uint4 v;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -202,68 +230,99 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+// Four K codes as fp16 pairs: an int8 code's byte alone is the
+// subnormal 2^-24 code, and its offset of 128 comes off the logit as 128 times the sum of the query row
+// (kv_make_q), which costs one operation a row instead of one a pair.
+template <int FMT>
+__device__ __forceinline__ void k_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == kKvInt8) {
+    lo = prmt(w, 0, 0x4140u);
+    hi = prmt(w, 0, 0x4342u);
+  } else {
+    codes_to_half<FMT>(w, lo, hi);
+  }
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The 16 query rows m0 .. of kv head h as A operands: lane (g, c) = (lane / 4, lane % 4) holds, for the
-// contraction step 4 i + w, the values 64 i + 16 c + 4 w .. + 3 of the rows g and g + 8 -- the order
-// in which a lane's 16 loaded K codes lie.  One warp writes D / 16 steps of 32 lanes to `sq` and the
-// rows' logit factors (the power of two taken out, times scale * log2 e) to `sf`.  Rows that do not
-// exist are 0.
+// The 8 query rows m0 .. of kv head h: lane (g, c) = (lane / 4, lane % 4) loads the values 64 i + 16 c ..
+// + 15 of row g.  Rows that do not exist are 0.
 template <int D>
-__device__ __forceinline__ void kv_load_q(const KvAttnParams& p, const KvSeq& seq, int s, int h, unsigned m0, uint4* sq,
-                                          float* sf) {
+__device__ __forceinline__ void kv_fetch_q(const KvAttnParams& p, const KvSeq& seq, int s, int h, unsigned m0,
+                                           uint4 (&raw)[D / 64][2]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  uint32_t half[2][D / 64][8];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const unsigned m = m0 + g + 8 * e, r = m / static_cast<unsigned>(p.G);
-    const bool live = r < static_cast<unsigned>(p.rows.R) && seq.start + static_cast<int>(r) < seq.len;
-    const bf16* from = p.q + s * p.qs + r * p.qr + (h * static_cast<int64_t>(p.G) + (m - r * p.G)) * D + 16 * c;
-    uint4 raw[D / 64][2];
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        raw[i][k] = make_uint4(0, 0, 0, 0);
-        if (live)
-          raw[i][k] = *reinterpret_cast<const uint4*>(from + 64 * i + 8 * k);
-        const uint32_t w[4] = {raw[i][k].x, raw[i][k].y, raw[i][k].z, raw[i][k].w};
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xFFFF0000u))));
-      }
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // 2^-x brings the largest value into [1, 2); the power is kept within fp32's normal range
-    const int x = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 120);
-    const float down = __uint_as_float(static_cast<uint32_t>(127 - x) << 23);
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t w[4] = {raw[i][k].x, raw[i][k].y, raw[i][k].z, raw[i][k].w};
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const __half2 v = __floats2half2_rn(__uint_as_float(w[y] << 16) * down,
-                                              __uint_as_float(w[y] & 0xFFFF0000u) * down);
-          half[e][i][4 * k + y] = *reinterpret_cast<const uint32_t*>(&v);
-        }
-      }
-    if (c == 0) sf[g + 8 * e] = __uint_as_float(static_cast<uint32_t>(127 + x) << 23) * (p.scale * kLog2e);
-  }
+  const unsigned m = m0 + g, r = m / static_cast<unsigned>(p.G);
+  const bool live = r < static_cast<unsigned>(p.rows.R) && seq.start + static_cast<int>(r) < seq.len;
+  const bf16* from = p.q + s * p.qs + r * p.qr + (h * static_cast<int64_t>(p.G) + (m - r * p.G)) * D + 16 * c;
 #pragma unroll
   for (int i = 0; i < D / 64; ++i)
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
-      sq[(4 * i + w) * 32 + lane] =
-          make_uint4(half[0][i][2 * w], half[1][i][2 * w], half[0][i][2 * w + 1], half[1][i][2 * w + 1]);
+    for (int k = 0; k < 2; ++k) {
+      raw[i][k] = make_uint4(0, 0, 0, 0);
+      if (live) raw[i][k] = *reinterpret_cast<const uint4*>(from + 64 * i + 8 * k);
+    }
+}
+
+// ... and as B operands: for the contraction step 4 i + y the lane holds the values 64 i + 16 c + 4 y .. + 3
+// of row g -- the order in which a lane's 16 loaded K codes lie.  logit / log 2 = (sum of products) * f - t,
+// times the page's K scale; f and t are those of row g.
+template <int D, int FMT>
+__device__ __forceinline__ void kv_make_q(const KvAttnParams& p, const uint4 (&raw)[D / 64][2], uint2 (&q)[D / 16],
+                                          float& f, float& t) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t w[4] = {raw[i][k].x, raw[i][k].y, raw[i][k].z, raw[i][k].w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xFFFF0000u))));
+    }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  // 2^-x brings the largest value into [1, 2); the power is kept within fp32's normal range
+  const int x = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 120);
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - x) << 23);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t w[4] = {raw[i][k].x, raw[i][k].y, raw[i][k].z, raw[i][k].w};
+      uint32_t u[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const __half2 v = __floats2half2_rn(__uint_as_float(w[y] << 16) * down, __uint_as_float(w[y] & 0xFFFF0000u) * down);
+        sum += __low2float(v) + __high2float(v);
+        u[y] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      q[4 * i + 2 * k] = make_uint2(u[0], u[1]);
+      q[4 * i + 2 * k + 1] = make_uint2(u[2], u[3]);
+    }
+  f = __uint_as_float(static_cast<uint32_t>(127 + x) << 23) * (p.scale * kLog2e);
+  t = 0.f;
+  if constexpr (FMT == kKvInt8) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    t = 128.f * f * sum;
+    f *= 0x1p24f;
+  }
+}
+
+// The same with sums that start at 0.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }

@@ -49,14 +49,30 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 
 }  // namespace
 
-bool row_tile_map(CUtensorMap* out, const void* base, int64_t rows, int64_t row_bytes, int pieces, int piece_bytes,
-                  int box_rows) {
-  static std::mutex mu;
-  static std::unordered_map<Key, CUtensorMap, KeyHash> cache;
+bool encode_row_tile_map(CUtensorMap* out, const void* base, int64_t rows, int64_t row_bytes, int pieces,
+                         int piece_bytes, int box_rows) {
   if ((piece_bytes != 128 && piece_bytes != 64 && piece_bytes != 16) || row_bytes % piece_bytes != 0 || pieces < 1 ||
       pieces > 256 ||
       rows < 1 || box_rows < 1 || box_rows > 256 || (reinterpret_cast<uintptr_t>(base) & 15))
     return false;
+  auto enc = encoder();
+  if (!enc) return false;
+  const cuuint64_t pb = static_cast<cuuint64_t>(piece_bytes);
+  cuuint64_t dims[3] = {pb, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(row_bytes) / pb};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes), pb};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(pb), static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(pieces)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE,
+             piece_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : (piece_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE),
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool row_tile_map(CUtensorMap* out, const void* base, int64_t rows, int64_t row_bytes, int pieces, int piece_bytes,
+                  int box_rows) {
+  static std::mutex mu;
+  static std::unordered_map<Key, CUtensorMap, KeyHash> cache;
   int dev = 0;
   cudaGetDevice(&dev);
   const Key key{base, rows, row_bytes, pieces, piece_bytes, box_rows, dev};
@@ -66,20 +82,8 @@ bool row_tile_map(CUtensorMap* out, const void* base, int64_t rows, int64_t row_
     *out = it->second;
     return true;
   }
-  auto enc = encoder();
-  if (!enc) return false;
   CUtensorMap m;
-  const cuuint64_t pb = static_cast<cuuint64_t>(piece_bytes);
-  cuuint64_t dims[3] = {pb, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(row_bytes) / pb};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes), pb};
-  cuuint32_t box[3] = {static_cast<cuuint32_t>(pb), static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(pieces)};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   piece_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                      : (piece_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE),
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return false;
+  if (!encode_row_tile_map(&m, base, rows, row_bytes, pieces, piece_bytes, box_rows)) return false;
   if (cache.size() > 4096) cache.clear();
   cache.emplace(key, m);
   *out = m;

@@ -22,6 +22,11 @@ namespace bolt {
 // 64-byte pieces use the 64-byte swizzle: [piece][row][64 B] with the 16-byte chunks of each
 // row permuted by XOR with ((row >> 1) & 3), which spreads eight consecutive rows over the banks.
 //
+// Encodes the map of `base` viewed as above with a box of (piece_bytes, box_rows, pieces), anew in every
+// call: for tensors of which a caller may have any number.
+bool encode_row_tile_map(CUtensorMap* out, const void* base, int64_t rows, int64_t row_bytes, int pieces,
+                         int piece_bytes, int box_rows);
+
 // Encodes (or returns the cached) map of `base` viewed as above with a box of
 // (piece_bytes, box_rows, pieces); piece_bytes is 128 or 64 (swizzled) or 16 (plain), box_rows
 // up to 256 (swz_off below assumes a multiple of 8; swz_line_off takes any count).
