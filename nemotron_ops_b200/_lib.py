@@ -75,8 +75,10 @@ _SHAPES: dict = {}
 def shape_arg(shape):
     """(int64_t* view, owning array) for a shape.  Shapes repeat from call to call, so the
     read-only arrays are cached (building one costs several microseconds per call)."""
-    key = tuple(int(s) for s in shape)
-    hit = _SHAPES.get(key)
+    hit = _SHAPES.get(shape) if isinstance(shape, tuple) else None  # a torch.Size is found by the tuple it equals
+    if hit is None:
+        key = tuple(int(s) for s in shape)
+        hit = _SHAPES.get(key)
     if hit is None:
         arr = (ctypes.c_int64 * max(1, len(key)))(*key)
         hit = (ctypes.cast(arr, _S), arr)

@@ -59,15 +59,6 @@ __device__ __forceinline__ int swizzle(int row, int f) {
   return f ^ (D == 128 ? c : (c & 1) | (c >> 1) << 2);
 }
 
-// A step's codes lie in the ring as the tensor copy writes them: 16 rows of D bytes of K, then of V, the
-// 16-byte chunks of row r exchanged by XOR with r % 8 (D = 128) or r / 2 % 4 (D = 64).  Row index i of a
-// tile of 8 positions stands for position place<D>(i): with this order the 8 lanes of a shared-memory phase
-// fall into different banks both when they read K (rows i = lane / 4) and V (rows i = 2 (lane % 4) and + 1).
-template <int D>
-__device__ __forceinline__ int place(int i) {
-  return D == 128 ? i ^ ((i & 1) << 2) : (i & 4) | ((i & 1) << 1) | (((i >> 1) ^ i) & 1);
-}
-
 // An 8 x 8 matrix of halves, two neighbours of a row a lane, transposed.
 __device__ __forceinline__ uint32_t transpose8(__half2 x) {
   uint32_t y;
@@ -78,11 +69,11 @@ __device__ __forceinline__ uint32_t transpose8(__half2 x) {
 template <int D>
 struct VCodes {
   uint32_t w[4][D / 32];  // position, word
-  // `at`: this lane's places of the positions 2 c and 2 c + 1 in the step's V rows; the others are 8 rows on
+  // `at`: this lane's places of the positions 2 c and 2 c + 1 in the step's V lines; the others are 8 positions on
   __device__ __forceinline__ void load(const uint8_t* v, const int (&at)[2]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t* from = v + at[i & 1] + (i >> 1) * 8 * D;
+      const uint8_t* from = v + (i < 2 ? at[i & 1] : kv_next_tile<D>(at[i & 1]));
       if constexpr (D == 128) {
         const uint4 x = lds128(from);
         w[i][0] = x.x;
@@ -108,7 +99,7 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
   uint4* tail = smem + (L::kRing > L::kJoin ? L::kRing : L::kJoin);
   uint2* sq = reinterpret_cast<uint2*>(tail);                              // [MW * NT][D / 16][32]
   float4* s_scale = reinterpret_cast<float4*>(sq + L::kQ);                 // [warps][64]: K scale, log2 and 1 / V scale, position and flags
-  int* s_row = reinterpret_cast<int*>(s_scale + L::kWarps * 64);           // [warps][64]: first row of the codes, or -1
+  int* s_row = reinterpret_cast<int*>(s_scale + L::kWarps * 64);           // [warps][64]: first line of the codes, or -1
   uint64_t* s_full = reinterpret_cast<uint64_t*>(s_row + L::kWarps * 64);  // [warps][STAGES]: barriers of the ring
   float* sm = reinterpret_cast<float*>(s_full + L::kWarps * STAGES);       // [TW][rows]
   float* sl = sm + TW * L::kRows;                                          // [TW][rows]
@@ -132,13 +123,8 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
   __syncwarp();
   unsigned taken = 0;   // steps that this warp has put into its ring, of all segments
   bool stuck = false;   // a copy did not arrive in time: the rest of the work is left
-  const int k_at = place<D>(g) * D + (D == 128 ? q4 ^ (place<D>(g) & 7) : q4 ^ ((place<D>(g) >> 1) & 3)) * 16;
-  int v_at[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t = place<D>(2 * q4 + i);
-    v_at[i] = t * D + (D == 128 ? (g ^ t) * 16 : ((g >> 1) ^ ((t >> 1) & 3)) * 16 + (g & 1) * 8);
-  }
+  const int k_at = kv_at<D>(place<D>(g), 16 * q4);  // the codes 64 i + 16 q4 .. are at k_at ^ 64 i
+  const int v_at[2] = {kv_at<D>(place<D>(2 * q4), D / 8 * g), kv_at<D>(place<D>(2 * q4 + 1), D / 8 * g)};
   const KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW * NP);
 
   if (!by_item && tid == 0) w.split[blockIdx.x].parts = 0;
@@ -202,7 +188,7 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
     const auto look_up_scales = [&](int k) {
       meta.check_page(c);
       meta.load_scales<true>(c, h);
-      s_row[k & 63] = meta.page < 0 ? -1 : (meta.page * c.heads + h) * c.T + (span.base(step_of(k)) & (c.T - 1));
+      s_row[k & 63] = meta.page < 0 ? -1 : ((meta.page * c.heads + h) * c.T + (span.base(step_of(k)) & (c.T - 1))) / (128 / D);
     };
     constexpr int kDead = 1, kWhole = 2;  // none of the warp's rows sees the step, or all see all of it
     const auto keep = [&](int k) {
@@ -320,7 +306,7 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
       for (int u = 0; u < NP; ++u)
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
-          const uint4 lo = lds128(b[u] + (k_at ^ (64 * i))), hi = lds128(b[u] + 8 * D + (k_at ^ (64 * i)));
+          const uint4 lo = lds128(b[u] + (k_at ^ (64 * i))), hi = lds128(b[u] + (kv_next_tile<D>(k_at) ^ (64 * i)));
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             uint32_t a0, a1, a2, a3;
@@ -600,8 +586,8 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(co
 struct Plan {
   int rows, round, per_sm;
 };
-Plan plan_of(int64_t M) {
-  if (M <= 8) return Plan{8, 4, 3};
+Plan plan_of(int64_t M, int D) {
+  if (M <= 8) return Plan{8, D == 64 ? 8 : 4, 3};
   if (M <= 16) return Plan{16, 4, 2};
   if (M <= 32) return Plan{32, 8, 1};
   if (M <= 64) return Plan{64, 4, 1};
@@ -615,18 +601,15 @@ cudaError_t launch(const KvAttnParams& p, const Work& w, unsigned blocks, const 
   auto kern = kv_attention_kernel<D, FMT, NT, MW, TW, NP, STAGES, CPS>;
   const cudaError_t e = allow_smem(kern, L::kSmem, opt);
   if (e != cudaSuccess) return e;
-  // a step's rows of K and of V, as the ring holds them
-  const int64_t rows = p.c.pages * p.c.heads * p.c.T;
   CUtensorMap map_k, map_v;
-  if (!encode_row_tile_map(&map_k, p.c.k, rows, D, 1, D, 16) || !encode_row_tile_map(&map_v, p.c.v, rows, D, 1, D, 16))
-    return cudaErrorInvalidValue;
+  if (!kv_code_map(&map_k, p.c, p.c.k) || !kv_code_map(&map_v, p.c, p.c.v)) return cudaErrorInvalidValue;
   return launch_kernel(kern, dim3(blocks), dim3(L::kThreads), L::kSmem, cfg, p, w, map_k, map_v);
 }
 
 template <int D, int FMT>
 cudaError_t launch_rows(const KvAttnParams& p, const Work& w, int rows, unsigned blocks, const LaunchCfg& cfg) {
   switch (rows) {
-    case 8: return launch<D, FMT, 1, 1, 4, 1, 4, 3>(p, w, blocks, cfg);
+    case 8: return launch<D, FMT, 1, 1, 4, D == 64 ? 2 : 1, D == 64 ? 6 : 4, 3>(p, w, blocks, cfg);
     case 16: return launch<D, FMT, 2, 1, 4, 1, 4, 2>(p, w, blocks, cfg);
     case 32: return launch<D, FMT, 4, 1, 8, 1, 4, 1>(p, w, blocks, cfg);
     case 64: return launch<D, FMT, 4, 2, 4, 1, 4, 1>(p, w, blocks, cfg);
@@ -639,7 +622,7 @@ int64_t align16(int64_t n) { return (n + 15) & ~int64_t(15); }
 }  // namespace
 
 int64_t kv_attention_workspace(int64_t rows, int D, int sms) {
-  const Plan t = plan_of(rows);
+  const Plan t = plan_of(rows, D);
   const int64_t blocks = static_cast<int64_t>(sms) * t.per_sm;
   return align16(blocks * 2 * t.rows * D * 4) + align16(blocks * 2 * t.rows * 8) + blocks * static_cast<int64_t>(sizeof(Split));
 }
@@ -647,7 +630,7 @@ int64_t kv_attention_workspace(int64_t rows, int D, int sms) {
 cudaError_t launch_kv_attention(const KvAttnParams& params, void* workspace, const LaunchCfg& cfg) {
   KvAttnParams p = params;
   const int64_t M = static_cast<int64_t>(p.rows.R) * p.G;
-  const Plan t = plan_of(M);
+  const Plan t = plan_of(M, p.c.D);
   const int64_t row_blocks = (M + t.rows - 1) / t.rows, items = p.c.S * row_blocks * p.c.heads;
   if (M > 0x7fffffff || p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   p.few_steps = items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16 + kItemCost) <= 0x7fffffff;

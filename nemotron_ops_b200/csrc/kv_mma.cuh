@@ -11,6 +11,7 @@
 #pragma once
 
 #include "kv.cuh"
+#include "tensor_map.h"
 
 namespace bolt {
 
@@ -204,13 +205,30 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A plain load: an earlier kernel of the stream may have written the codes while this one was starting.
-__device__ __forceinline__ uint4 ld128(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// A step's codes lie in the ring as the tensor copy writes them: lines of 128 bytes (a position of 128
+// values, or two of 64: a copy's rate goes by its lines), the 16-byte chunks of line i exchanged by XOR with
+// i % 8.  Row index i of a tile of 8 positions stands for position place<D>(i): with this order the 8
+// (16, for 8-byte loads) lanes of a shared-memory phase fall into different banks both when they read K
+// (rows i = lane / 4) and V (rows i = 2 (lane % 4) and + 1).
+template <int D>
+__device__ __forceinline__ int place(int i) {
+  return D == 128 ? i ^ ((i & 1) << 2) : (i & 4) | ((i & 1) << 1) | (((i >> 1) ^ i) & 1);
+}
+
+// Byte offset of byte `b` of position t < 8 of a step; position 8 + t is at kv_next_tile of it.
+template <int D>
+__device__ __forceinline__ int kv_at(int t, int b) {
+  if (D == 128) return t * 128 + (((b >> 4) ^ t) << 4 | (b & 15));
+  return (t >> 1) * 128 + ((((t & 1) * 4 + (b >> 4)) ^ (t >> 1)) << 4 | (b & 15));
+}
+template <int D>
+__device__ __forceinline__ int kv_next_tile(int at) {
+  return D == 128 ? at + 1024 : (at ^ 64) + 512;
+}
+
+// The map of a cache's codes by lines, with a box of one step; row r of the cache (of D bytes) is line r D / 128.
+inline bool kv_code_map(CUtensorMap* out, const KvCache& c, const uint8_t* codes) {
+  return encode_row_tile_map(out, codes, c.pages * c.heads * c.T * c.D / 128, 128, 1, 128, 16 * c.D / 128);
 }
 
 // Four codes (a word) as two fp16 pairs, exact.

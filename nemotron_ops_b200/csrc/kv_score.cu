@@ -1,10 +1,11 @@
 // KvScore: score[s, h, j] += sum over the rows and the query heads of cache head h of
 // exp(scale * q . k_j - lse), the attention weights that KvAttention gave position j.
 //
-// The steps of all (sequence, head) pairs are shared evenly over the blocks (kv_mma.cuh); a step's
-// 16 positions belong to one warp, which keeps their K codes as fp16 operands in registers while it
-// goes through the row tiles, so a sum is made by one warp in one order and added to the score once
-// for each kRowTiles * 8 rows.
+// The steps of all (sequence, head) pairs are shared evenly over the blocks (kv_mma.cuh).  A step's
+// 16 positions belong to one warp, which copies their K codes into a ring of its own ahead of time and
+// keeps them as fp16 operands in registers while it goes through the row tiles: a sum is made by one warp
+// in one order and added to the score once for each kRowTiles * 8 rows, by a reduction in memory that
+// nothing waits for and no other warp makes for these positions.
 #include "kv_mma.cuh"
 
 namespace bolt {
@@ -13,17 +14,42 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kRowTiles = 16;  // tiles of 8 query rows in shared memory at a time
+// Steps that a warp takes at a time and steps of its ring.  Steps of 64 values are too short for one alone
+// (32 sequences of up to 8,192 positions, 8 heads: 54 us one at a time, 42 us two); two of 128 values leave one block an SM (65,536 positions, 2 heads: 12 us one at a time, 18 us two).
+template <int D>
+constexpr int kTogether = D == 64 ? 2 : 1;
+template <int D>
+constexpr int kRing = D == 64 ? 6 : 4;
+template <int D>
+constexpr size_t kScoreSmem = kWarps * (kRing<D> * (16 * D + 8) + 64 * 12) + 1024;
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(kWarps * 32, 2) kv_score_kernel(const KvAttnParams p) {
+__global__ void __launch_bounds__(kWarps * 32, 2) kv_score_kernel(const KvAttnParams p, const __grid_constant__ CUtensorMap map_k) {
+  constexpr int kPairs = kTogether<D>, kStages = kRing<D>;
+  extern __shared__ uint8_t smem_raw[];
   __shared__ uint2 sq[kRowTiles * (D / 16) * 32];
-  __shared__ float4 srow[kRowTiles * 8];  // a row's logit factor and shift, lse / log 2, and position or -1
+  __shared__ float4 srow[kRowTiles * 8];  // a row's logit factor and shift, lse / log 2 (of no row: infinite, so that its weights are 0), and position or -1
   pdl_wait();
   pdl_trigger();
   const KvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + warp * kStages * 16 * D;
+  uint64_t* s_full = reinterpret_cast<uint64_t*>(smem + kWarps * kStages * 16 * D) + warp * kStages;  // the ring's barriers
+  // of 64 of the warp's steps: first line of the codes or -1, and the page's scale and the first position
+  float2* s_scale = reinterpret_cast<float2*>(smem + kWarps * kStages * (16 * D + 8)) + warp * 64;
+  int* s_row = reinterpret_cast<int*>(smem + kWarps * (kStages * (16 * D + 8) + 64 * 8)) + warp * 64;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(s_full + i), 1);
+    fence_barrier_init();
+    asm volatile("fence.proxy.async;" ::: "memory");
+  }
+  __syncwarp();
+  unsigned taken = 0;  // steps that this warp has put into its ring, of all segments
+  bool stuck = false;  // a copy did not arrive in time: the rest of the work is left
+  const int k_at = kv_at<D>(place<D>(g), 16 * q4);  // the codes 64 i + 16 q4 .. are at k_at ^ 64 i
   const unsigned M = static_cast<unsigned>(p.rows.R) * p.G;
-  const KvShare share = kv_share<kWarps * 32>(p, 1, M, kWarps);
+  const KvShare share = kv_share<kWarps * 32>(p, 1, M, kWarps * kPairs);
   int64_t left = share.left, off = share.off;
   for (int next_s = share.pair; left > 0;) {
     const int s = next_s;
@@ -46,104 +72,172 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv_score_kernel(const KvAttnPa
     }
     if (i0 == i1) continue;
     float* score = p.score + (static_cast<int64_t>(s) * c.heads + h) * p.score_width;
-    const int steps = max(0, (i1 - i0 - warp + kWarps - 1) / kWarps);
-    const auto base_of = [&](int n) { return span.base(i0 + warp + n * kWarps); };
-    const uint8_t* kc = c.k + static_cast<int64_t>(h) * c.T * D;
-    const int64_t page_codes = static_cast<int64_t>(c.heads) * c.T * D;
+    // this warp's k-th step is the k % kPairs-th of the group k / kPairs * kWarps + warp
+    const int most = max(0, (i1 - i0 - warp * kPairs + kWarps * kPairs - 1) / (kWarps * kPairs));
+    const auto step_of = [&](int k) { return i0 + (k / kPairs * kWarps + warp) * kPairs + k % kPairs; };
     for (unsigned m0 = 0; m0 < M; m0 += kRowTiles * 8) {
       const int tiles = min((M - m0 + 7) / 8, static_cast<unsigned>(kRowTiles));
       const KvSpan chunk = kv_span(p, seq, m0, kRowTiles * 8);
       if (chunk.n == 0) break;  // rows past the sequence's end, here and in every later chunk
-      __syncthreads();          // the previous chunk's operands are still read
+      const int rounds = stuck ? 0 : most;
+      KvPages meta;
+      const auto look_up = [&](int k) {
+        const int i = step_of(k);
+        meta.load_page(c, s, k < rounds * kPairs && i < i1, span.base(min(i, i1 - 1)));
+      };
+      const auto look_up_scales = [&](int k) {
+        meta.check_page(c);
+        meta.load_scales<false>(c, h);
+        s_row[k & 63] = meta.page < 0 ? -1 : ((meta.page * c.heads + h) * c.T + (span.base(step_of(k)) & (c.T - 1))) / (128 / D);
+      };
+      constexpr int kDead = 1, kWhole = 2;  // no row of the chunk sees the step, or all see all of it
+      const auto keep = [&](int k) {
+        const int j0 = span.base(min(step_of(k), i1 - 1));
+        int flags = 0;
+        if (meta.page < 0 || j0 > chunk.last)
+          flags = kDead;
+        else if (j0 + 15 <= chunk.first &&
+                 (p.mask.window == 0 || j0 > chunk.last - p.mask.window || j0 + 15 < p.mask.sinks))
+          flags = kWhole;
+        s_scale[k & 63] = make_float2(meta.ks, __int_as_float(j0 | flags));
+      };
+      const auto fetch = [&](int n) {
+        __syncwarp();  // no lane reads its places in the ring any more
+        if (lane != 0 || n >= rounds) return;
+#pragma unroll
+        for (int u = 0; u < kPairs; ++u) {
+          const unsigned slot = (taken + n * kPairs + u) % kStages;
+          const int row = s_row[(n * kPairs + u) & 63];
+          const uint32_t bar = smem_u32(s_full + slot);
+          if (row >= 0) {
+            mbar_arrive_expect_tx(bar, 16 * D);
+            tma_load_3d(smem_u32(ring + slot * 16 * D), &map_k, 0, row, 0, bar);
+          } else {
+            mbar_arrive(bar);
+          }
+        }
+      };
+      constexpr int kAhead = kStages / kPairs - 1;
+      look_up(lane);
+      look_up_scales(lane);
+      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) fetch(n);
+      __syncthreads();  // the previous chunk's operands have been read
       for (int t = warp; t < tiles; t += kWarps) {
         uint2 x[D / 16];
         float f, sh;
         uint4 rq[D / 64][2];
         kv_fetch_q<D>(p, seq, s, h, m0 + t * 8, rq);
+        const unsigned m = m0 + t * 8 + g, r = m / static_cast<unsigned>(p.G);
+        const bool live = m < M && seq.start + static_cast<int>(r) < seq.len;
+        const float z = live ? p.lse[(static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * p.G + (m - r * p.G)] * kLog2e : INFINITY;
         kv_make_q<D, FMT>(p, rq, x, f, sh);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) sq[(t * (D / 16) + kk) * 32 + lane] = x[kk];
-        if (q4 == 0) {
-          const unsigned m = m0 + t * 8 + g, r = m / static_cast<unsigned>(p.G);
-          const bool live = m < M && seq.start + static_cast<int>(r) < seq.len;
-          const float z = live ? p.lse[(static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * p.G + (m - r * p.G)] * kLog2e : 0.f;
-          srow[t * 8 + g] = make_float4(f, sh, z, __int_as_float(live ? seq.start + static_cast<int>(r) : -1));
-        }
+        if (q4 == 0) srow[t * 8 + g] = make_float4(f, sh, z, __int_as_float(live ? seq.start + static_cast<int>(r) : -1));
       }
-      KvPages meta{-1, 0.f, 0.f}, next;
-      next.load_page(c, s, lane < steps, base_of(lane));
-      next.check_page(c);
-      next.load_scales<false>(c, h);
-      uint4 raw[2][D / 64], ahead[2][D / 64];
-      const auto fetch = [&](int n, const KvPages& of) {
-        const int page = __shfl_sync(0xffffffffu, of.page, n & 31);
-        if (page < 0) return;
-        // lane (g, q4) takes the codes 64 i + 16 q4 .. + 15 of the positions g and 8 + g
-        const uint8_t* from = kc + page * page_codes + ((base_of(n) & (c.T - 1)) + g) * D + 16 * q4;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i) ahead[t][i] = ld128(from + 8 * t * D + 64 * i);
-      };
-      if (steps > 0) fetch(0, next);
+      keep(lane);
       __syncthreads();
-      for (int n = 0; n < steps; ++n) {
-        if ((n & 31) == 0) {
-          meta = next;
-          next.load_page(c, s, n + 32 + lane < steps, base_of(min(n + 32 + lane, steps)));
+      for (int n = 0; n < rounds; ++n) {
+        const int k0 = n * kPairs;
+        if ((k0 & 7) == 0) {
+          const int later = (k0 & ~31) + 32 + lane;
+          __syncwarp();  // no lane reads the entries of 32 steps ago any more
+          if ((k0 & 31) == 0) look_up(later);
+          if ((k0 & 31) == 8) look_up_scales(later);
+          if ((k0 & 31) == 16) keep(later);
+          __syncwarp();
         }
-        if ((n & 31) == 8) {
-          next.check_page(c);
-          next.load_scales<false>(c, h);
+        fetch(n + kAhead);
+        bool late = false;
+#pragma unroll
+        for (int u = 0; u < kPairs; ++u) {
+          const unsigned i = taken + k0 + u;
+          late |= !mbar_wait(smem_u32(s_full + i % kStages), (i / kStages) & 1, kStatusFullWait);
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i) raw[t][i] = ahead[t][i];
-        if (n + 1 < steps) fetch(n + 1, ((n + 1) & 31) == 0 ? next : meta);
-        const int page = __shfl_sync(0xffffffffu, meta.page, n & 31);
-        const float ks = __shfl_sync(0xffffffffu, meta.ks, n & 31);
-        const int j0 = base_of(n);
-        if (page < 0 || j0 > chunk.last) continue;
-        uint32_t a[D / 16][4];
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          k_to_half<FMT>(word_of(raw[0][kk >> 2], kk & 3), a[kk][0], a[kk][2]);
-          k_to_half<FMT>(word_of(raw[1][kk >> 2], kk & 3), a[kk][1], a[kk][3]);
+        if (__any_sync(0xffffffffu, late)) {
+          // wait, within limits, for what else is on its way into the ring
+          for (int k = k0; k < min(n + kAhead + 1, rounds) * kPairs; ++k)
+            mbar_wait(smem_u32(s_full + (taken + k) % kStages), ((taken + k) / kStages) & 1, kStatusDrainWait);
+          stuck = true;
+          break;
         }
-        float sum[2] = {0.f, 0.f};  // positions g and 8 + g
+        float ks[kPairs];
+        int j0[kPairs], all = kDead | kWhole;
+        uint32_t a[kPairs][D / 16][4];
+#pragma unroll
+        for (int u = 0; u < kPairs; ++u) {
+          const float2 sc = s_scale[(k0 + u) & 63];
+          ks[u] = sc.x;
+          j0[u] = __float_as_int(sc.y);
+          all &= j0[u];
+          // a step that was not copied holds anything; its weights are left out below
+          const uint8_t* b = ring + (taken + k0 + u) % kStages * 16 * D;
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            const uint4 lo = lds128(b + (k_at ^ (64 * i))), hi = lds128(b + (kv_next_tile<D>(k_at) ^ (64 * i)));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              k_to_half<FMT>(word_of(lo, y), a[u][4 * i + y][0], a[u][4 * i + y][2]);
+              k_to_half<FMT>(word_of(hi, y), a[u][4 * i + y][1], a[u][4 * i + y][3]);
+            }
+          }
+        }
+        if (all & kDead) continue;
+        const bool whole = all & kWhole;
+        float sum[kPairs][2] = {};  // positions place(g) and 8 + place(g)
         for (int t = 0; t < tiles; ++t) {
-          float x[4];
-          const uint2 b0 = sq[t * (D / 16) * 32 + lane];
-          mma16816_first(x, a[0][0], a[0][1], a[0][2], a[0][3], b0.x, b0.y);
+          float x[kPairs][4];
 #pragma unroll
-          for (int kk = 1; kk < D / 16; ++kk) {
+          for (int kk = 0; kk < D / 16; ++kk) {
             const uint2 b = sq[(t * (D / 16) + kk) * 32 + lane];
-            mma16816(x, a[kk][0], a[kk][1], a[kk][2], a[kk][3], b.x, b.y);
+#pragma unroll
+            for (int u = 0; u < kPairs; ++u) {
+              if (kk == 0)
+                mma16816_first(x[u], a[u][kk][0], a[u][kk][1], a[u][kk][2], a[u][kk][3], b.x, b.y);
+              else
+                mma16816(x[u], a[u][kk][0], a[u][kk][1], a[u][kk][2], a[u][kk][3], b.x, b.y);
+            }
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float4 row = srow[t * 8 + 2 * q4 + e];
-            const int pos = __float_as_int(row.w);
-            const float f = row.x * ks, d = -row.y * ks - row.z;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float w = ex2(x[2 * i + e] * f + d);
-              if (kv_sees(p.mask, pos, j0 + 8 * i + g)) sum[i] += w;
+            for (int u = 0; u < kPairs; ++u) {
+              const float f = row.x * ks[u], d = -row.y * ks[u] - row.z;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float w = ex2(x[u][2 * i + e] * f + d);
+                if (!whole && ((j0[u] & kDead) || !kv_sees(p.mask, __float_as_int(row.w), (j0[u] & ~15) + 8 * i + place<D>(g))))
+                  w = 0.f;
+                sum[u][i] += w;
+              }
             }
           }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float v = sum[i];
-          v += __shfl_xor_sync(0xffffffffu, v, 1);
-          v += __shfl_xor_sync(0xffffffffu, v, 2);
-          const int j = j0 + 8 * i + g;
-          if (q4 == 0 && j <= chunk.last) score[j] += v;
-        }
+        for (int u = 0; u < kPairs; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float v = sum[u][i];
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            const int j = (j0[u] & ~15) + 8 * i + place<D>(g);
+            if (q4 == 0 && !(j0[u] & kDead) && j <= chunk.last) atomicAdd(score + j, v);
+          }
       }
+      taken += rounds * kPairs;
     }
   }
+}
+
+template <int D, int FMT>
+cudaError_t launch(const KvAttnParams& p, const CUtensorMap& map_k, unsigned blocks, const LaunchCfg& cfg) {
+  static SmemOptIn opt;
+  const cudaError_t e = allow_smem(kv_score_kernel<D, FMT>, kScoreSmem<D>, opt);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kv_score_kernel<D, FMT>, dim3(blocks), dim3(kWarps * 32), kScoreSmem<D>, cfg, p, map_k);
 }
 
 }  // namespace
@@ -153,10 +247,14 @@ cudaError_t launch_kv_score(const KvAttnParams& params, const LaunchCfg& cfg) {
   const int64_t steps = std::max<int64_t>(
       static_cast<int64_t>(p.c.S) * p.c.heads * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16), 1);
   p.few_steps = steps + static_cast<int64_t>(p.c.S) * p.c.heads * kItemCost <= 0x7fffffff;
-  const int64_t blocks = std::min<int64_t>(cfg.sms * 2, (steps + kWarps - 1) / kWarps);
-  auto kern = p.c.D == 128 ? (p.c.fmt == kKvInt8 ? kv_score_kernel<128, kKvInt8> : kv_score_kernel<128, kKvE4m3>)
-                           : (p.c.fmt == kKvInt8 ? kv_score_kernel<64, kKvInt8> : kv_score_kernel<64, kKvE4m3>);
-  return launch_kernel(kern, dim3(static_cast<unsigned>(blocks)), dim3(kWarps * 32), 0, cfg, p);
+  const int round = kWarps * (p.c.D == 64 ? kTogether<64> : kTogether<128>);
+  const int64_t blocks = std::min<int64_t>(cfg.sms * 2, (steps + round - 1) / round);
+  CUtensorMap map_k;
+  if (!kv_code_map(&map_k, p.c, p.c.k)) return cudaErrorInvalidValue;
+  const unsigned n = static_cast<unsigned>(blocks);
+  const bool i8 = p.c.fmt == kKvInt8;
+  if (p.c.D == 128) return i8 ? launch<128, kKvInt8>(p, map_k, n, cfg) : launch<128, kKvE4m3>(p, map_k, n, cfg);
+  return i8 ? launch<64, kKvInt8>(p, map_k, n, cfg) : launch<64, kKvE4m3>(p, map_k, n, cfg);
 }
 
 }  // namespace bolt

@@ -296,53 +296,52 @@ def Relu2(x):
 #   table i32 [S, width]: position j of sequence s is slot j % T of page table[s, j // T]
 #   start, lens i32 [S]: row r of a call is position start[s] + r, if that is below lens[s]
 # ---------------------------------------------------------------------------------------------
-def _kv_cache_args(op, k_cache, v_cache, k_scale, v_scale, table):
-    _need(k_cache, v_cache, k_scale, v_scale, table)
-    if not (k_cache.dtype == v_cache.dtype == torch.uint8 and k_scale.dtype == v_scale.dtype == torch.float32):
+def _kv_args(op, k_cache, v_cache, k_scale, v_scale, table, lens, start=None):
+    """Checks what the cache ops share; returns the shape arguments of the cache and the page table."""
+    start = lens if start is None else start
+    for t in (k_cache, v_cache, k_scale, v_scale, table, lens, start):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError("bolt ops take CUDA tensors (there is no CPU implementation)")
+        if not t.is_contiguous():
+            raise RuntimeError("bolt ops take contiguous tensors")
+    if not (k_cache.dtype is v_cache.dtype is torch.uint8 and k_scale.dtype is v_scale.dtype is torch.float32):
         raise RuntimeError(f"{op}: caches are u8, scales f32")
-    shape = k_cache.shape
-    if len(shape) != 4 or v_cache.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
+    shape, pages = k_cache.shape, k_scale.shape
+    if len(shape) != 4 or v_cache.shape != shape or pages != shape[:2] or v_scale.shape != pages:
         raise RuntimeError(f"{op}: cache must be [pages, heads, tokens, head size], scales [pages, heads]")
-    if table.dim() != 2:
+    if not (table.dtype is lens.dtype is start.dtype is torch.int32):
+        raise RuntimeError(f"{op}: page tables, starts and lengths are i32")
+    tables = table.shape
+    if len(tables) != 2:
         raise RuntimeError(f"{op}: page table must be [sequences, pages of a sequence]")
-
-
-def _kv_indices(op, sequences, *tensors):
-    for t in tensors:
-        if t.dtype != torch.int32:
-            raise RuntimeError(f"{op}: page tables, starts and lengths are i32")
-    for t in tensors[1:]:
-        if t.shape != (sequences,):
-            raise RuntimeError(f"{op}: starts and lengths must be [sequences]")
+    if lens.shape != tables[:1] or start.shape != tables[:1]:
+        raise RuntimeError(f"{op}: starts and lengths must be [sequences]")
+    return shape_arg(shape)[0], shape_arg(tables)[0]
 
 
 def _kv_rows(op, t, what):
-    """Strides of the sequence and row axes of rows [S, R, heads, D] whose last two axes are dense."""
+    """Shape argument of rows [S, R, heads, D] whose last two axes are dense, and that of the strides of the
+    sequence and row axes."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError("bolt ops take CUDA tensors (there is no CPU implementation)")
     if t.dtype != torch.bfloat16 or t.dim() != 4:
         raise RuntimeError(f"{op}: {what} must be bf16 [sequences, rows, heads, head size]")
     seq, row, head, one = t.stride()
-    D = t.shape[3]
-    if (one != 1 and D != 1) or (head != D and t.shape[2] != 1):
+    S, R, H, D = shape = t.shape
+    if (one != 1 and D != 1) or (head != D and H != 1):
         raise RuntimeError(f"{op}: {what} must be dense over its heads and values")
     # an axis of one entry has no step
-    return shape_arg((seq if t.shape[0] > 1 else 0, row if t.shape[1] > 1 else 0))
+    return shape_arg(shape)[0], shape_arg((seq if S > 1 else 0, row if R > 1 else 0))[0]
 
 
 def KvAppend(k, v, k_cache, v_cache, k_scale, v_scale, table, start, lens, fmt: int = KV_INT8):
     """Quantise the rows k, v bf16 [S, R, heads, D] into their pages, in place: a page's scale grows to
     max|x| / 127 (KV_INT8) or / 448 (KV_E4M3) where a row needs it, and its older codes with it."""
-    _kv_cache_args("KvAppend", k_cache, v_cache, k_scale, v_scale, table)
-    _need(start, lens)
-    _kv_indices("KvAppend", table.shape[0], table, start, lens)
-    ks, _k1 = _kv_rows("KvAppend", k, "k")
-    vs, _k2 = _kv_rows("KvAppend", v, "v")
+    cs, ts = _kv_args("KvAppend", k_cache, v_cache, k_scale, v_scale, table, lens, start)
+    shape, ks = _kv_rows("KvAppend", k, "k")
+    _, vs = _kv_rows("KvAppend", v, "v")
     if v.shape != k.shape:
         raise RuntimeError("KvAppend: k and v must have the same shape")
-    shape, _k3 = shape_arg(k.shape)
-    cs, _k4 = shape_arg(k_cache.shape)
-    ts, _k5 = shape_arg(table.shape)
     _check(lib().bolt_kv_append(_ptr(k), shape, ks, _ptr(v), vs, _ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale),
                                 _ptr(v_scale), _ptr(table), ts, _ptr(start), _ptr(lens), int(fmt), _stream(k_cache)))
 
@@ -350,14 +349,9 @@ def KvAppend(k, v, k_cache, v_cache, k_scale, v_scale, table, start, lens, fmt: 
 def KvRead(k_cache, v_cache, k_scale, v_scale, table, start, lens, rows: int, fmt: int = KV_INT8):
     """Returns (k, v) bf16 [S, rows, heads, D]: what the cache holds of the positions from start on, 0 from
     lens on."""
-    _kv_cache_args("KvRead", k_cache, v_cache, k_scale, v_scale, table)
-    _need(start, lens)
-    S = table.shape[0]
-    _kv_indices("KvRead", S, table, start, lens)
-    k = torch.empty(S, rows, k_cache.shape[1], k_cache.shape[3], dtype=torch.bfloat16, device=k_cache.device)
+    cs, ts = _kv_args("KvRead", k_cache, v_cache, k_scale, v_scale, table, lens, start)
+    k = k_cache.new_empty((table.shape[0], rows, k_cache.shape[1], k_cache.shape[3]), dtype=torch.bfloat16)
     v = torch.empty_like(k)
-    cs, _k1 = shape_arg(k_cache.shape)
-    ts, _k2 = shape_arg(table.shape)
     _check(lib().bolt_kv_read(_ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(table), ts,
                               _ptr(start), _ptr(lens), int(rows), int(fmt), _ptr(k), _ptr(v), _stream(k_cache)))
     return k, v
@@ -367,16 +361,12 @@ def KvAttention(q, k_cache, v_cache, k_scale, v_scale, table, start, lens, scale
                 sinks: int = 0, fmt: int = KV_INT8):
     """Returns (o bf16 [S, R, Hq, D], lse f32 [S, R, Hq]) of the rows q bf16 [S, R, Hq, D]: the row at
     position p sees the positions j <= p and, with a window, only j > p - window or j < sinks."""
-    _kv_cache_args("KvAttention", k_cache, v_cache, k_scale, v_scale, table)
-    _need(start, lens)
-    _kv_indices("KvAttention", table.shape[0], table, start, lens)
-    st, _k1 = _kv_rows("KvAttention", q, "q")
-    o = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    shape, _k2 = shape_arg(q.shape)
-    cs, _k3 = shape_arg(k_cache.shape)
-    ts, _k4 = shape_arg(table.shape)
-    ws = torch.empty(max(0, lib().bolt_kv_attention_workspace(shape, cs)), dtype=torch.uint8, device=q.device)
+    cs, ts = _kv_args("KvAttention", k_cache, v_cache, k_scale, v_scale, table, lens, start)
+    shape, st = _kv_rows("KvAttention", q, "q")
+    # new_empty of a tensor of the type: half the host time of torch.empty with a type and a device
+    o = q.new_empty(q.shape)
+    lse = k_scale.new_empty(q.shape[:3])
+    ws = k_cache.new_empty((max(0, lib().bolt_kv_attention_workspace(shape, cs)),))
     _check(lib().bolt_kv_attention(_ptr(q), shape, st, _ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
                                    _ptr(table), ts, _ptr(start), _ptr(lens), float(scale), int(window), int(sinks),
                                    int(fmt), _ptr(o), _ptr(lse), _ptr(ws), ws.numel(), _stream(k_cache)))
@@ -387,18 +377,13 @@ def KvScore(q, k_cache, k_scale, table, start, lens, lse, score, scale: float, w
             fmt: int = KV_INT8):
     """Adds every cached position's attention weight to score f32 [S, heads, >= width * T], in place (and
     returns it); q, the mask and lse as in the KvAttention call whose weights are taken."""
-    _kv_cache_args("KvScore", k_cache, k_cache, k_scale, k_scale, table)
-    _need(start, lens, lse, score)
-    S, heads = table.shape[0], k_cache.shape[1]
-    _kv_indices("KvScore", S, table, start, lens)
-    st, _k1 = _kv_rows("KvScore", q, "q")
+    cs, ts = _kv_args("KvScore", k_cache, k_cache, k_scale, k_scale, table, lens, start)
+    _need(lse, score)
+    shape, st = _kv_rows("KvScore", q, "q")
     if lse.dtype != torch.float32 or lse.shape != q.shape[:3]:
         raise RuntimeError("KvScore: lse must be f32 [sequences, rows, query heads]")
-    if score.dtype != torch.float32 or score.dim() != 3 or score.shape[:2] != (S, heads):
+    if score.dtype != torch.float32 or score.dim() != 3 or score.shape[:2] != (table.shape[0], k_cache.shape[1]):
         raise RuntimeError("KvScore: score must be f32 [sequences, heads, positions]")
-    shape, _k2 = shape_arg(q.shape)
-    cs, _k3 = shape_arg(k_cache.shape)
-    ts, _k4 = shape_arg(table.shape)
     _check(lib().bolt_kv_score(_ptr(q), shape, st, _ptr(k_cache), cs, _ptr(k_scale), _ptr(table), ts, _ptr(start),
                                _ptr(lens), _ptr(lse), float(scale), int(window), int(sinks), int(fmt), _ptr(score),
                                score.shape[2], _stream(k_cache)))
@@ -410,19 +395,16 @@ def KvEvict(k_cache, v_cache, k_scale, v_scale, table, lens, score, new_table, k
     """Cuts every (sequence, head) to its first `sinks` positions, its last `recent` and those of the largest
     score, `keep` in all, laid out in order in the pages of new_table i32 [S, >= keep / T].  Returns
     (kept i32 [S, heads, keep], new_lens i32 [S], new_score f32 [S, heads, keep])."""
-    _kv_cache_args("KvEvict", k_cache, v_cache, k_scale, v_scale, table)
-    _need(lens, score, new_table)
+    cs, ts = _kv_args("KvEvict", k_cache, v_cache, k_scale, v_scale, table, lens)
+    _need(score, new_table)
     S, heads = table.shape[0], k_cache.shape[1]
-    _kv_indices("KvEvict", S, table, lens)
     if new_table.dtype != torch.int32 or new_table.dim() != 2 or new_table.shape[0] != S:
         raise RuntimeError("KvEvict: the new page table must be i32 [sequences, pages of a sequence]")
     if score.dtype != torch.float32 or score.dim() != 3 or score.shape[:2] != (S, heads):
         raise RuntimeError("KvEvict: score must be f32 [sequences, heads, positions]")
-    kept = torch.empty(S, heads, keep, dtype=torch.int32, device=score.device)
-    new_lens = torch.empty(S, dtype=torch.int32, device=score.device)
-    new_score = torch.empty(S, heads, keep, dtype=torch.float32, device=score.device)
-    cs, _k1 = shape_arg(k_cache.shape)
-    ts, _k2 = shape_arg(table.shape)
+    kept = table.new_empty((S, heads, keep))
+    new_lens = torch.empty_like(lens)
+    new_score = score.new_empty((S, heads, keep))
     _check(lib().bolt_kv_evict(_ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(table), ts,
                                _ptr(lens), _ptr(score), score.shape[2], _ptr(new_table), new_table.shape[1],
                                int(keep), int(sinks), int(recent), int(fmt), _ptr(kept), _ptr(new_lens),
