@@ -13,26 +13,49 @@ __device__ __forceinline__ constexpr float kv_qmax() {
   return FMT == kKvInt8 ? 127.f : 448.f;
 }
 
-// The value (in units of the scale) of a code.
+// The values (in units of the scale) of a word's four codes, exact.
 template <int FMT>
-__device__ __forceinline__ float kv_decode(uint32_t code) {
+__device__ __forceinline__ void kv_decode4(uint32_t w, float (&x)[4]) {
   if constexpr (FMT == kKvInt8) {
-    return static_cast<float>(static_cast<int>(code) - 128);
+    // a byte under the exponent of 2^23 is 2^23 + code
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(prmt(w, 0x4B000000u, 0x7440u + e)) - 8388736.f;  // 2^23 + 128
   } else {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const __half2 h(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * e)), __NV_E4M3));
+      x[2 * e] = __low2float(h);
+      x[2 * e + 1] = __high2float(h);
+    }
   }
 }
 
-// The code nearest to x (in units of the scale), ties to even; NaN gives the code of 0.
+// The codes nearest to x (in units of the scale), ties to even; NaN gives the code of 0.
 template <int FMT>
-__device__ __forceinline__ uint32_t kv_encode(float x) {
+__device__ __forceinline__ uint32_t kv_encode4(const float (&x)[4]) {
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = x[e] != x[e] ? 0.f : x[e];
   if constexpr (FMT == kKvInt8) {
-    if (x != x) x = 0.f;
-    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f)) + 128);
+    // adding 1.5 * 2^23 rounds to a whole number, which the low byte then holds; 128 more for the offset
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(fminf(fmaxf(y[e], -127.f), 127.f) + 12582912.f);
+    return prmt(prmt(b[0], b[1], 0x0040u), prmt(b[2], b[3], 0x0040u), 0x5410u) ^ 0x80808080u;
   } else {
-    if (x != x) x = 0.f;
-    return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+    return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3)) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
   }
+}
+
+// A word's codes at ratio times their values.
+template <int FMT>
+__device__ __forceinline__ uint32_t kv_rescale4(uint32_t w, float ratio) {
+  float x[4];
+  kv_decode4<FMT>(w, x);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] *= ratio;
+  return kv_encode4<FMT>(x);
 }
 
 // Length of sequence s, and the position of its first row (the length, where it would lie beyond).

@@ -9,11 +9,15 @@
 // +-Q * s' and 0, and leave the rest of the page as it is.
 #include "kv.cuh"
 
+//
+// Both are streams of HBM bytes (append 2 in, 1 out a value; read 1 in, 2 out).  KvAppend gives a block the
+// new rows of one (page, head), which it holds in registers between the maximum and the rounding, so each
+// value is read once.
 namespace bolt {
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
 
 // max over the block of a non-negative value, for every thread
 __device__ __forceinline__ float block_max(float v, float* red) {
@@ -35,30 +39,21 @@ struct AppendParams {
   int blocks;  // most pages that a sequence's rows touch
 };
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-
-// one block per (sequence, touched page, head, K or V)
-template <int FMT>
+// one block per (sequence, touched page, head, K or V); a thread holds up to NV vectors of 8 values
+template <int FMT, int NV>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams p) {
   __shared__ float red[kThreads / 32];
   pdl_wait();
   pdl_trigger();
   const KvCache& c = p.c;
-  int64_t u = blockIdx.x;
+  unsigned u = blockIdx.x;
   const bool is_v = u & 1;
   u >>= 1;
   const int h = static_cast<int>(u % c.heads);
   u /= c.heads;
-  const int b = static_cast<int>(u % p.blocks), s = static_cast<int>(u / p.blocks);
+  const int s = static_cast<int>(u / p.blocks), b = static_cast<int>(u - s * p.blocks);
   const KvSeq q = kv_seq(c, p.rows.start, p.rows.lens, s);
-  const int end = min(static_cast<int64_t>(q.len), static_cast<int64_t>(q.start) + p.rows.R);
+  const int end = static_cast<int>(min(static_cast<int64_t>(q.len), static_cast<int64_t>(q.start) + p.rows.R));
   const int blk = (q.start >> c.tshift) + b;
   const int lo = blk << c.tshift;
   if (q.start >= end || lo >= end) return;
@@ -68,84 +63,126 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
   const int64_t unit = static_cast<int64_t>(page) * c.heads + h;
   uint8_t* codes = (is_v ? c.v : c.k) + unit * c.T * c.D;
   float* scale = (is_v ? c.vs : c.ks) + unit;
-  const bf16* src = (is_v ? p.v : p.k) + s * (is_v ? p.v_seq : p.k_seq) + static_cast<int64_t>(h) * c.D;
   const int64_t row_stride = is_v ? p.v_row : p.k_row;
-  const int vecs = c.D >> 3;  // vectors of 8 values a row
-  float amax = 0.f;
-  for (int i = threadIdx.x; i < (hi - first) * vecs; i += kThreads) {
-    const int r = first - q.start + i / vecs, d = (i % vecs) * 8;
-    float x[8];
-    unpack8(*reinterpret_cast<const uint4*>(src + r * row_stride + d), x);
+  const bf16* src = (is_v ? p.v : p.k) + s * (is_v ? p.v_seq : p.k_seq) + static_cast<int64_t>(h) * c.D +
+                    (first - q.start) * row_stride;
+  const int shift = c.D == 128 ? 4 : 3, n = (hi - first) << shift;  // vectors of 8 values
+  uint4 x[NV];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(x[e]);
-      if (a < INFINITY) amax = fmaxf(amax, a);
-    }
+  for (int i = 0; i < NV; ++i) {
+    const int at = threadIdx.x + i * kThreads;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (at < n) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (at >> shift) * row_stride) + (at & ((1 << shift) - 1)));
   }
   const float before = lo < q.start ? *scale : 0.f;
-  amax = block_max(amax, red);
-  const float after = fmaxf(before, amax / kv_qmax<FMT>());
-  if (threadIdx.x == 0) *scale = after;
-  if (first > lo && after > before) {
-    const float ratio = before / after;
-    uint32_t* w = reinterpret_cast<uint32_t*>(codes);
-    for (int i = threadIdx.x; i < (first - lo) * c.D / 4; i += kThreads) {
-      const uint32_t x = w[i];
-      uint32_t y = 0;
+  float amax = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y |= kv_encode<FMT>(kv_decode<FMT>((x >> (8 * e)) & 255) * ratio) << (8 * e);
-      w[i] = y;
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = fabsf(__uint_as_float(w[e] << 16)), b2 = fabsf(__uint_as_float(w[e] & 0xFFFF0000u));
+      if (a < INFINITY) amax = fmaxf(amax, a);
+      if (b2 < INFINITY) amax = fmaxf(amax, b2);
     }
   }
-  for (int i = threadIdx.x; i < (hi - first) * vecs; i += kThreads) {
-    const int t = first + i / vecs, d = (i % vecs) * 8;
-    float x[8];
-    unpack8(*reinterpret_cast<const uint4*>(src + (t - q.start) * row_stride + d), x);
-    uint32_t y[2] = {0, 0};
+  amax = block_max(amax, red);
+  const float after = fmaxf(before, amax / kv_qmax<FMT>());
+  if (threadIdx.x == 0) *scale = after;  // every thread has read it: block_max has a barrier
+  if (first > lo && after > before) {
+    const float ratio = before / after;
+    uint4* w = reinterpret_cast<uint4*>(codes);
+    for (int i = threadIdx.x; i < (first - lo) * c.D / 16; i += kThreads) {
+      const uint4 y = w[i];
+      w[i] = make_uint4(kv_rescale4<FMT>(y.x, ratio), kv_rescale4<FMT>(y.y, ratio), kv_rescale4<FMT>(y.z, ratio),
+                        kv_rescale4<FMT>(y.w, ratio));
+    }
+  }
+  uint2* out = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(first - lo) * c.D);
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      y[e >> 2] |= kv_encode<FMT>(after > 0.f ? x[e] / after : 0.f) << (8 * (e & 3));
-    *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(t - lo) * c.D + d) = make_uint2(y[0], y[1]);
+  for (int i = 0; i < NV; ++i) {
+    const int at = threadIdx.x + i * kThreads;
+    if (at >= n) break;
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    uint32_t y[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float z[4] = {__uint_as_float(w[2 * e] << 16), __uint_as_float(w[2 * e] & 0xFFFF0000u),
+                    __uint_as_float(w[2 * e + 1] << 16), __uint_as_float(w[2 * e + 1] & 0xFFFF0000u)};
+#pragma unroll
+      for (int f = 0; f < 4; ++f) z[f] = after > 0.f ? z[f] / after : 0.f;
+      y[e] = kv_encode4<FMT>(z);
+    }
+    out[at] = make_uint2(y[0], y[1]);
   }
 }
 
-// one thread per 8 values of a (sequence, row, head)
+// Block y: a sequence.  A thread takes vectors of 16 values of a (row, head), kReadVecs of them.
+constexpr int kReadVecs = 2;
 template <int FMT>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCache c, const KvRows rows, bf16* k, bf16* v,
-                                                           int64_t n) {
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCache c, const KvRows rows, bf16* k, bf16* v) {
   pdl_wait();
   pdl_trigger();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= n) return;
-  const int vecs = c.D >> 3;
-  int64_t u = i;
-  const int d = static_cast<int>(u % vecs) * 8;
-  u /= vecs;
-  const int h = static_cast<int>(u % c.heads);
-  u /= c.heads;
-  const int r = static_cast<int>(u % rows.R), s = static_cast<int>(u / rows.R);
+  const int s = blockIdx.y, shift = c.D == 128 ? 3 : 2;
   const KvSeq q = kv_seq(c, rows.start, rows.lens, s);
-  const int64_t pos = static_cast<int64_t>(q.start) + r;
-  const int page = pos < q.len ? kv_page(c.table, c.width, c.pages, s, static_cast<int>(pos >> c.tshift)) : -1;
+  const int64_t n = static_cast<int64_t>(rows.R) * c.heads << shift;  // vectors of the sequence
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kReadVecs) + threadIdx.x;
+  uint4 x[kReadVecs][2];
+  float sc[kReadVecs][2];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (page >= 0) {
-      const int64_t unit = static_cast<int64_t>(page) * c.heads + h;
-      const float sc = (kv ? c.vs : c.ks)[unit];
-      const uint2 x = *reinterpret_cast<const uint2*>((kv ? c.v : c.k) + (unit * c.T + (pos & (c.T - 1))) * c.D + d);
-      uint32_t y[4];
+  for (int i = 0; i < kReadVecs; ++i) {
+    const int64_t at = i0 + i * kThreads;
+    x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+    sc[i][0] = sc[i][1] = 0.f;
+    if (at >= n) break;
+    const int64_t rh = at >> shift;
+    const int r = rh <= 0x7fffffff ? static_cast<int>(static_cast<unsigned>(rh) / static_cast<unsigned>(c.heads))
+                                   : static_cast<int>(rh / c.heads);
+    const int h = static_cast<int>(rh - static_cast<int64_t>(r) * c.heads);
+    const int64_t pos = static_cast<int64_t>(q.start) + r;
+    if (pos >= q.len) continue;
+    const int page = kv_page(c.table, c.width, c.pages, s, static_cast<int>(pos >> c.tshift));
+    if (page < 0) continue;
+    const int64_t unit = static_cast<int64_t>(page) * c.heads + h;
+    const int64_t from = ((unit << c.tshift) + (pos & (c.T - 1))) * c.D + (at & ((1 << shift) - 1)) * 16;
+    x[i][0] = *reinterpret_cast<const uint4*>(c.k + from);
+    x[i][1] = *reinterpret_cast<const uint4*>(c.v + from);
+    sc[i][0] = c.ks[unit];
+    sc[i][1] = c.vs[unit];
+  }
+#pragma unroll
+  for (int i = 0; i < kReadVecs; ++i) {
+    const int64_t at = i0 + i * kThreads;
+    if (at >= n) break;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint32_t w[4] = {x[i][kv].x, x[i][kv].y, x[i][kv].z, x[i][kv].w};
+      uint32_t y[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t w = (e < 2 ? x.x : x.y) >> (16 * (e & 1));
-        const __nv_bfloat162 pair =
-            __floats2bfloat162_rn(kv_decode<FMT>(w & 255) * sc, kv_decode<FMT>((w >> 8) & 255) * sc);
-        y[e] = *reinterpret_cast<const uint32_t*>(&pair);
+        float z[4];
+        kv_decode4<FMT>(w[e], z);
+        const __nv_bfloat162 a = __floats2bfloat162_rn(z[0] * sc[i][kv], z[1] * sc[i][kv]);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(z[2] * sc[i][kv], z[3] * sc[i][kv]);
+        y[2 * e] = *reinterpret_cast<const uint32_t*>(&a);
+        y[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&b);
       }
-      out = make_uint4(y[0], y[1], y[2], y[3]);
+      uint4* out = reinterpret_cast<uint4*>((kv ? v : k) + (static_cast<int64_t>(s) * n + at) * 16);
+      __stcs(out, make_uint4(y[0], y[1], y[2], y[3]));
+      __stcs(out + 1, make_uint4(y[4], y[5], y[6], y[7]));
     }
-    *reinterpret_cast<uint4*>((kv ? v : k) + i * 8) = out;
   }
+}
+
+template <int FMT>
+cudaError_t append(const AppendParams& p, unsigned grid, const LaunchCfg& cfg) {
+  const int per_thread = (p.c.T * p.c.D / 8 + kThreads - 1) / kThreads;  // vectors of a page: 1 .. 16
+  auto kern = per_thread <= 1   ? kv_append_kernel<FMT, 1>
+              : per_thread <= 2 ? kv_append_kernel<FMT, 2>
+              : per_thread <= 4 ? kv_append_kernel<FMT, 4>
+              : per_thread <= 8 ? kv_append_kernel<FMT, 8>
+                                : kv_append_kernel<FMT, 16>;
+  return launch_kernel(kern, dim3(grid), dim3(kThreads), 0, cfg, p);
 }
 
 }  // namespace
@@ -157,16 +194,16 @@ cudaError_t launch_kv_append(const KvCache& c, const KvRows& rows, const bf16* k
   p.blocks = static_cast<int>(std::min<int64_t>((static_cast<int64_t>(rows.R) + c.T - 2) / c.T + 1, c.width));
   const int64_t grid = static_cast<int64_t>(c.S) * p.blocks * c.heads * 2;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return launch_kernel(c.fmt == kKvInt8 ? kv_append_kernel<kKvInt8> : kv_append_kernel<kKvE4m3>,
-                       dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, cfg, p);
+  const unsigned n = static_cast<unsigned>(grid);
+  return c.fmt == kKvInt8 ? append<kKvInt8>(p, n, cfg) : append<kKvE4m3>(p, n, cfg);
 }
 
 cudaError_t launch_kv_read(const KvCache& c, const KvRows& rows, bf16* k, bf16* v, const LaunchCfg& cfg) {
-  const int64_t n = static_cast<int64_t>(c.S) * rows.R * c.heads * (c.D >> 3);
-  const int64_t grid = (n + kThreads - 1) / kThreads;
+  const int64_t n = static_cast<int64_t>(rows.R) * c.heads * (c.D >> 4);
+  const int64_t grid = (n + kThreads * kReadVecs - 1) / (kThreads * kReadVecs);
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
   return launch_kernel(c.fmt == kKvInt8 ? kv_read_kernel<kKvInt8> : kv_read_kernel<kKvE4m3>,
-                       dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, cfg, c, rows, k, v, n);
+                       dim3(static_cast<unsigned>(grid), static_cast<unsigned>(c.S)), dim3(kThreads), 0, cfg, c, rows, k, v);
 }
 
 }  // namespace bolt
