@@ -30,22 +30,28 @@ __device__ __forceinline__ void kv_decode4(uint32_t w, float (&x)[4]) {
   }
 }
 
-// The codes nearest to x (in units of the scale), ties to even; NaN gives the code of 0.
+// The codes nearest to x (in units of the scale; finite), ties to even.
+template <int FMT>
+__device__ __forceinline__ uint32_t kv_encode4_finite(const float (&x)[4]) {
+  if constexpr (FMT == kKvInt8) {
+    // adding 1.5 * 2^23 rounds to a whole number, which the low byte then holds; 128 more for the offset
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(fminf(fmaxf(x[e], -127.f), 127.f) + 12582912.f);
+    return prmt(prmt(b[0], b[1], 0x0040u), prmt(b[2], b[3], 0x0040u), 0x5410u) ^ 0x80808080u;
+  } else {
+    return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3)) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
+  }
+}
+
+// The same of any x: infinities give the largest codes, NaN the code of 0.
 template <int FMT>
 __device__ __forceinline__ uint32_t kv_encode4(const float (&x)[4]) {
   float y[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = x[e] != x[e] ? 0.f : x[e];
-  if constexpr (FMT == kKvInt8) {
-    // adding 1.5 * 2^23 rounds to a whole number, which the low byte then holds; 128 more for the offset
-    uint32_t b[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(fminf(fmaxf(y[e], -127.f), 127.f) + 12582912.f);
-    return prmt(prmt(b[0], b[1], 0x0040u), prmt(b[2], b[3], 0x0040u), 0x5410u) ^ 0x80808080u;
-  } else {
-    return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3)) |
-           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
-  }
+  return kv_encode4_finite<FMT>(y);
 }
 
 // A word's codes at ratio times their values.

@@ -19,16 +19,63 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// max over the block of a non-negative value, for every thread
+// max over the block of a value that is not negative (NaN, if any is), for every thread
 __device__ __forceinline__ float block_max(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  // of such values the bits are in their order, and NaN's the largest
+  unsigned m = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+  __syncthreads();  // red may hold an earlier maximum
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = __uint_as_float(m);
   __syncthreads();
-  v = red[0];
 #pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, red[w]);
-  return v;
+  for (int w = 0; w < kThreads / 32; ++w) m = max(m, __float_as_uint(red[w]));
+  return __uint_as_float(m);
+}
+
+__device__ __forceinline__ void unpack4(uint32_t a, uint32_t b, float (&x)[4]) {
+  x[0] = __uint_as_float(a << 16);
+  x[1] = __uint_as_float(a & 0xFFFF0000u);
+  x[2] = __uint_as_float(b << 16);
+  x[3] = __uint_as_float(b & 0xFFFF0000u);
+}
+
+// Codes of four finite bf16 values of at most Q * s, by the definition round(x / s), where they are the same at
+// x * lo and x * hi, lo and hi being 1 / s less and more 2^-21 of it: x / s and its rounding to fp32 lie
+// between.  Otherwise (a value that close to a tie; rare) sets bits of `near`.  A division for every value
+// takes several times the operations, and these are what bounds the kernel.
+template <int FMT>
+__device__ __forceinline__ uint32_t quantise4(uint32_t a, uint32_t b, float lo, float hi, uint32_t& near) {
+  float x[4];
+  unpack4(a, b, x);
+  if constexpr (FMT == kKvInt8) {
+    uint32_t c[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // 1.5 * 2^23 more: the low byte is the rounded value
+      c[e] = __float_as_uint(fmaf(x[e], lo, 12582912.f));
+      near |= c[e] ^ __float_as_uint(fmaf(x[e], hi, 12582912.f));
+    }
+    return prmt(prmt(c[0], c[1], 0x0040u), prmt(c[2], c[3], 0x0040u), 0x5410u) ^ 0x80808080u;
+  } else {
+    float y[4], z[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = x[e] * lo;
+      z[e] = x[e] * hi;
+    }
+    const uint32_t c = kv_encode4_finite<FMT>(y);
+    near |= c ^ kv_encode4_finite<FMT>(z);
+    return c;
+  }
+}
+
+// ... and by the division itself; any x.
+template <int FMT>
+__device__ __forceinline__ uint32_t divide4(uint32_t a, uint32_t b, float s) {
+  float x[4];
+  unpack4(a, b, x);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = s > 0.f ? x[e] / s : 0.f;
+  return kv_encode4<FMT>(x);
 }
 
 struct AppendParams {
@@ -57,12 +104,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
   const int blk = (q.start >> c.tshift) + b;
   const int lo = blk << c.tshift;
   if (q.start >= end || lo >= end) return;
-  const int page = kv_page(c.table, c.width, c.pages, s, blk);
-  if (page < 0) return;
   const int hi = min(lo + c.T, end), first = max(lo, q.start);
-  const int64_t unit = static_cast<int64_t>(page) * c.heads + h;
-  uint8_t* codes = (is_v ? c.v : c.k) + unit * c.T * c.D;
-  float* scale = (is_v ? c.vs : c.ks) + unit;
   const int64_t row_stride = is_v ? p.v_row : p.k_row;
   const bf16* src = (is_v ? p.v : p.k) + s * (is_v ? p.v_seq : p.k_seq) + static_cast<int64_t>(h) * c.D +
                     (first - q.start) * row_stride;
@@ -74,19 +116,33 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
     x[i] = make_uint4(0, 0, 0, 0);
     if (at < n) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + (at >> shift) * row_stride) + (at & ((1 << shift) - 1)));
   }
+  const int page = kv_page(c.table, c.width, c.pages, s, blk);
+  if (page < 0) return;
+  const int64_t unit = static_cast<int64_t>(page) * c.heads + h;
+  uint8_t* codes = (is_v ? c.v : c.k) + unit * c.T * c.D;
+  float* scale = (is_v ? c.vs : c.ks) + unit;
   const float before = lo < q.start ? *scale : 0.f;
-  float amax = 0.f;
+  __nv_bfloat162 top = __float2bfloat162_rn(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float a = fabsf(__uint_as_float(w[e] << 16)), b2 = fabsf(__uint_as_float(w[e] & 0xFFFF0000u));
-      if (a < INFINITY) amax = fmaxf(amax, a);
-      if (b2 < INFINITY) amax = fmaxf(amax, b2);
+      const uint32_t a = w[e] & 0x7FFF7FFFu;
+      top = __hmax2_nan(top, *reinterpret_cast<const __nv_bfloat162*>(&a));
     }
   }
-  amax = block_max(amax, red);
+  float amax = block_max(__bfloat162float(__hmax_nan(top.x, top.y)), red);
+  const bool odd = !(amax < INFINITY);  // an infinity or a NaN among the values: the largest of the others
+  if (odd) {
+    amax = 0.f;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n * 8; i += kThreads) {
+      const float a = fabsf(__bfloat162float(src[(i >> (shift + 3)) * row_stride + (i & ((8 << shift) - 1))]));
+      if (a < INFINITY) amax = fmaxf(amax, a);
+    }
+    amax = block_max(amax, red);
+  }
   const float after = fmaxf(before, amax / kv_qmax<FMT>());
   if (threadIdx.x == 0) *scale = after;  // every thread has read it: block_max has a barrier
   if (first > lo && after > before) {
@@ -99,28 +155,28 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
     }
   }
   uint2* out = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(first - lo) * c.D);
+  const bool exact = odd || !(after >= 0x1p-100f);  // every value by division
+  const float inv = 1.f / after, inv_lo = inv * (1.f - 0x1p-21f), inv_hi = inv * (1.f + 0x1p-21f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int at = threadIdx.x + i * kThreads;
     if (at >= n) break;
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-    uint32_t y[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float z[4] = {__uint_as_float(w[2 * e] << 16), __uint_as_float(w[2 * e] & 0xFFFF0000u),
-                    __uint_as_float(w[2 * e + 1] << 16), __uint_as_float(w[2 * e + 1] & 0xFFFF0000u)};
-#pragma unroll
-      for (int f = 0; f < 4; ++f) z[f] = after > 0.f ? z[f] / after : 0.f;
-      y[e] = kv_encode4<FMT>(z);
+    uint32_t near = exact;
+    uint2 y;
+    y.x = quantise4<FMT>(x[i].x, x[i].y, inv_lo, inv_hi, near);
+    y.y = quantise4<FMT>(x[i].z, x[i].w, inv_lo, inv_hi, near);
+    if (near) {
+      y.x = divide4<FMT>(x[i].x, x[i].y, after);
+      y.y = divide4<FMT>(x[i].z, x[i].w, after);
     }
-    out[at] = make_uint2(y[0], y[1]);
+    out[at] = y;
   }
 }
 
 // Block y: a sequence.  A thread takes vectors of 16 values of a (row, head), kReadVecs of them.
-constexpr int kReadVecs = 2;
+constexpr int kReadVecs = 1;
 template <int FMT>
-__global__ void __launch_bounds__(kThreads) kv_read_kernel(const KvCache c, const KvRows rows, bf16* k, bf16* v) {
+__global__ void __launch_bounds__(kThreads, 8) kv_read_kernel(const KvCache c, const KvRows rows, bf16* k, bf16* v) {
   pdl_wait();
   pdl_trigger();
   const int s = blockIdx.y, shift = c.D == 128 ? 3 : 2;

@@ -8,7 +8,7 @@
 // code c of a position with scale s becomes round(c * (s / s')), so codes whose scale is the page's
 // largest stay as they are.
 //
-// Two kernels.  Selection, one block per (sequence, head): the ranks go to shared memory once (up to
+// Two kernels.  Selection, one block per (sequence, head): the weights go to shared memory once (up to
 // kSelKeys positions), the cut is found eleven bits at a time by histograms, and the kept positions are
 // written in order.  Then the codes move, one block per (sequence, head, 128 positions or one page of 256):
 // look-ups of positions, pages and scales serve K and V, and the copies are 16 bytes a thread.
@@ -28,6 +28,12 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   if (x != x) return 0xFFFFFFFFu;
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// Sum of the first `warp` of 32 sums, one a warp of the block.
+__device__ __forceinline__ unsigned sum_before(const unsigned* sums, int warp) {
+  const int lane = threadIdx.x & 31;
+  return __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0u);
 }
 
 // Of the 32-bit ranks get(i), lo <= i < hi: the left-th largest; `left` becomes the number of those equal
@@ -57,8 +63,7 @@ __device__ __forceinline__ uint32_t find_cut(Get&& get, int lo, int hi, int& lef
     }
     if (lane == 31) warp_sums[warp] = sum;
     __syncthreads();
-    unsigned before = sum - a - b;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
+    const unsigned before = sum - a - b + sum_before(warp_sums, warp);
     const unsigned need = static_cast<unsigned>(left);
     if (before < need && need <= before + a)
       *found = make_uint2(top, need - before);
@@ -74,9 +79,8 @@ __device__ __forceinline__ uint32_t find_cut(Get&& get, int lo, int hi, int& lef
 }
 
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const KvEvictParams p, int key_room) {
-  extern __shared__ uint32_t keys[];  // [key_room]
-  __shared__ unsigned hist[kBins], warp_sums[kSelThreads / 32];
-  __shared__ int2 kept_sums[kSelThreads / 32];
+  extern __shared__ float keys[];  // [key_room]
+  __shared__ unsigned hist[kBins], warp_sums[kSelThreads / 32], above_sums[kSelThreads / 32], equal_sums[kSelThreads / 32];
   __shared__ uint2 found;
   pdl_wait();
   pdl_trigger();
@@ -100,10 +104,11 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const KvEvictPar
   const bool some = left > 0, in_smem = n <= key_room;
   if (in_smem) {
 #pragma unroll 8
-    for (int i = tid; i < n; i += kSelThreads) keys[i] = rank_of(score[i]);
+    for (int i = tid; i < n; i += kSelThreads) keys[i] = score[i];
     __syncthreads();
   }
-  const auto get = [&](int i) { return in_smem ? keys[i] : rank_of(score[i]); };
+  const auto weight = [&](int i) { return in_smem ? keys[i] : score[i]; };
+  const auto get = [&](int i) { return rank_of(weight(i)); };
   const uint32_t cut = some ? find_cut(get, lo, hi, left, hist, warp_sums, &found) : 0;
   // every rank above `cut` is kept, and the first `left` equal to it; a warp takes consecutive positions
   const int per = ((n + kSelThreads - 1) / kSelThreads) * 32, i0 = min(warp * per, n), i1 = min(i0 + per, n);
@@ -118,13 +123,12 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const KvEvictPar
     above += __popc(__ballot_sync(0xffffffffu, k == 2));
     equal += __popc(__ballot_sync(0xffffffffu, k == 1));
   }
-  if (lane == 0) kept_sums[warp] = make_int2(above, equal);
-  __syncthreads();
-  int a = 0, e = 0;
-  for (int w = 0; w < warp; ++w) {
-    a += kept_sums[w].x;
-    e += kept_sums[w].y;
+  if (lane == 0) {
+    above_sums[warp] = above;
+    equal_sums[warp] = equal;
   }
+  __syncthreads();
+  int a = sum_before(above_sums, warp), e = sum_before(equal_sums, warp);
   const unsigned lower = (1u << lane) - 1;
   for (int i = i0; i < i1; i += 32) {
     const int k = i + lane < i1 ? class_of(i + lane) : 0;
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const KvEvictPar
     if (k == 2 || (k == 1 && my_e < left)) {
       const int at = a + __popc(ma & lower) + min(my_e, left);
       kept[at] = i + lane;
-      out[at] = score[i + lane];
+      out[at] = weight(i + lane);
     }
     a += __popc(ma);
     e += __popc(me);
