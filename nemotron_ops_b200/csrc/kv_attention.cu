@@ -17,26 +17,14 @@
 // and a reference m that is raised to the row's maximum only when some x passes m + 7: weights stay
 // below 2^15, those down to 2^-22 of the reference keep all 11 bits, and most steps need neither the
 // maximum over the row's lanes nor a rescaling.
-#include "kv_mma.cuh"
-#include "tensor_map.h"
+#include "kv_split.cuh"
 
 namespace bolt {
 
 namespace {
 
-constexpr float kWeightLog = 8.f, kWeightTop = 15.f;
-
-struct Split {   // segments of one item: the first in block `block`'s slot 2 block + 1, the i-th in 2 (block + i)
-  int s, mb, h, block, parts;
-};
-
-struct Work {
-  float* part;    // [2 blocks][rows of a block][D]
-  float2* ml;     // [2 blocks][rows of a block]: max and sum
-  Split* split;   // [splits]
-  int splits;     // min(items, blocks): an entry an item, or an entry a block
-  int row_blocks;
-};
+// Of an item's set-up, in steps: about 6 us, measured in a batch of 64 sequences of up to 8,192 positions.
+constexpr int kItemCost = 16;
 
 // NT tiles of 8 rows a warp, MW warps along the rows, TW along the steps; a warp takes NP steps at a
 // time, from a ring of STAGES steps.
@@ -54,10 +42,12 @@ struct Tile {
 
 // float4 index f of a row's values in the joining buffer, spread over the banks
 template <int D>
-__device__ __forceinline__ int swizzle(int row, int f) {
-  const int c = (row >> 1) & 3;
-  return f ^ (D == 128 ? c : (c & 1) | (c >> 1) << 2);
-}
+struct Swizzle {
+  __device__ __forceinline__ int operator()(int row, int f) const {
+    const int c = (row >> 1) & 3;
+    return f ^ (D == 128 ? c : (c & 1) | (c >> 1) << 2);
+  }
+};
 
 // An 8 x 8 matrix of halves, two neighbours of a row a lane, transposed.
 __device__ __forceinline__ uint32_t transpose8(__half2 x) {
@@ -110,8 +100,6 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
   const int mw = warp % MW, tk = warp / MW;
   uint8_t* ring = reinterpret_cast<uint8_t*>(smem + warp * STAGES * L::kStep);
   const unsigned M = static_cast<unsigned>(p.rows.R) * p.G, G = p.G;
-  const int pairs = c.S * w.row_blocks;
-  const bool by_item = static_cast<int64_t>(pairs) * c.heads == w.splits;
   s_scale += warp * 64;
   s_row += warp * 64;
   s_full += warp * STAGES;
@@ -125,50 +113,16 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
   bool stuck = false;   // a copy did not arrive in time: the rest of the work is left
   const int k_at = kv_at<D>(place<D>(g), 16 * q4);  // the codes 64 i + 16 q4 .. are at k_at ^ 64 i
   const int v_at[2] = {kv_at<D>(place<D>(2 * q4), D / 8 * g), kv_at<D>(place<D>(2 * q4 + 1), D / 8 * g)};
-  const KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW * NP);
+  const KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW * NP, kItemCost);
 
-  if (!by_item && tid == 0) w.split[blockIdx.x].parts = 0;
-  // items without steps: their rows see nothing
-  for (int i = blockIdx.x; i < pairs; i += gridDim.x) {
-    const int s = i / w.row_blocks;
-    const unsigned m0 = (i - s * w.row_blocks) * L::kRows;
-    if (kv_span(p, kv_seq(c, p.rows.start, p.rows.lens, s), m0, L::kRows).n > 0) continue;
-    const unsigned rows = min(M - m0, static_cast<unsigned>(L::kRows)) * c.heads;
-    for (unsigned e = tid; e < rows * (D / 8); e += L::kThreads) {
-      const unsigned row = e / (D / 8), h = row % c.heads, m = m0 + row / c.heads, r = m / G;
-      const int64_t out = (static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * G + (m - r * G);
-      reinterpret_cast<uint4*>(p.o + out * D)[e % (D / 8)] = make_uint4(0, 0, 0, 0);
-      if (e % (D / 8) == 0) p.lse[out] = -INFINITY;
-    }
-    if (by_item)
-      for (int h = tid; h < c.heads; h += L::kThreads) w.split[static_cast<int64_t>(i) * c.heads + h].parts = 0;
-  }
+  kv_empty_items<D, L::kRows, L::kThreads>(p, w);
 
-  int64_t left = share.left, off = share.off, at = share.at;
-  for (int pair = share.pair; left > 0;) {
-    const int s = pair / w.row_blocks, mb = pair - s * w.row_blocks;
-    const unsigned m0 = static_cast<unsigned>(mb) * L::kRows;
-    const KvSeq seq = kv_seq(c, p.rows.start, p.rows.lens, s);
-    const KvSpan span = kv_span(p, seq, m0, L::kRows);
-    if (span.n == 0) {
-      ++pair;
-      continue;
-    }
-    // units u0 .. u1 - 1 of the item, of which those from share.cost on are its steps
-    const int size = span.n + share.cost;
-    const int h = static_cast<int>(kv_div(off, size)), u0 = static_cast<int>(off - static_cast<int64_t>(h) * size);
-    const int u1 = static_cast<int>(min(static_cast<int64_t>(size), u0 + left));
-    const int i0 = max(0, u0 - share.cost), i1 = max(0, u1 - share.cost);
-    const int64_t end = at - u0 + size;  // on the axis, behind this item
-    left -= u1 - u0;
-    at += u1 - u0;
-    off += u1 - u0;
-    const int item_pair = pair;
-    if (off == static_cast<int64_t>(size) * c.heads) {
-      ++pair;
-      off = 0;
-    }
-    if (i0 == i1) continue;
+  KvWalk walk(share);
+  for (KvSegment seg; walk.next(p, w.row_blocks, L::kRows, seg);) {
+    const int s = seg.s, h = seg.h, i0 = seg.i0, i1 = seg.i1;
+    const unsigned m0 = seg.m0;
+    const KvSeq& seq = seg.seq;
+    const KvSpan& span = seg.span;
 
     // ---- the segment: steps i0 .. i1 - 1; this warp's k-th is the k % NP-th of the group k / NP * TW + tk
     const unsigned m1 = m0 + mw * NT * 8;  // this warp's first row
@@ -449,63 +403,11 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
         for (int t = 0; t < D / 16; t += 2) {
           float4 v = make_float4(o[r][t][e] * f, o[r][t][2 + e] * f, o[r][t + 1][e] * f, o[r][t + 1][2 + e] * f);
           if (f == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-          to[swizzle<D>(row, D / 32 * g + t / 2)] = v;
+          to[Swizzle<D>()(row, D / 32 * g + t / 2)] = v;
         }
       }
     __syncthreads();
-    const bool item = i0 == 0 && i1 == span.n;
-    const int slot = 2 * blockIdx.x + (i0 == 0);
-    if (!item && i0 == 0 && tid == 0) {
-      const int parts = share.cross ? static_cast<int>((end - 1) / share.per) - static_cast<int>(blockIdx.x) + 1
-                                    : static_cast<int>((span.n + share.per - 1) / share.per);
-      w.split[by_item ? static_cast<int64_t>(item_pair) * c.heads + h : blockIdx.x] =
-          Split{s, mb, h, static_cast<int>(blockIdx.x), parts};
-    }
-    if (item && by_item && tid == 0) w.split[static_cast<int64_t>(item_pair) * c.heads + h].parts = 0;
-    for (int e = tid; e < L::kRows * (D / 8); e += L::kThreads) {
-      const int row = e / (D / 8), f = 2 * (e % (D / 8));
-      const unsigned m = m0 + row;
-      if (m >= M) break;
-      float top = sm[row];
-#pragma unroll
-      for (int k = 1; k < TW; ++k) top = fmaxf(top, sm[k * L::kRows + row]);
-      float l = 0.f;
-      float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll
-      for (int k = 0; k < TW; ++k) {
-        const float mk = sm[k * L::kRows + row];
-        if (mk != -INFINITY) l += sl[k * L::kRows + row] * ex2(mk - top);
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float4 z = so[(k * L::kRows + row) * (D / 4) + swizzle<D>(row, f + y)];
-          v[y].x += z.x;
-          v[y].y += z.y;
-          v[y].z += z.z;
-          v[y].w += z.w;
-        }
-      }
-      if (item) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const unsigned r = m / G;
-        const int64_t out = (static_cast<int64_t>(s) * p.rows.R + r) * p.Hq + h * G + (m - r * G);
-        uint4 u;
-        __nv_bfloat162 y0 = __floats2bfloat162_rn(v[0].x * inv, v[0].y * inv);
-        __nv_bfloat162 y1 = __floats2bfloat162_rn(v[0].z * inv, v[0].w * inv);
-        __nv_bfloat162 y2 = __floats2bfloat162_rn(v[1].x * inv, v[1].y * inv);
-        __nv_bfloat162 y3 = __floats2bfloat162_rn(v[1].z * inv, v[1].w * inv);
-        u.x = *reinterpret_cast<uint32_t*>(&y0);
-        u.y = *reinterpret_cast<uint32_t*>(&y1);
-        u.z = *reinterpret_cast<uint32_t*>(&y2);
-        u.w = *reinterpret_cast<uint32_t*>(&y3);
-        *reinterpret_cast<uint4*>(p.o + out * D + 4 * f) = u;
-        if (f == 0) p.lse[out] = l > 0.f ? (top - kWeightLog + log2f(l)) * kLn2 : -INFINITY;
-      } else {
-        float4* to = reinterpret_cast<float4*>(w.part + (static_cast<int64_t>(slot) * L::kRows + row) * D) + f;
-        to[0] = v[0];
-        to[1] = v[1];
-        if (f == 0) w.ml[static_cast<int64_t>(slot) * L::kRows + row] = make_float2(top, l);
-      }
-    }
+    kv_finish<D, L::kRows, TW, L::kThreads>(p, w, share, seg, sm, sl, so, Swizzle<D>());
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next segment's copies come after these reads and writes
     __syncthreads();
   }
@@ -582,7 +484,7 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(co
 
 // The tiling for M = R * G rows a kv head.  Up to 16 rows: tiles of 8 or 16 rows whose steps four warps
 // share, several blocks an SM.  More: 32 rows a warp, so that a converted operand serves four tiles, one
-// block an SM.
+// block an SM; beyond 64 rows the tensor-memory kernel (kv_attention_umma.cu).
 struct Plan {
   int rows, round, per_sm;
 };
@@ -591,7 +493,7 @@ Plan plan_of(int64_t M) {
   if (M <= 16) return Plan{16, 4, 2};
   if (M <= 32) return Plan{32, 8, 1};
   if (M <= 64) return Plan{64, 4, 1};
-  return Plan{128, 2, 1};
+  return Plan{128, 8, 1};
 }
 
 template <int D, int FMT, int NT, int MW, int TW, int NP, int STAGES, int CPS>
@@ -613,7 +515,7 @@ cudaError_t launch_rows(const KvAttnParams& p, const Work& w, int rows, unsigned
     case 16: return launch<D, FMT, 2, 1, 4, 1, 4, 2>(p, w, blocks, cfg);
     case 32: return launch<D, FMT, 4, 1, 8, 1, 4, 1>(p, w, blocks, cfg);
     case 64: return launch<D, FMT, 4, 2, 4, 1, 4, 1>(p, w, blocks, cfg);
-    default: return launch<D, FMT, 4, 4, 2, 1, 4, 1>(p, w, blocks, cfg);
+    default: return launch_kv_attention_umma(p, w, blocks, cfg);
   }
 }
 
@@ -633,7 +535,7 @@ cudaError_t launch_kv_attention(const KvAttnParams& params, void* workspace, con
   const Plan t = plan_of(M);
   const int64_t row_blocks = (M + t.rows - 1) / t.rows, items = p.c.S * row_blocks * p.c.heads;
   if (M > 0x7fffffff || p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  p.few_steps = items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16 + kItemCost) <= 0x7fffffff;
+  p.few_steps = items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16 + kMostItemCost) <= 0x7fffffff;
   // no more blocks than the longest sequences could fill
   const int64_t steps = std::max<int64_t>(items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16), 1);
   const int64_t blocks = std::min<int64_t>(static_cast<int64_t>(cfg.sms) * t.per_sm, (steps + t.round - 1) / t.round);

@@ -50,13 +50,13 @@ __device__ __forceinline__ int64_t kv_div(int64_t a, int b) {
 }
 
 // The blocks share the steps of all (sequence, row block, head) items evenly.  The items lie one after
-// another on one axis (head fastest within a (sequence, row block) pair), each behind kItemCost units that
+// another on one axis (head fastest within a (sequence, row block) pair), each behind `item_cost` units that
 // stand for a block's set-up of an item, and each block takes a piece of `per` consecutive units of it.
 // Where there are few items (at most a quarter of the blocks), pieces do not cross from one item to the
 // next and there is nothing to level: a piece of two items costs its block a second set-up, which takes
 // longer than the few steps that the last pieces of the items leave idle.  Lengths are only known on the
 // device, so every block adds them up itself.
-constexpr int kItemCost = 16;  // about 6 us, measured in a batch of 64 sequences: the steps that a block takes in that time
+constexpr int kMostItemCost = 64;
 
 struct KvShare {
   int64_t per;   // units of a piece
@@ -64,12 +64,13 @@ struct KvShare {
   int64_t off;   // of its first unit within its pair
   int64_t at;    // of its first unit on the axis (pieces that cross items)
   int pair;
-  int cost;      // units in front of an item's steps: kItemCost, or 0 where pieces do not cross items
+  int cost;      // units in front of an item's steps: 0 where pieces do not cross items
   bool cross;
 };
 
 template <int THREADS>
-__device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_blocks, unsigned block_rows, int round) {
+__device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_blocks, unsigned block_rows, int round,
+                                            int item_cost) {
   __shared__ int64_t s_sum[THREADS / 32], s_off;
   __shared__ int s_pair;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -81,7 +82,7 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_block
   const int64_t items = static_cast<int64_t>(pairs) * p.c.heads;
   const int blocks = static_cast<int>(gridDim.x);
   KvShare w{0, 0, 0, 0, 0, 0, items * 4 > blocks};
-  w.cost = w.cross ? kItemCost : 0;
+  w.cost = w.cross ? item_cost : 0;
   const auto units = [&](unsigned i) {
     const int n = steps(i);
     return n > 0 ? n + w.cost : 0;
@@ -174,6 +175,55 @@ __device__ __forceinline__ KvShare kv_share(const KvAttnParams& p, int row_block
   }
   return w;
 }
+
+// The segments of a block: one item's consecutive steps i0 .. i1 - 1 each.
+struct KvSegment {
+  int s, mb, h, pair, i0, i1;
+  unsigned m0;   // the row block's first row
+  int64_t end;   // on the axis, behind the item (pieces that cross items)
+  KvSeq seq;
+  KvSpan span;
+  __device__ __forceinline__ bool whole_item() const { return i0 == 0 && i1 == span.n; }
+};
+
+struct KvWalk {
+  KvShare share;
+  int64_t left, off, at;
+  int pair;
+  __device__ __forceinline__ explicit KvWalk(const KvShare& w)
+      : share(w), left(w.left), off(w.off), at(w.at), pair(w.pair) {}
+  __device__ __forceinline__ bool next(const KvAttnParams& p, int row_blocks, unsigned block_rows, KvSegment& t) {
+    while (left > 0) {
+      t.pair = pair;
+      t.s = row_blocks == 1 ? pair : pair / row_blocks;
+      t.mb = pair - t.s * row_blocks;
+      t.m0 = static_cast<unsigned>(t.mb) * block_rows;
+      t.seq = kv_seq(p.c, p.rows.start, p.rows.lens, t.s);
+      t.span = kv_span(p, t.seq, t.m0, block_rows);
+      if (t.span.n == 0) {
+        ++pair;
+        continue;
+      }
+      // units u0 .. u1 - 1 of the item, of which those from share.cost on are its steps
+      const int size = t.span.n + share.cost;
+      t.h = static_cast<int>(kv_div(off, size));
+      const int u0 = static_cast<int>(off - static_cast<int64_t>(t.h) * size);
+      const int u1 = static_cast<int>(min(static_cast<int64_t>(size), u0 + left));
+      t.i0 = max(0, u0 - share.cost);
+      t.i1 = max(0, u1 - share.cost);
+      t.end = at - u0 + size;
+      left -= u1 - u0;
+      at += u1 - u0;
+      off += u1 - u0;
+      if (off == static_cast<int64_t>(size) * p.c.heads) {
+        ++pair;
+        off = 0;
+      }
+      if (t.i0 < t.i1) return true;
+    }
+    return false;
+  }
+};
 
 // Page and scales of 32 of a warp's steps, one a lane.
 struct KvPages {

@@ -13,6 +13,7 @@ namespace bolt {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kItemCost = 16;  // of an item's set-up, in steps (kv_attention.cu has the measurement)
 constexpr int kRowTiles = 16;  // tiles of 8 query rows in shared memory at a time
 // Steps that a warp takes at a time and steps of its ring.  Steps of 64 values are too short for one alone
 // (32 sequences of up to 8,192 positions, 8 heads: 54 us one at a time, 42 us two); two of 128 values leave one block an SM (65,536 positions, 2 heads: 12 us one at a time, 18 us two).
@@ -49,28 +50,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv_score_kernel(const KvAttnPa
   bool stuck = false;  // a copy did not arrive in time: the rest of the work is left
   const int k_at = kv_at<D>(place<D>(g), 16 * q4);  // the codes 64 i + 16 q4 .. are at k_at ^ 64 i
   const unsigned M = static_cast<unsigned>(p.rows.R) * p.G;
-  const KvShare share = kv_share<kWarps * 32>(p, 1, M, kWarps * kPairs);
-  int64_t left = share.left, off = share.off;
-  for (int next_s = share.pair; left > 0;) {
-    const int s = next_s;
-    const KvSeq seq = kv_seq(c, p.rows.start, p.rows.lens, s);
-    const KvSpan span = kv_span(p, seq, 0, M);
-    if (span.n == 0) {
-      ++next_s;
-      continue;
-    }
-    // units u0 .. u1 - 1 of the item, of which those from share.cost on are its steps
-    const int size = span.n + share.cost;
-    const int h = static_cast<int>(kv_div(off, size)), u0 = static_cast<int>(off - static_cast<int64_t>(h) * size);
-    const int u1 = static_cast<int>(min(static_cast<int64_t>(size), u0 + left));
-    const int i0 = max(0, u0 - share.cost), i1 = max(0, u1 - share.cost);
-    left -= u1 - u0;
-    off += u1 - u0;
-    if (off == static_cast<int64_t>(size) * c.heads) {
-      ++next_s;
-      off = 0;
-    }
-    if (i0 == i1) continue;
+  const KvShare share = kv_share<kWarps * 32>(p, 1, M, kWarps * kPairs, kItemCost);
+  KvWalk walk(share);
+  for (KvSegment seg; walk.next(p, 1, M, seg);) {
+    const int s = seg.s, h = seg.h, i0 = seg.i0, i1 = seg.i1;
+    const KvSeq& seq = seg.seq;
+    const KvSpan& span = seg.span;
     float* score = p.score + (static_cast<int64_t>(s) * c.heads + h) * p.score_width;
     // this warp's k-th step is the k % kPairs-th of the group k / kPairs * kWarps + warp
     const int most = max(0, (i1 - i0 - warp * kPairs + kWarps * kPairs - 1) / (kWarps * kPairs));
@@ -246,7 +231,7 @@ cudaError_t launch_kv_score(const KvAttnParams& params, const LaunchCfg& cfg) {
   KvAttnParams p = params;
   const int64_t steps = std::max<int64_t>(
       static_cast<int64_t>(p.c.S) * p.c.heads * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16), 1);
-  p.few_steps = steps + static_cast<int64_t>(p.c.S) * p.c.heads * kItemCost <= 0x7fffffff;
+  p.few_steps = steps + static_cast<int64_t>(p.c.S) * p.c.heads * kMostItemCost <= 0x7fffffff;
   const int round = kWarps * (p.c.D == 64 ? kTogether<64> : kTogether<128>);
   const int64_t blocks = std::min<int64_t>(cfg.sms * 2, (steps + round - 1) / round);
   CUtensorMap map_k;
