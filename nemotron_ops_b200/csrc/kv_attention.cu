@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
 
   kv_empty_items<D, L::kRows, L::kThreads>(p, w);
 
-  KvWalk walk(share);
+  KvWalk walk;
+  walk.start(share);
   for (KvSegment seg; walk.next(p, w.row_blocks, L::kRows, seg);) {
     const int s = seg.s, h = seg.h, i0 = seg.i0, i1 = seg.i1;
     const unsigned m0 = seg.m0;

@@ -5,11 +5,11 @@
 //   P = exp2(...)  a thread a row: no exchange between threads for the maxima and the sums
 //   O += P V       tcgen05.mma, P fp16 in tensor memory (in S's place), V fp16 in shared memory, O in tensor memory
 //
-// One block an SM, 13 warps:
+// One block an SM, 17 warps:
 //   * two groups of 4 softmax warps.  Group i takes the segment's tiles i, i + 2, ... as a stream of its own
 //     with its own S / P, O, references and sums (2 x 256 of the 512 tensor-memory columns), so that one
 //     stream's products run while the other's weights are made; the streams are joined at the segment's end.
-//   * 4 conversion warps, two steps of each tile each: codes from global memory (a tile ahead, in registers)
+//   * 8 conversion warps, one step of each tile each: codes from global memory (a tile ahead, in registers)
 //     to exact fp16 in shared memory.
 //   * one warp that issues the products.
 // Both operands have one shared-memory image, 8 positions x 8 values a core matrix: it is K-major for S and
@@ -22,8 +22,7 @@ namespace bolt {
 namespace {
 
 constexpr int kRows = 128, kSteps = 8, kTileTokens = kSteps * 16;
-constexpr int kSoftWarps = 8, kConvWarps = 4;  // 13 warps: 128 registers a thread
-constexpr int kHalves = kSteps / kConvWarps;   // steps of a tile that a conversion warp takes
+constexpr int kSoftWarps = 8, kConvWarps = kSteps;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps;
 constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kItemCost = 48;  // of an item's set-up, in steps
@@ -71,36 +70,36 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
       " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar)
       : "memory");
 }
-// 32 columns of this thread's row
-__device__ __forceinline__ void tm_ld32(uint32_t at, float (&v)[32]) {
+// 16 columns of this thread's row: begun, and arrived (the values pass through the wait, so that no use of
+// them comes before it)
+__device__ __forceinline__ void tm_begin16(uint32_t at, float (&v)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
-        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
       : "r"(at)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tm_st32(uint32_t at, const float (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
-      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
-      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
-      "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
-      "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
-      : "memory");
+__device__ __forceinline__ void tm_arrived16(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
 }
-__device__ __forceinline__ void tm_st16(uint32_t at, const uint32_t (&v)[16]) {
+__device__ __forceinline__ void tm_st16(uint32_t at, const float (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
       "%15, %16};" ::"r"(at),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
       : "memory");
+}
+__device__ __forceinline__ void tm_st8(uint32_t at, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -131,6 +130,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
   extern __shared__ uint4 smem_raw[];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_lost;
+  // the block's place in its work is kept here: the roles need the registers
+  __shared__ KvWalk s_walk;
+  __shared__ KvSegment s_seg;
+  __shared__ int s_more;
   uint8_t* smem = reinterpret_cast<uint8_t*>(smem_raw);
   float4* s_meta = reinterpret_cast<float4*>(smem + L::kMeta);  // [stream][2][step]: K scale, log2 and 1 / V scale, position and flags
   float* sf = reinterpret_cast<float*>(smem + L::kFactor);      // [row]: logit factor
@@ -138,8 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
   float* sl = reinterpret_cast<float*>(smem + L::kSum);         // [stream][row]
   float4* so = reinterpret_cast<float4*>(smem + L::kK);         // [stream][row][D / 4], when the products are done
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
-  const auto k_full = [&](int i) { return smem_u32(bars + i); };      // 4: K of the stream's next tile is in place
-  const auto v_full = [&](int i) { return smem_u32(bars + 2 + i); };  // 4: its V
+  const auto k_full = [&](int i) { return smem_u32(bars + i); };      // 8: K of the stream's next tile is in place
+  const auto v_full = [&](int i) { return smem_u32(bars + 2 + i); };  // 8: its V
   const auto s_full = [&](int i) { return smem_u32(bars + 4 + i); };  // 2: its S is complete (and K free)
   const auto p_full = [&](int i) { return smem_u32(bars + 6 + i); };  // 4: its P is in place
   const auto o_full = [&](int i) { return smem_u32(bars + 8 + i); };  // its part of O is added (V, S and P free)
@@ -171,10 +174,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
   const auto o_col = [&](int i) { return tmem + 256u + 128u * i; };
   pdl_wait();
   pdl_trigger();
-  const unsigned M = static_cast<unsigned>(p.rows.R) * p.G, G = p.G;
-  const KvShare share = kv_share<kThreads>(p, w.row_blocks, kRows, kSteps, kItemCost);
+  {
+    const KvShare share = kv_share<kThreads>(p, w.row_blocks, kRows, kSteps, kItemCost);
+    if (tid == 0) s_walk.start(share);
+  }
   kv_empty_items<D, kRows, kThreads>(p, w);
-  unsigned done[2] = {0, 0};  // tiles of each stream, of all segments so far
+  unsigned done0 = 0, done1 = 0;  // tiles of each stream, of all segments so far
   bool lost = false;          // a wait ran out: the remaining segments are written as if their rows saw nothing
   const auto wait = [&](uint32_t bar, unsigned n) {  // for the completion of phase n
     const bool ok = mbar_wait(bar, n & 1, kStatusFullWait);
@@ -182,16 +187,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
     return __all_sync(0xffffffffu, ok);
   };
 
-  KvWalk walk(share);
-  for (KvSegment seg; walk.next(p, w.row_blocks, kRows, seg);) {
-    const KvSpan& span = seg.span;
-    const int tiles = (seg.i1 - seg.i0 + kSteps - 1) / kSteps;
+  while (true) {
+    if (tid == 0) s_more = s_walk.next(p, w.row_blocks, kRows, s_seg);
+    __syncthreads();
+    if (!s_more) break;
+    const int i0 = s_seg.i0, i1 = s_seg.i1, tiles = (i1 - i0 + kSteps - 1) / kSteps;
     // the query rows: a warp takes tiles of 8 rows
     for (int tile = warp; tile < kRows / 8; tile += kMmaWarp + 1) {
       uint4 raw[D / 64][2];
       uint2 q[D / 16];
       float f, t;
-      kv_fetch_q<D>(p, seg.seq, seg.s, seg.h, seg.m0 + tile * 8, raw);
+      kv_fetch_q<D>(p, s_seg.seq, s_seg.s, s_seg.h, s_seg.m0 + tile * 8, raw);
       kv_make_q<D, kKvE4m3>(p, raw, q, f, t);  // exact codes of either format
       const uint32_t flip = f < 0.f ? 0x80008000u : 0u;  // a negative scale goes into the rows: factors are not negative
       const int g = lane >> 2, q4 = lane & 3;
@@ -214,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
       // ---- the products
       const auto scores = [&](int t) {  // S of tile t
         const int i = t & 1;
-        const unsigned n = done[i] + (t >> 1);
+        const unsigned n = (i ? done1 : done0) + (t >> 1);
         if (!wait(k_full(i), n)) return false;
         if (n > 0 && !wait(o_full(i), n - 1)) return false;
         tc_after();
@@ -230,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
       bool ok = scores(0) && (tiles < 2 || scores(1));
       for (int t = 0; ok && t < tiles; ++t) {
         const int i = t & 1;
-        const unsigned n = done[i] + (t >> 1);
+        const unsigned n = (i ? done1 : done0) + (t >> 1);
         ok = wait(p_full(i), n) && wait(v_full(i), n);
         if (!ok) break;
         tc_after();
@@ -243,81 +249,74 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
         ok = t + 2 >= tiles || scores(t + 2);
       }
     } else if (warp >= kSoftWarps) {
-      // ---- codes to fp16: this warp's steps of each tile, cw and cw + 4
-      const int cw = warp - kSoftWarps, r = lane & 7, chunk = lane >> 3;
-      constexpr int kVecs = D / 32;  // 16-byte vectors of a lane and step: 2 groups of 8 positions x D / 64
+      // ---- codes to fp16: this warp's step of each tile
+      const int cw = warp - kSoftWarps, r = lane & 7, chunk = lane >> 3, s = s_seg.s, h = s_seg.h;
+      const KvSpan span = s_seg.span;
+      constexpr int kVecs = D / 32;  // 16-byte vectors of a lane: 2 groups of 8 positions x D / 64
       constexpr uint32_t kZero = FMT == kKvInt8 ? 0x80808080u : 0u;  // four codes of 0
-      const int64_t page_codes = static_cast<int64_t>(c.heads) * c.T * D, head_codes = static_cast<int64_t>(seg.h) * c.T * D;
-      const auto step_of = [&](int t, int half) { return seg.i0 + t * kSteps + half * kConvWarps + cw; };
-      // pages and scales of 16 tiles: of step cw in the lanes 0 .. 15, of step cw + 4 in the others
-      KvPages meta;
+      const int64_t page_codes = static_cast<int64_t>(c.heads) * c.T * D;
+      const int64_t head_codes = static_cast<int64_t>(h) * c.T * D + r * D + chunk * 16;
+      const auto base_of = [&](int t) { return span.base(min(i0 + t * kSteps + cw, i1 - 1)); };
+      KvPages meta;  // of 32 tiles, one a lane
       float vlog = 0.f, vinv = 0.f;
-      const auto look_up = [&](int t0) {
-        const int t = t0 + (lane & 15), i = step_of(t, lane >> 4);
-        meta.load_page(c, seg.s, t < tiles && i < seg.i1, span.base(min(i, seg.i1 - 1)));
+      const auto look_up = [&](int t) {
+        meta.load_page(c, s, i0 + t * kSteps + cw < i1, base_of(t));
         meta.check_page(c);
-        meta.load_scales<true>(c, seg.h);
+        if (base_of(t) > span.last) meta.page = -1;
+        meta.load_scales<true>(c, h);
         const float vs = fmaxf(meta.vs, 0x1p-96f);
         vlog = log2f(vs);
         vinv = 1.f / vs;
       };
-      const auto lane_of = [&](int t, int half) { return (t & 15) + 16 * half; };
-      const auto base_of = [&](int t, int half) { return span.base(min(step_of(t, half), seg.i1 - 1)); };
-      uint4 kx[kHalves][kVecs], vx[kHalves][kVecs];
+      uint4 kx[kVecs], vx[kVecs];
       // codes of tile t; zeros where there are none
-      const auto load = [&](int t, const uint8_t* codes, bool values, uint4 (&x)[kHalves][kVecs]) {
+      const auto load = [&](int t, const uint8_t* codes, bool values, uint4 (&x)[kVecs]) {
+        const int page = __shfl_sync(0xffffffffu, meta.page, t & 31), j0 = base_of(t);
+        const uint8_t* from = codes + page * page_codes + head_codes + (j0 & (c.T - 1)) * D;
 #pragma unroll
-        for (int half = 0; half < kHalves; ++half) {
-          const int page = __shfl_sync(0xffffffffu, meta.page, lane_of(t, half)), j0 = base_of(t, half);
-          const bool some = page >= 0 && j0 <= span.last;
-          const uint8_t* from = codes + page * page_codes + head_codes + ((j0 & (c.T - 1)) + r) * D + chunk * 16;
-#pragma unroll
-          for (int v = 0; v < kVecs; ++v) {
-            x[half][v] = make_uint4(kZero, kZero, kZero, kZero);
-            bool take = some;
-            if (FMT == kKvE4m3 && values) {
-              // what no row of the block sees may be a NaN code, which a weight of 0 must not meet
-              const int j = j0 + (v & 1) * 8 + r;
-              take &= j <= span.last && !(p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks);
-            }
-            if (take) x[half][v] = *reinterpret_cast<const uint4*>(from + (v & 1) * 8 * D + (v >> 1) * 64);
+        for (int v = 0; v < kVecs; ++v) {
+          x[v] = make_uint4(kZero, kZero, kZero, kZero);
+          bool take = page >= 0;
+          if (FMT == kKvE4m3 && values) {
+            // what no row of the block sees may be a NaN code, which a weight of 0 must not meet
+            const int j = j0 + (v & 1) * 8 + r;
+            take &= j <= span.last && !(p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks);
           }
+          if (take) x[v] = *reinterpret_cast<const uint4*>(from + (v & 1) * 8 * D + (v >> 1) * 64);
         }
       };
-      const auto store = [&](uint8_t* tile, const uint4 (&x)[kHalves][kVecs]) {
+      const auto store = [&](uint8_t* tile, const uint4 (&x)[kVecs]) {
 #pragma unroll
-        for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-          for (int v = 0; v < kVecs; ++v) {
-            uint4 lo, hi;
-            convert16<FMT>(x[half][v], lo, hi);
-            uint8_t* to = tile + (2 * (half * kConvWarps + cw) + (v & 1)) * L::kGroup + 2 * (chunk + (v >> 1) * 4) * 128 + r * 16;
-            *reinterpret_cast<uint4*>(to) = lo;
-            *reinterpret_cast<uint4*>(to + 128) = hi;
-          }
+        for (int v = 0; v < kVecs; ++v) {
+          uint4 lo, hi;
+          convert16<FMT>(x[v], lo, hi);
+          uint8_t* to = tile + (2 * cw + (v & 1)) * L::kGroup + 2 * (chunk + (v >> 1) * 4) * 128 + r * 16;
+          *reinterpret_cast<uint4*>(to) = lo;
+          *reinterpret_cast<uint4*>(to + 128) = hi;
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       };
-      look_up(0);
+      look_up(lane);
       load(0, c.k, false, kx);
       load(0, c.v, true, vx);
       for (int t = 0; t < tiles; ++t) {
         const int i = t & 1;
-        const unsigned n = done[i] + (t >> 1);
+        const unsigned n = (i ? done1 : done0) + (t >> 1);
         if (n > 0 && !wait(s_full(i), n - 1)) break;
-        if ((lane & 15) == (t & 15)) {  // the lanes that hold this tile's steps
-          const int half = lane >> 4, j0 = base_of(t, half);
+        if (lane == (t & 31)) {  // the lane that holds this tile's step
+          const int j0 = base_of(t);
           int flags = 0;
-          if (meta.page < 0 || j0 > span.last)
+          if (meta.page < 0)
             flags = kDead;
           else if (j0 + 15 <= span.first && (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
             flags = kWhole;
           // the stream's tile before the last has been read: S of the last was made after its P
-          s_meta[(i * 2 + (n & 1)) * kSteps + half * kConvWarps + cw] = make_float4(meta.ks, vlog, vinv, __int_as_float(j0 | flags));
+          s_meta[(i * 2 + (n & 1)) * kSteps + cw] = make_float4(meta.ks, vlog, vinv, __int_as_float(j0 | flags));
         }
         store(smem + L::kK + i * L::kTile, kx);
         __syncwarp();
         if (lane == 0) mbar_arrive(k_full(i));
-        if (((t + 1) & 15) == 0) look_up(t + 1);
+        if (((t + 1) & 31) == 0) look_up(t + 1 + lane);
         if (t + 1 < tiles) load(t + 1, c.k, false, kx);
         if (n > 0 && !wait(o_full(i), n - 1)) break;
         store(smem + L::kV + i * L::kTile, vx);
@@ -329,103 +328,107 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
       // ---- weights: stream i, this thread's row
       const int i = warp >> 2, row = tid & 127;
       const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 rows a warp, in the address's upper half
-      const unsigned m = seg.m0 + row;
-      const int at_row = seg.seq.start + static_cast<int>(m / G);
-      const int pos = m < M && at_row < seg.seq.len ? at_row : -1;
+      const unsigned m = s_seg.m0 + row, G = p.G;
+      const int at_row = s_seg.seq.start + static_cast<int>(m / G);
+      const int pos = m < static_cast<unsigned>(p.rows.R) * G && at_row < s_seg.seq.len ? at_row : -1;
       const float qf = sf[row];
-      float ref = 0.f, top_off = -INFINITY, l = 0.f;  // the reference m - 8; how far a logit may pass it
+      float ref = 0.f, top_off = -INFINITY, l = 0.f;  // the reference m - 8; how far a logit may pass it: not at all until there is one
       bool ok = true;
       int n_tiles = 0;
       for (int t = i; t < tiles; t += 2, ++n_tiles) {
-        const unsigned n = done[i] + (t >> 1);
+        const unsigned n = (i ? done1 : done0) + (t >> 1);
         ok = wait(s_full(i), n);
         if (!ok) break;
         tc_after();
         const float4* meta = s_meta + (i * 2 + (n & 1)) * kSteps;
-        // the largest logit: of the raw sums by step, since a step's factor is not negative
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int q = 0; q < kSteps / 2; ++q) {
-          float x[32];
-          tm_ld32((s_col(i) + 32 * q) + lanes, x);
+        const auto weigh = [&](int k, float (&x)[16]) {  // step k of the tile: 16 logits to 16 weights
+          const float4 sc = meta[k];
+          const int j0 = __float_as_int(sc.w);
+          const float f = qf * sc.x, d = sc.y - ref;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float4 sc = meta[2 * q + u];
-            const int j0 = __float_as_int(sc.w);
-            float raw = -INFINITY;
-            if (j0 & kWhole) {
+          for (int e = 0; e < 16; ++e) x[e] = x[e] * f + d;
+          if (!(j0 & kWhole)) {
+            const uint32_t seen = j0 & kDead ? 0u : seen_bits(p.mask, pos, j0 & ~15);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) raw = fmaxf(raw, x[16 * u + e]);
-            } else if (!(j0 & kDead)) {
-              const uint32_t seen = seen_bits(p.mask, pos, j0 & ~15);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) raw = fmaxf(raw, seen >> e & 1 ? x[16 * u + e] : -INFINITY);
-            }
-            if (raw != -INFINITY) top = fmaxf(top, raw * (qf * sc.x) + (sc.y - ref));
+            for (int e = 0; e < 16; ++e) x[e] = seen >> e & 1 ? x[e] : -INFINITY;
           }
-        }
-        if (__any_sync(0xffffffffu, top > top_off)) {
-          const bool fresh = top_off == -INFINITY, move = top > -INFINITY;
-          const float up = !move ? 0.f : fresh ? top - kWeightLog : fmaxf(0.f, top - kWeightLog);
-          const float f = fresh ? 0.f : ex2(-up);
-          if (t != i) {  // the stream has an O
-            // all its products so far are complete: this S came after them
-#pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-              float x[32];
-              tm_ld32((o_col(i) + 32 * q) + lanes, x);
+          float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] *= f;
-              tm_st32((o_col(i) + 32 * q) + lanes, x);
+          for (int e = 4; e < 16; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
+          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          if (__any_sync(0xffffffffu, most > top_off)) {
+            // raise the reference, by a whole number: what is there already takes a power of two
+            const bool fresh = top_off == -INFINITY, move = most > -INFINITY;
+            const float up = !move ? 0.f : fresh ? ceilf(most - kWeightLog) : fmaxf(0.f, ceilf(most - kWeightLog));
+            const float g = fresh ? 0.f : ex2(-up);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] -= up;
+            l *= g;
+            ref += up;
+            if (move) top_off = kWeightTop;
+            tm_wait_st();
+            const __half2 g2 = __float2half2_rn(g);
+            float y[16];
+#pragma unroll 1
+            for (int z = 0; z < (k + 1) / 2; ++z) {  // this tile's weights so far, two steps a time
+              tm_begin16(s_col(i) + 16 * z + lanes, y);
+              tm_arrived16(y);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                // an odd last step's other half holds logits
+                const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&y[e]), g2);
+                if (e < 8 || 2 * z + 1 < k) y[e] = *reinterpret_cast<const float*>(&v);
+              }
+              tm_st16(s_col(i) + 16 * z + lanes, y);
+            }
+            if (t != i) {  // the stream's O: all its products so far are complete, this S came after them
+#pragma unroll 1
+              for (int z = 0; z < D / 16; ++z) {
+                tm_begin16(o_col(i) + 16 * z + lanes, y);
+                tm_arrived16(y);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) y[e] *= g;
+                tm_st16(o_col(i) + 16 * z + lanes, y);
+              }
             }
             tm_wait_st();
           }
-          l *= f;
-          ref += up;
-          if (move) top_off = kWeightTop;
-        }
-#pragma unroll 1
-        for (int q = 0; q < kSteps / 2; ++q) {
-          float x[32];
-          tm_ld32((s_col(i) + 32 * q) + lanes, x);
-          uint32_t h[16];
+          uint32_t h[8];
+          float sum[2] = {0.f, 0.f};
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float4 sc = meta[2 * q + u];
-            const int j0 = __float_as_int(sc.w);
-            const float f = qf * sc.x, d = sc.y - ref;
-            float y[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = ex2(x[16 * u + e] * f + d);
-            if (!(j0 & kWhole)) {
-              const uint32_t seen = j0 & kDead ? 0u : seen_bits(p.mask, pos, j0 & ~15);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] = seen >> e & 1 ? y[e] : 0.f;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              sum += y[e] + y[e + 1];
-              const __half2 z = __floats2half2_rn(y[e], y[e + 1]);
-              h[8 * u + e / 2] = *reinterpret_cast<const uint32_t*>(&z);
-            }
-            l += sum * sc.z;
+          for (int e = 0; e < 16; e += 2) {
+            const float y0 = ex2(x[e]), y1 = ex2(x[e + 1]);
+            sum[(e >> 1) & 1] += y0 + y1;
+            const __half2 z = __floats2half2_rn(y0, y1);
+            h[e / 2] = *reinterpret_cast<const uint32_t*>(&z);
           }
-          tm_st16((s_col(i) + 16 * q) + lanes, h);  // columns that have been read
+          l += (sum[0] + sum[1]) * sc.z;
+          tm_st8(s_col(i) + 8 * k + lanes, h);  // columns that have been read
+        };
+        float xa[16], xb[16];
+        tm_begin16(s_col(i) + lanes, xa);
+#pragma unroll 1
+        for (int k = 0; k < kSteps; k += 2) {
+          tm_arrived16(xa);
+          tm_begin16(s_col(i) + 16 * (k + 1) + lanes, xb);
+          weigh(k, xa);
+          tm_arrived16(xb);
+          if (k + 2 < kSteps) tm_begin16(s_col(i) + 16 * (k + 2) + lanes, xa);
+          weigh(k + 1, xb);
         }
         tm_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(i));
       }
-      if (ok && n_tiles > 0) ok = wait(o_full(i), done[i] + n_tiles - 1);
+      if (ok && n_tiles > 0) ok = wait(o_full(i), (i ? done1 : done0) + n_tiles - 1);
       tc_after();
       ref = pos < 0 || top_off == -INFINITY || !ok ? -INFINITY : ref + kWeightLog;
       sm[i * kRows + row] = ref;
       sl[i * kRows + row] = l;
     }
-    done[0] += (tiles + 1) / 2;
-    done[1] += tiles / 2;
+    done0 += (tiles + 1) / 2;
+    done1 += tiles / 2;
     __syncthreads();  // all products are complete: K and V make room for the values
     lost |= s_lost != 0;
     if (warp < kSoftWarps) {
@@ -434,20 +437,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
       const float ref = sm[i * kRows + row], top = fmaxf(sm[row], sm[kRows + row]);
       const float f = ref == -INFINITY ? 0.f : ex2(ref - top);
 #pragma unroll 1
-      for (int q = 0; q < D / 32; ++q) {
-        float x[32];
-        if (i < tiles) tm_ld32((o_col(i) + 32 * q) + lanes, x);
+      for (int q = 0; q < D / 16; ++q) {
+        float x[16];
+        if (i < tiles) {
+          tm_begin16(o_col(i) + 16 * q + lanes, x);
+          tm_arrived16(x);
+        }
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
+        for (int e = 0; e < 16; e += 4) {
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
           if (f != 0.f) v = make_float4(x[e] * f, x[e + 1] * f, x[e + 2] * f, x[e + 3] * f);
-          so[(i * kRows + row) * (D / 4) + SwizzleRow()(row, 8 * q + e / 4)] = v;
+          so[(i * kRows + row) * (D / 4) + SwizzleRow()(row, 4 * q + e / 4)] = v;
         }
       }
       tc_before();
     }
     __syncthreads();
-    kv_finish<D, kRows, 2, kThreads>(p, w, share, seg, sm, sl, so, SwizzleRow());
+    kv_finish<D, kRows, 2, kThreads>(p, w, s_walk.share, s_seg, sm, sl, so, SwizzleRow());
     __syncthreads();  // the next segment writes the shared buffers
     tc_after();
   }

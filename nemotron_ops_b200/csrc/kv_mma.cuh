@@ -190,8 +190,13 @@ struct KvWalk {
   KvShare share;
   int64_t left, off, at;
   int pair;
-  __device__ __forceinline__ explicit KvWalk(const KvShare& w)
-      : share(w), left(w.left), off(w.off), at(w.at), pair(w.pair) {}
+  __device__ __forceinline__ void start(const KvShare& w) {
+    share = w;
+    left = w.left;
+    off = w.off;
+    at = w.at;
+    pair = w.pair;
+  }
   __device__ __forceinline__ bool next(const KvAttnParams& p, int row_blocks, unsigned block_rows, KvSegment& t) {
     while (left > 0) {
       t.pair = pair;

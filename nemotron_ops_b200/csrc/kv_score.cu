@@ -51,7 +51,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv_score_kernel(const KvAttnPa
   const int k_at = kv_at<D>(place<D>(g), 16 * q4);  // the codes 64 i + 16 q4 .. are at k_at ^ 64 i
   const unsigned M = static_cast<unsigned>(p.rows.R) * p.G;
   const KvShare share = kv_share<kWarps * 32>(p, 1, M, kWarps * kPairs, kItemCost);
-  KvWalk walk(share);
+  KvWalk walk;
+  walk.start(share);
   for (KvSegment seg; walk.next(p, 1, M, seg);) {
     const int s = seg.s, h = seg.h, i0 = seg.i0, i1 = seg.i1;
     const KvSeq& seq = seg.seq;
