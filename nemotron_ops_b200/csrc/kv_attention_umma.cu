@@ -9,8 +9,8 @@
 //   * two groups of 4 softmax warps.  Group i takes the segment's tiles i, i + 2, ... as a stream of its own
 //     with its own S / P, O, references and sums (2 x 256 of the 512 tensor-memory columns), so that one
 //     stream's products run while the other's weights are made; the streams are joined at the segment's end.
-//   * 8 conversion warps, one step of each tile each: codes from global memory (a tile ahead, in registers)
-//     to exact fp16 in shared memory.
+//   * 8 conversion warps, one step of each tile each: codes from a ring of tensor copies, a tile ahead, to
+//     exact fp16 in shared memory.
 //   * one warp that issues the products.
 // Both operands have one shared-memory image, 8 positions x 8 values a core matrix: it is K-major for S and
 // MN-major (transposed in the instruction) for O.  The weights' exponentials bound the kernel: 128 x 128 a
@@ -23,9 +23,12 @@ namespace {
 
 constexpr int kRows = 128, kSteps = 8, kTileTokens = kSteps * 16;
 constexpr int kSoftWarps = 8, kConvWarps = kSteps;
+constexpr int kSlots = 3;  // of a conversion warp's ring: the next tile's K and V are under way
 constexpr int kMmaWarp = kSoftWarps + kConvWarps;
 constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kItemCost = 48;  // of an item's set-up, in steps
+
+constexpr int kDead = 1, kWhole = 2;  // of a step: no row of the block sees it; all see all of it
 
 template <int D>
 struct Smem {
@@ -33,11 +36,12 @@ struct Smem {
   static constexpr int kGroup = D * 16;      // bytes of 8 rows: D / 8 core matrices of 128 bytes
   static constexpr int kQ = 0, kK = kTile, kV = 3 * kTile, kMeta = 5 * kTile;  // K and V: one tile a stream
   static constexpr int kFactor = kMeta + 2 * 2 * kSteps * 16, kRef = kFactor + kRows * 4, kSum = kRef + 2 * kRows * 4;
-  static constexpr int kBars = kSum + 2 * kRows * 4, kBytes = kBars + 11 * 8;
+  static constexpr int kBars = kSum + 2 * kRows * 4, kLine = kBars + (11 + kConvWarps * kSlots) * 8;
+  // per conversion warp a ring of kSlots copies of a step's K or V codes, on 1,024-byte boundaries
+  static constexpr int kRing = (kLine + kConvWarps * 64 * 4 + 1023) / 1024 * 1024, kSlot = 16 * D;
+  static constexpr int kBytes = kRing + kConvWarps * kSlots * kSlot + 1024;
   static_assert(2 * kRows * D * 4 == 4 * kTile, "the joining buffer takes the place of K and V");
 };
-
-constexpr int kDead = 1, kWhole = 2;  // of a step: no row of the block sees it; all see all of it
 
 // fp32 D, fp16 A and B; 128 rows, N columns; B K-major (S) or MN-major (O)
 __device__ constexpr uint32_t idesc(int n, bool mn) {
@@ -125,7 +129,8 @@ struct SwizzleRow {
 };
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const KvAttnParams p, const Work w) {
+__global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
+    const KvAttnParams p, const Work w, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using L = Smem<D>;
   extern __shared__ uint4 smem_raw[];
   __shared__ uint32_t s_tmem;
@@ -134,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
   __shared__ KvWalk s_walk;
   __shared__ KvSegment s_seg;
   __shared__ int s_more;
-  uint8_t* smem = reinterpret_cast<uint8_t*>(smem_raw);
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float4* s_meta = reinterpret_cast<float4*>(smem + L::kMeta);  // [stream][2][step]: K scale, log2 and 1 / V scale, position and flags
   float* sf = reinterpret_cast<float*>(smem + L::kFactor);      // [row]: logit factor
   float* sm = reinterpret_cast<float*>(smem + L::kRef);         // [stream][row]
@@ -147,6 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
   const auto p_full = [&](int i) { return smem_u32(bars + 6 + i); };  // 4: its P is in place
   const auto o_full = [&](int i) { return smem_u32(bars + 8 + i); };  // its part of O is added (V, S and P free)
   const uint32_t drained = smem_u32(bars + 10);  // after a lost wait: the products are complete
+  constexpr uint32_t kZero = FMT == kKvInt8 ? 0x80808080u : 0u;  // four codes of 0
   const KvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -159,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
       mbar_init(o_full(i), 1);
     }
     mbar_init(drained, 1);
+    for (int i = 0; i < kConvWarps * kSlots; ++i) mbar_init(smem_u32(bars + 11 + i), 1);
     fence_barrier_init();
     s_lost = 0;
   }
@@ -180,6 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
   }
   kv_empty_items<D, kRows, kThreads>(p, w);
   unsigned done0 = 0, done1 = 0;  // tiles of each stream, of all segments so far
+  unsigned taken = 0;             // (conversion warps) copies into this warp's ring, of all segments
   bool lost = false;          // a wait ran out: the remaining segments are written as if their rows saw nothing
   const auto wait = [&](uint32_t bar, unsigned n) {  // for the completion of phase n
     const bool ok = mbar_wait(bar, n & 1, kStatusFullWait);
@@ -249,81 +257,108 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(const Kv
         ok = t + 2 >= tiles || scores(t + 2);
       }
     } else if (warp >= kSoftWarps) {
-      // ---- codes to fp16: this warp's step of each tile
+      // ---- codes to fp16: this warp's step of each tile; unit 2 t is tile t's K, 2 t + 1 its V
       const int cw = warp - kSoftWarps, r = lane & 7, chunk = lane >> 3, s = s_seg.s, h = s_seg.h;
       const KvSpan span = s_seg.span;
-      constexpr int kVecs = D / 32;  // 16-byte vectors of a lane: 2 groups of 8 positions x D / 64
-      constexpr uint32_t kZero = FMT == kKvInt8 ? 0x80808080u : 0u;  // four codes of 0
-      const int64_t page_codes = static_cast<int64_t>(c.heads) * c.T * D;
-      const int64_t head_codes = static_cast<int64_t>(h) * c.T * D + r * D + chunk * 16;
+      uint8_t* ring = smem + L::kRing + cw * kSlots * L::kSlot;
+      uint64_t* full = bars + 11 + cw * kSlots;
+      int* lines = reinterpret_cast<int*>(smem + L::kLine) + cw * 64;  // of 64 tiles: first line of the codes, or -1
       const auto base_of = [&](int t) { return span.base(min(i0 + t * kSteps + cw, i1 - 1)); };
-      KvPages meta;  // of 32 tiles, one a lane
+      KvPages meta{-1, 0.f, 0.f}, ahead;  // of 32 tiles, one a lane, and of the 32 after them
       float vlog = 0.f, vinv = 0.f;
-      const auto look_up = [&](int t) {
-        meta.load_page(c, s, i0 + t * kSteps + cw < i1, base_of(t));
-        meta.check_page(c);
-        if (base_of(t) > span.last) meta.page = -1;
-        meta.load_scales<true>(c, h);
+      const auto look_up = [&](int t, KvPages& of) {
+        of.load_page(c, s, i0 + t * kSteps + cw < i1, base_of(t));
+        of.check_page(c);
+        if (base_of(t) > span.last) of.page = -1;
+        of.load_scales<true>(c, h);
+        lines[t & 63] = of.page < 0 ? -1 : ((of.page * c.heads + h) * c.T + (base_of(t) & (c.T - 1))) / (128 / D);
+      };
+      const auto use = [&]() {
         const float vs = fmaxf(meta.vs, 0x1p-96f);
         vlog = log2f(vs);
         vinv = 1.f / vs;
       };
-      uint4 kx[kVecs], vx[kVecs];
-      // codes of tile t; zeros where there are none
-      const auto load = [&](int t, const uint8_t* codes, bool values, uint4 (&x)[kVecs]) {
-        const int page = __shfl_sync(0xffffffffu, meta.page, t & 31), j0 = base_of(t);
-        const uint8_t* from = codes + page * page_codes + head_codes + (j0 & (c.T - 1)) * D;
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-          x[v] = make_uint4(kZero, kZero, kZero, kZero);
-          bool take = page >= 0;
-          if (FMT == kKvE4m3 && values) {
-            // what no row of the block sees may be a NaN code, which a weight of 0 must not meet
-            const int j = j0 + (v & 1) * 8 + r;
-            take &= j <= span.last && !(p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks);
-          }
-          if (take) x[v] = *reinterpret_cast<const uint4*>(from + (v & 1) * 8 * D + (v >> 1) * 64);
+      const auto fetch = [&](int u) {
+        __syncwarp();  // no lane reads the unit's place in the ring any more
+        if (lane != 0 || u >= 2 * tiles) return;
+        const unsigned slot = (taken + u) % kSlots;
+        const uint32_t bar = smem_u32(full + slot);
+        const int line = lines[(u >> 1) & 63];
+        if (line >= 0) {
+          mbar_arrive_expect_tx(bar, L::kSlot);
+          tma_load_3d(smem_u32(ring + slot * L::kSlot), u & 1 ? &map_v : &map_k, 0, line, 0, bar);
+        } else {
+          mbar_arrive(bar);
         }
       };
-      const auto store = [&](uint8_t* tile, const uint4 (&x)[kVecs]) {
+      // unit u, of a step with flags, from the ring to its place among the operands: a lane takes the chunks
+      // `chunk` (and + 4) of the positions r and 8 + r; zeros where there are none
+      const auto convert = [&](int u, int j0, bool dead, uint8_t* tile) {
+        const unsigned n = taken + u;
+        const bool ok = wait(smem_u32(full + n % kSlots), n / kSlots);
+        const uint8_t* from = ring + n % kSlots * L::kSlot;
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
+        for (int v = 0; v < D / 32; ++v) {
+          const int at = kv_at<D>(r, (chunk + (v >> 1) * 4) * 16);
+          uint4 x = lds128(from + (v & 1 ? kv_next_tile<D>(at) : at));
+          bool none = dead;
+          if (FMT == kKvE4m3 && (u & 1)) {
+            // what no row of the block sees may be a NaN code, which a weight of 0 must not meet
+            const int j = j0 + (v & 1) * 8 + r;
+            none |= j > span.last || (p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks);
+          }
+          if (none) x = make_uint4(kZero, kZero, kZero, kZero);
           uint4 lo, hi;
-          convert16<FMT>(x[v], lo, hi);
+          convert16<FMT>(x, lo, hi);
           uint8_t* to = tile + (2 * cw + (v & 1)) * L::kGroup + 2 * (chunk + (v >> 1) * 4) * 128 + r * 16;
           *reinterpret_cast<uint4*>(to) = lo;
           *reinterpret_cast<uint4*>(to + 128) = hi;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        return ok;
       };
-      look_up(lane);
-      load(0, c.k, false, kx);
-      load(0, c.v, true, vx);
-      for (int t = 0; t < tiles; ++t) {
+      look_up(lane, meta);
+      __syncwarp();
+      fetch(0);
+      fetch(1);
+      use();
+      int t = 0;
+      for (; t < tiles; ++t) {
         const int i = t & 1;
         const unsigned n = (i ? done1 : done0) + (t >> 1);
+        if ((t & 31) == 0) {
+          if (t > 0) {
+            meta = ahead;
+            use();
+          }
+          __syncwarp();
+          look_up(t + 32 + lane, ahead);
+          __syncwarp();
+        }
+        const int page = __shfl_sync(0xffffffffu, meta.page, t & 31), j0 = base_of(t);
+        fetch(2 * t + 2);
         if (n > 0 && !wait(s_full(i), n - 1)) break;
         if (lane == (t & 31)) {  // the lane that holds this tile's step
-          const int j0 = base_of(t);
           int flags = 0;
-          if (meta.page < 0)
+          if (page < 0)
             flags = kDead;
           else if (j0 + 15 <= span.first && (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
             flags = kWhole;
           // the stream's tile before the last has been read: S of the last was made after its P
           s_meta[(i * 2 + (n & 1)) * kSteps + cw] = make_float4(meta.ks, vlog, vinv, __int_as_float(j0 | flags));
         }
-        store(smem + L::kK + i * L::kTile, kx);
-        __syncwarp();
+        if (!convert(2 * t, j0, page < 0, smem + L::kK + i * L::kTile)) break;
         if (lane == 0) mbar_arrive(k_full(i));
-        if (((t + 1) & 31) == 0) look_up(t + 1 + lane);
-        if (t + 1 < tiles) load(t + 1, c.k, false, kx);
+        fetch(2 * t + 3);
         if (n > 0 && !wait(o_full(i), n - 1)) break;
-        store(smem + L::kV + i * L::kTile, vx);
-        __syncwarp();
+        if (!convert(2 * t + 1, j0, page < 0, smem + L::kV + i * L::kTile)) break;
         if (lane == 0) mbar_arrive(v_full(i));
-        if (t + 1 < tiles) load(t + 1, c.v, true, vx);
       }
+      if (t < tiles)  // lost: wait, within limits, for what is on its way into the ring
+        for (int u = 2 * t; u < min(2 * t + 4, 2 * tiles); ++u)
+          mbar_wait(smem_u32(full + (taken + u) % kSlots), ((taken + u) / kSlots) & 1, kStatusDrainWait);
+      taken += 2 * tiles;
     } else {
       // ---- weights: stream i, this thread's row
       const int i = warp >> 2, row = tid & 127;
@@ -477,7 +512,9 @@ cudaError_t launch(const KvAttnParams& p, const Work& w, unsigned blocks, const 
   auto kern = kv_attention_umma_kernel<D, FMT>;
   const cudaError_t e = allow_smem(kern, Smem<D>::kBytes, opt);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kern, dim3(blocks), dim3(kThreads), Smem<D>::kBytes, cfg, p, w);
+  CUtensorMap map_k, map_v;
+  if (!kv_code_map(&map_k, p.c, p.c.k) || !kv_code_map(&map_v, p.c, p.c.v)) return cudaErrorInvalidValue;
+  return launch_kernel(kern, dim3(blocks), dim3(kThreads), Smem<D>::kBytes, cfg, p, w, map_k, map_v);
 }
 
 }  // namespace
