@@ -5,16 +5,18 @@
 //   P = exp2(...)  a thread a row: no exchange between threads for the maxima and the sums
 //   O += P V       tcgen05.mma, P fp16 in tensor memory (in S's place), V fp16 in shared memory, O in tensor memory
 //
-// One block an SM, 17 warps:
+// One block an SM, 18 warps:
 //   * two groups of 4 softmax warps.  Group i takes the segment's tiles i, i + 2, ... as a stream of its own
 //     with its own S / P, O, references and sums (2 x 256 of the 512 tensor-memory columns), so that one
 //     stream's products run while the other's weights are made; the streams are joined at the segment's end.
 //   * 8 conversion warps, one step of each tile each: codes from a ring of tensor copies, a tile ahead, to
-//     exact fp16 in shared memory.
+//     exact fp16 in shared memory, and one warp that issues the copies, a lane a ring.
 //   * one warp that issues the products.
 // Both operands have one shared-memory image, 8 positions x 8 values a core matrix: it is K-major for S and
 // MN-major (transposed in the instruction) for O.  The weights' exponentials bound the kernel: 128 x 128 a
 // tile at 16 a cycle and SM are 1,024 cycles, the tile's two products 512.
+#include <type_traits>
+
 #include "kv_split.cuh"
 
 namespace bolt {
@@ -24,8 +26,9 @@ namespace {
 constexpr int kRows = 128, kSteps = 8, kTileTokens = kSteps * 16;
 constexpr int kSoftWarps = 8, kConvWarps = kSteps;
 constexpr int kSlots = 3;  // of a conversion warp's ring: the next tile's K and V are under way
-constexpr int kMmaWarp = kSoftWarps + kConvWarps;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kMmaWarp = kSoftWarps + kConvWarps, kCopyWarp = kMmaWarp + 1;
+constexpr int kThreads = (kCopyWarp + 1) * 32;
+constexpr int kMetaTiles = 64;
 constexpr int kItemCost = 48;  // of an item's set-up, in steps
 
 constexpr int kDead = 1, kWhole = 2;  // of a step: no row of the block sees it; all see all of it
@@ -35,10 +38,10 @@ struct Smem {
   static constexpr int kTile = 128 * D * 2;  // bytes of 128 rows of fp16
   static constexpr int kGroup = D * 16;      // bytes of 8 rows: D / 8 core matrices of 128 bytes
   static constexpr int kQ = 0, kK = kTile, kV = 3 * kTile, kMeta = 5 * kTile;  // K and V: one tile a stream
-  static constexpr int kFactor = kMeta + 2 * 2 * kSteps * 16, kRef = kFactor + kRows * 4, kSum = kRef + 2 * kRows * 4;
-  static constexpr int kBars = kSum + 2 * kRows * 4, kLine = kBars + (11 + kConvWarps * kSlots) * 8;
+  static constexpr int kFactor = kMeta + kMetaTiles * kSteps * 16, kRef = kFactor + kRows * 8, kSum = kRef + 2 * kRows * 4;
+  static constexpr int kBars = kSum + 2 * kRows * 4, kLine = kBars + (11 + 2 * kConvWarps * kSlots) * 8;
   // per conversion warp a ring of kSlots copies of a step's K or V codes, on 1,024-byte boundaries
-  static constexpr int kRing = (kLine + kConvWarps * 64 * 4 + 1023) / 1024 * 1024, kSlot = 16 * D;
+  static constexpr int kRing = (kLine + kConvWarps * kMetaTiles * 4 + 1023) / 1024 * 1024, kSlot = 16 * D;
   static constexpr int kBytes = kRing + kConvWarps * kSlots * kSlot + 1024;
   static_assert(2 * kRows * D * 4 == 4 * kTile, "the joining buffer takes the place of K and V");
 };
@@ -107,6 +110,12 @@ __device__ __forceinline__ void tm_st8(uint32_t at, const uint32_t (&v)[8]) {
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // The positions of a step (16 from j0 on) that a row at `pos` sees, as bits.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 16 ? 0xFFFFu : (1u << n) - 1; }
 __device__ __forceinline__ uint32_t seen_bits(const KvMask& m, int pos, int j0) {
@@ -115,13 +124,20 @@ __device__ __forceinline__ uint32_t seen_bits(const KvMask& m, int pos, int j0) 
   return seen;
 }
 
-// 16 codes as 16 halves in order.
-template <int FMT>
+// 16 codes as 16 halves in order: exact V codes, or K's (k_to_half).
+template <int FMT, bool V>
 __device__ __forceinline__ void convert16(const uint4& x, uint4& lo, uint4& hi) {
-  codes_to_half<FMT>(x.x, lo.x, lo.y);
-  codes_to_half<FMT>(x.y, lo.z, lo.w);
-  codes_to_half<FMT>(x.z, hi.x, hi.y);
-  codes_to_half<FMT>(x.w, hi.z, hi.w);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t y[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (V)
+      codes_to_half<FMT>(w[e], y[2 * e], y[2 * e + 1]);
+    else
+      k_to_half<FMT>(w[e], y[2 * e], y[2 * e + 1]);
+  }
+  lo = make_uint4(y[0], y[1], y[2], y[3]);
+  hi = make_uint4(y[4], y[5], y[6], y[7]);
 }
 
 struct SwizzleRow {
@@ -140,8 +156,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
   __shared__ KvSegment s_seg;
   __shared__ int s_more;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float4* s_meta = reinterpret_cast<float4*>(smem + L::kMeta);  // [stream][2][step]: K scale, log2 and 1 / V scale, position and flags
-  float* sf = reinterpret_cast<float*>(smem + L::kFactor);      // [row]: logit factor
+  float4* s_meta = reinterpret_cast<float4*>(smem + L::kMeta);  // [tile % 64][step]: K scale, log2 and 1 / V scale, position and flags
+  float2* sf = reinterpret_cast<float2*>(smem + L::kFactor);    // [row]: logit factor and shift (kv_make_q)
   float* sm = reinterpret_cast<float*>(smem + L::kRef);         // [stream][row]
   float* sl = reinterpret_cast<float*>(smem + L::kSum);         // [stream][row]
   float4* so = reinterpret_cast<float4*>(smem + L::kK);         // [stream][row][D / 4], when the products are done
@@ -165,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
       mbar_init(o_full(i), 1);
     }
     mbar_init(drained, 1);
-    for (int i = 0; i < kConvWarps * kSlots; ++i) mbar_init(smem_u32(bars + 11 + i), 1);
+    for (int i = 0; i < 2 * kConvWarps * kSlots; ++i) mbar_init(smem_u32(bars + 11 + i), 1);
     fence_barrier_init();
     s_lost = 0;
   }
@@ -187,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
   }
   kv_empty_items<D, kRows, kThreads>(p, w);
   unsigned done0 = 0, done1 = 0;  // tiles of each stream, of all segments so far
-  unsigned taken = 0;             // (conversion warps) copies into this warp's ring, of all segments
+  unsigned taken = 0;             // copies into each conversion warp's ring, of all segments
   bool lost = false;          // a wait ran out: the remaining segments are written as if their rows saw nothing
   const auto wait = [&](uint32_t bar, unsigned n) {  // for the completion of phase n
     const bool ok = mbar_wait(bar, n & 1, kStatusFullWait);
@@ -200,13 +216,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
     __syncthreads();
     if (!s_more) break;
     const int i0 = s_seg.i0, i1 = s_seg.i1, tiles = (i1 - i0 + kSteps - 1) / kSteps;
+    // conversion warp cw, lane l: the entries of step cw of tile t0 + l
+    const auto meta_table = [&](int t0) {
+      const KvSpan span = s_seg.span;
+      const int cw = warp - kSoftWarps, t = t0 + lane, step = i0 + t * kSteps + cw;
+      const int j0 = span.base(min(step, i1 - 1));
+      KvPages meta;
+      meta.load_page(c, s_seg.s, step < i1 && j0 <= span.last, j0);
+      meta.check_page(c);
+      meta.load_scales<true>(c, s_seg.h);
+      int flags = 0;
+      if (meta.page < 0)
+        flags = kDead;
+      else if (j0 + 15 <= span.first && (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
+        flags = kWhole;
+      const float vs = fmaxf(meta.vs, 0x1p-96f);
+      s_meta[t % kMetaTiles * kSteps + cw] = make_float4(meta.ks, log2f(vs), 1.f / vs, __int_as_float(j0 | flags));
+      reinterpret_cast<int*>(smem + L::kLine)[cw * kMetaTiles + t % kMetaTiles] =
+          meta.page < 0 ? -1 : ((meta.page * c.heads + s_seg.h) * c.T + (j0 & (c.T - 1))) / (128 / D);
+    };
+    if (warp >= kSoftWarps && warp < kMmaWarp) meta_table(0);
     // the query rows: a warp takes tiles of 8 rows
-    for (int tile = warp; tile < kRows / 8; tile += kMmaWarp + 1) {
+    for (int tile = warp; tile < kRows / 8; tile += kCopyWarp + 1) {
       uint4 raw[D / 64][2];
       uint2 q[D / 16];
       float f, t;
       kv_fetch_q<D>(p, s_seg.seq, s_seg.s, s_seg.h, s_seg.m0 + tile * 8, raw);
-      kv_make_q<D, kKvE4m3>(p, raw, q, f, t);  // exact codes of either format
+      kv_make_q<D, FMT>(p, raw, q, f, t);
       const uint32_t flip = f < 0.f ? 0x80008000u : 0u;  // a negative scale goes into the rows: factors are not negative
       const int g = lane >> 2, q4 = lane & 3;
 #pragma unroll
@@ -217,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
           *reinterpret_cast<uint4*>(smem + L::kQ + tile * L::kGroup + (8 * i + 2 * q4 + y) * 128 + g * 16) =
               make_uint4(a.x ^ flip, a.y ^ flip, b.x ^ flip, b.y ^ flip);
         }
-      if (q4 == 0) sf[tile * 8 + g] = fabsf(f);
+      if (q4 == 0) sf[tile * 8 + g] = make_float2(fabsf(f), t);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
@@ -256,109 +292,86 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
         tc_commit(o_full(i));
         ok = t + 2 >= tiles || scores(t + 2);
       }
-    } else if (warp >= kSoftWarps) {
-      // ---- codes to fp16: this warp's step of each tile; unit 2 t is tile t's K, 2 t + 1 its V
-      const int cw = warp - kSoftWarps, r = lane & 7, chunk = lane >> 3, s = s_seg.s, h = s_seg.h;
-      const KvSpan span = s_seg.span;
-      uint8_t* ring = smem + L::kRing + cw * kSlots * L::kSlot;
-      uint64_t* full = bars + 11 + cw * kSlots;
-      int* lines = reinterpret_cast<int*>(smem + L::kLine) + cw * 64;  // of 64 tiles: first line of the codes, or -1
-      const auto base_of = [&](int t) { return span.base(min(i0 + t * kSteps + cw, i1 - 1)); };
-      KvPages meta{-1, 0.f, 0.f}, ahead;  // of 32 tiles, one a lane, and of the 32 after them
-      float vlog = 0.f, vinv = 0.f;
-      const auto look_up = [&](int t, KvPages& of) {
-        of.load_page(c, s, i0 + t * kSteps + cw < i1, base_of(t));
-        of.check_page(c);
-        if (base_of(t) > span.last) of.page = -1;
-        of.load_scales<true>(c, h);
-        lines[t & 63] = of.page < 0 ? -1 : ((of.page * c.heads + h) * c.T + (base_of(t) & (c.T - 1))) / (128 / D);
-      };
-      const auto use = [&]() {
-        const float vs = fmaxf(meta.vs, 0x1p-96f);
-        vlog = log2f(vs);
-        vinv = 1.f / vs;
-      };
-      const auto fetch = [&](int u) {
-        __syncwarp();  // no lane reads the unit's place in the ring any more
-        if (lane != 0 || u >= 2 * tiles) return;
-        const unsigned slot = (taken + u) % kSlots;
-        const uint32_t bar = smem_u32(full + slot);
-        const int line = lines[(u >> 1) & 63];
-        if (line >= 0) {
-          mbar_arrive_expect_tx(bar, L::kSlot);
-          tma_load_3d(smem_u32(ring + slot * L::kSlot), u & 1 ? &map_v : &map_k, 0, line, 0, bar);
-        } else {
-          mbar_arrive(bar);
+    } else if (warp == kCopyWarp) {
+      // ---- copies into the rings, lane i for conversion warp i: unit 2 t is its step of tile t's K, 2 t + 1 of V
+      const int* lines = reinterpret_cast<const int*>(smem + L::kLine) + (lane & 7) * kMetaTiles;
+      uint64_t* full = bars + 11 + (lane & 7) * kSlots;
+      uint64_t* empty = full + kConvWarps * kSlots;
+      for (int u = 0; u < 2 * tiles; ++u) {
+        const unsigned n = taken + u, slot = n % kSlots, round = n / kSlots;
+        // the first kSlots units find their places free; the wait also orders the reading of `lines` behind
+        // its writing: unit u's line was written before unit u - kSlots was handed back
+        if (round > 0 && !wait(smem_u32(empty + slot), round - 1)) break;
+        if (lane < kConvWarps) {
+          const int line = lines[(u >> 1) % kMetaTiles];
+          const uint32_t bar = smem_u32(full + slot);
+          if (line >= 0) {
+            mbar_arrive_expect_tx(bar, L::kSlot);
+            tma_load_3d(smem_u32(smem + L::kRing + (lane * kSlots + slot) * L::kSlot), u & 1 ? &map_v : &map_k, 0, line, 0,
+                        bar);
+          } else {
+            mbar_arrive(bar);
+          }
         }
-      };
-      // unit u, of a step with flags, from the ring to its place among the operands: a lane takes the chunks
-      // `chunk` (and + 4) of the positions r and 8 + r; zeros where there are none
-      const auto convert = [&](int u, int j0, bool dead, uint8_t* tile) {
-        const unsigned n = taken + u;
-        const bool ok = wait(smem_u32(full + n % kSlots), n / kSlots);
-        const uint8_t* from = ring + n % kSlots * L::kSlot;
+        __syncwarp();
+      }
+    } else if (warp >= kSoftWarps) {
+      // ---- codes to fp16: this warp's step of each tile
+      const int cw = warp - kSoftWarps, r = lane & 7, chunk = lane >> 3;
+      const KvSpan span = s_seg.span;
+      const uint8_t* ring = smem + L::kRing + cw * kSlots * L::kSlot;
+      uint64_t* full = bars + 11 + cw * kSlots;
+      uint64_t* empty = full + kConvWarps * kSlots;
+      const int* lines = reinterpret_cast<const int*>(smem + L::kLine) + cw * kMetaTiles;
+      const int from_at = kv_at<D>(r, chunk * 16), to_at = 2 * cw * L::kGroup + 2 * chunk * 128 + r * 16;
+      const auto convert = [&](int u, auto is_v, bool dead, int j0, uint8_t* tile) {
+        constexpr bool V = decltype(is_v)::value;
+        const unsigned n = taken + u, slot = n % kSlots;
+        if (!wait(smem_u32(full + slot), n / kSlots)) return false;
+        const uint8_t* from = ring + slot * L::kSlot;
+        uint4 x[D / 32];
+#pragma unroll
+        for (int v = 0; v < D / 32; ++v) x[v] = lds128(from + ((v & 1 ? kv_next_tile<D>(from_at) : from_at) ^ (v >> 1) * 64));
+        if (dead) {  // no codes
+#pragma unroll
+          for (int v = 0; v < D / 32; ++v) x[v] = make_uint4(kZero, kZero, kZero, kZero);
+        } else if (FMT == kKvE4m3 && V && (j0 + 15 > span.first || p.mask.window)) {
+          // what no row of the block sees may be a NaN code, which a weight of 0 must not meet
+#pragma unroll
+          for (int v = 0; v < D / 32; ++v) {
+            const int j = j0 + (v & 1) * 8 + r;
+            if (j > span.last || (p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks))
+              x[v] = make_uint4(kZero, kZero, kZero, kZero);
+          }
+        }
 #pragma unroll
         for (int v = 0; v < D / 32; ++v) {
-          const int at = kv_at<D>(r, (chunk + (v >> 1) * 4) * 16);
-          uint4 x = lds128(from + (v & 1 ? kv_next_tile<D>(at) : at));
-          bool none = dead;
-          if (FMT == kKvE4m3 && (u & 1)) {
-            // what no row of the block sees may be a NaN code, which a weight of 0 must not meet
-            const int j = j0 + (v & 1) * 8 + r;
-            none |= j > span.last || (p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks);
-          }
-          if (none) x = make_uint4(kZero, kZero, kZero, kZero);
           uint4 lo, hi;
-          convert16<FMT>(x, lo, hi);
-          uint8_t* to = tile + (2 * cw + (v & 1)) * L::kGroup + 2 * (chunk + (v >> 1) * 4) * 128 + r * 16;
+          convert16<FMT, V>(x[v], lo, hi);
+          uint8_t* to = tile + to_at + (v & 1) * L::kGroup + (v >> 1) * 8 * 128;
           *reinterpret_cast<uint4*>(to) = lo;
           *reinterpret_cast<uint4*>(to + 128) = hi;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        return ok;
+        if (lane == 0) mbar_arrive(smem_u32(empty + slot));
+        return true;
       };
-      look_up(lane, meta);
-      __syncwarp();
-      fetch(0);
-      fetch(1);
-      use();
-      int t = 0;
-      for (; t < tiles; ++t) {
+      for (int t = 0; t < tiles; ++t) {
         const int i = t & 1;
         const unsigned n = (i ? done1 : done0) + (t >> 1);
-        if ((t & 31) == 0) {
-          if (t > 0) {
-            meta = ahead;
-            use();
-          }
-          __syncwarp();
-          look_up(t + 32 + lane, ahead);
-          __syncwarp();
-        }
-        const int page = __shfl_sync(0xffffffffu, meta.page, t & 31), j0 = base_of(t);
-        fetch(2 * t + 2);
+        // the entries of the next 32 tiles, when no role reads those of 32 tiles ago any more: K of this tile
+        // can be replaced only when S of the last but one, and so the weights before it, are made
+        if ((t & 31) == 8) meta_table(t + 24);
         if (n > 0 && !wait(s_full(i), n - 1)) break;
-        if (lane == (t & 31)) {  // the lane that holds this tile's step
-          int flags = 0;
-          if (page < 0)
-            flags = kDead;
-          else if (j0 + 15 <= span.first && (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
-            flags = kWhole;
-          // the stream's tile before the last has been read: S of the last was made after its P
-          s_meta[(i * 2 + (n & 1)) * kSteps + cw] = make_float4(meta.ks, vlog, vinv, __int_as_float(j0 | flags));
-        }
-        if (!convert(2 * t, j0, page < 0, smem + L::kK + i * L::kTile)) break;
+        const bool dead = lines[t % kMetaTiles] < 0;
+        const int j0 = span.base(min(i0 + t * kSteps + cw, i1 - 1));
+        if (!convert(2 * t, std::false_type(), dead, j0, smem + L::kK + i * L::kTile)) break;
         if (lane == 0) mbar_arrive(k_full(i));
-        fetch(2 * t + 3);
         if (n > 0 && !wait(o_full(i), n - 1)) break;
-        if (!convert(2 * t + 1, j0, page < 0, smem + L::kV + i * L::kTile)) break;
+        if (!convert(2 * t + 1, std::true_type(), dead, j0, smem + L::kV + i * L::kTile)) break;
         if (lane == 0) mbar_arrive(v_full(i));
       }
-      if (t < tiles)  // lost: wait, within limits, for what is on its way into the ring
-        for (int u = 2 * t; u < min(2 * t + 4, 2 * tiles); ++u)
-          mbar_wait(smem_u32(full + (taken + u) % kSlots), ((taken + u) / kSlots) & 1, kStatusDrainWait);
-      taken += 2 * tiles;
     } else {
       // ---- weights: stream i, this thread's row
       const int i = warp >> 2, row = tid & 127;
@@ -366,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
       const unsigned m = s_seg.m0 + row, G = p.G;
       const int at_row = s_seg.seq.start + static_cast<int>(m / G);
       const int pos = m < static_cast<unsigned>(p.rows.R) * G && at_row < s_seg.seq.len ? at_row : -1;
-      const float qf = sf[row];
+      const float qf = sf[row].x, qt = sf[row].y;
       float ref = 0.f, top_off = -INFINITY, l = 0.f;  // the reference m - 8; how far a logit may pass it: not at all until there is one
       bool ok = true;
       int n_tiles = 0;
@@ -375,82 +388,100 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
         ok = wait(s_full(i), n);
         if (!ok) break;
         tc_after();
-        const float4* meta = s_meta + (i * 2 + (n & 1)) * kSteps;
-        const auto weigh = [&](int k, float (&x)[16]) {  // step k of the tile: 16 logits to 16 weights
+        const float4* meta = s_meta + t % kMetaTiles * kSteps;
+        float xa[16], xb[16];
+        // the row's largest logit: of a step's sums before their factor, which is not negative
+        float most = -INFINITY;
+        int whole = kWhole;
+        const auto largest = [&](int k, const float (&x)[16]) {
           const float4 sc = meta[k];
           const int j0 = __float_as_int(sc.w);
-          const float f = qf * sc.x, d = sc.y - ref;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = x[e] * f + d;
-          if (!(j0 & kWhole)) {
+          whole &= j0;
+          float top;
+          if (j0 & kWhole) {
+            top = max3(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[8])),
+                       max3(x[9], x[10], x[11]), max3(max3(x[12], x[13], x[14]), x[15], x[15]));
+          } else {
             const uint32_t seen = j0 & kDead ? 0u : seen_bits(p.mask, pos, j0 & ~15);
+            top = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = seen >> e & 1 ? x[e] : -INFINITY;
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, seen >> e & 1 ? x[e] : -INFINITY);
           }
-          float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-          for (int e = 4; e < 16; ++e) top[e & 3] = fmaxf(top[e & 3], x[e]);
-          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          if (__any_sync(0xffffffffu, most > top_off)) {
-            // raise the reference, by a whole number: what is there already takes a power of two
-            const bool fresh = top_off == -INFINITY, move = most > -INFINITY;
-            const float up = !move ? 0.f : fresh ? ceilf(most - kWeightLog) : fmaxf(0.f, ceilf(most - kWeightLog));
-            const float g = fresh ? 0.f : ex2(-up);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] -= up;
-            l *= g;
-            ref += up;
-            if (move) top_off = kWeightTop;
-            tm_wait_st();
-            const __half2 g2 = __float2half2_rn(g);
-            float y[16];
-#pragma unroll 1
-            for (int z = 0; z < (k + 1) / 2; ++z) {  // this tile's weights so far, two steps a time
-              tm_begin16(s_col(i) + 16 * z + lanes, y);
-              tm_arrived16(y);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                // an odd last step's other half holds logits
-                const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&y[e]), g2);
-                if (e < 8 || 2 * z + 1 < k) y[e] = *reinterpret_cast<const float*>(&v);
-              }
-              tm_st16(s_col(i) + 16 * z + lanes, y);
-            }
-            if (t != i) {  // the stream's O: all its products so far are complete, this S came after them
-#pragma unroll 1
-              for (int z = 0; z < D / 16; ++z) {
-                tm_begin16(o_col(i) + 16 * z + lanes, y);
-                tm_arrived16(y);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] *= g;
-                tm_st16(o_col(i) + 16 * z + lanes, y);
-              }
-            }
-            tm_wait_st();
-          }
-          uint32_t h[8];
-          float sum[2] = {0.f, 0.f};
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const float y0 = ex2(x[e]), y1 = ex2(x[e + 1]);
-            sum[(e >> 1) & 1] += y0 + y1;
-            const __half2 z = __floats2half2_rn(y0, y1);
-            h[e / 2] = *reinterpret_cast<const uint32_t*>(&z);
-          }
-          l += (sum[0] + sum[1]) * sc.z;
-          tm_st8(s_col(i) + 8 * k + lanes, h);  // columns that have been read
+          const float z = top * (qf * sc.x) + (sc.y - ref - qt * sc.x);
+          most = fmaxf(most, top > -INFINITY ? z : -INFINITY);
         };
-        float xa[16], xb[16];
         tm_begin16(s_col(i) + lanes, xa);
 #pragma unroll 1
         for (int k = 0; k < kSteps; k += 2) {
           tm_arrived16(xa);
           tm_begin16(s_col(i) + 16 * (k + 1) + lanes, xb);
-          weigh(k, xa);
+          largest(k, xa);
           tm_arrived16(xb);
-          if (k + 2 < kSteps) tm_begin16(s_col(i) + 16 * (k + 2) + lanes, xa);
-          weigh(k + 1, xb);
+          tm_begin16(s_col(i) + (k + 2 < kSteps ? 16 * (k + 2) : 0) + lanes, xa);  // at the end: the first again
+          largest(k + 1, xb);
         }
+        if (__any_sync(0xffffffffu, most > top_off)) {
+          const bool fresh = top_off == -INFINITY, move = most > -INFINITY;
+          const float up = !move ? 0.f : fresh ? most - kWeightLog : fmaxf(0.f, most - kWeightLog);
+          const float g = fresh ? 0.f : ex2(-up);
+          l *= g;
+          ref += up;
+          if (move) top_off = kWeightTop;
+          if (t != i) {  // the stream's O: all its products so far are complete, this S came after them
+            float y[16];
+#pragma unroll 1
+            for (int z = 0; z < D / 16; ++z) {
+              tm_begin16(o_col(i) + 16 * z + lanes, y);
+              tm_arrived16(y);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) y[e] *= g;
+              tm_st16(o_col(i) + 16 * z + lanes, y);
+            }
+          }
+        }
+        const auto weigh = [&](int k, auto all, float (&x)[16]) {  // step k of the tile: 16 logits to 16 weights
+          const float4 sc = meta[k];
+          const float f = qf * sc.x, d = sc.y - ref - qt * sc.x;
+          const float2 f2 = make_float2(f, f), d2 = make_float2(d, d);
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float2 y = ffma2(make_float2(x[e], x[e + 1]), f2, d2);
+            x[e] = ex2(y.x);
+            x[e + 1] = ex2(y.y);
+          }
+          if constexpr (!decltype(all)::value) {
+            const int j0 = __float_as_int(sc.w);
+            const uint32_t seen = j0 & kWhole ? 0xFFFFu : j0 & kDead ? 0u : seen_bits(p.mask, pos, j0 & ~15);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = seen >> e & 1 ? x[e] : 0.f;
+          }
+          uint32_t h[8];
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            sum[(e >> 1) & 1] = fadd2(sum[(e >> 1) & 1], make_float2(x[e], x[e + 1]));
+            const __half2 z = __floats2half2_rn(x[e], x[e + 1]);
+            h[e / 2] = *reinterpret_cast<const uint32_t*>(&z);
+          }
+          const float2 both = fadd2(sum[0], sum[1]);
+          l += (both.x + both.y) * sc.z;
+          tm_st8(s_col(i) + 8 * k + lanes, h);  // columns that have been read
+        };
+        const auto weigh_all = [&](auto all) {
+#pragma unroll 1
+          for (int k = 0; k < kSteps; k += 2) {
+            tm_arrived16(xa);
+            tm_begin16(s_col(i) + 16 * (k + 1) + lanes, xb);
+            weigh(k, all, xa);
+            tm_arrived16(xb);
+            if (k + 2 < kSteps) tm_begin16(s_col(i) + 16 * (k + 2) + lanes, xa);
+            weigh(k + 1, all, xb);
+          }
+        };
+        if (whole)
+          weigh_all(std::true_type());
+        else
+          weigh_all(std::false_type());
         tm_wait_st();
         tc_before();
         __syncwarp();
@@ -464,7 +495,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
     }
     done0 += (tiles + 1) / 2;
     done1 += tiles / 2;
+    taken += 2 * tiles;
     __syncthreads();  // all products are complete: K and V make room for the values
+    if (!lost && s_lost && warp == kCopyWarp && lane < kConvWarps)
+      // wait, within limits, for what is on its way into the rings
+      for (unsigned i = 0; i < kSlots; ++i) mbar_wait(smem_u32(bars + 11 + lane * kSlots + i), ((taken + i) / kSlots) & 1, kStatusDrainWait);
     lost |= s_lost != 0;
     if (warp < kSoftWarps) {
       const int i = warp >> 2, row = tid & 127;
