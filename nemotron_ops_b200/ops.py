@@ -299,11 +299,16 @@ def Relu2(x):
 def _kv_args(op, k_cache, v_cache, k_scale, v_scale, table, lens, start=None):
     """Checks what the cache ops share; returns the shape arguments of the cache and the page table."""
     start = lens if start is None else start
-    for t in (k_cache, v_cache, k_scale, v_scale, table, lens, start):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    try:
+        if not (k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and table.is_cuda
+                and lens.is_cuda and start.is_cuda):
             raise RuntimeError("bolt ops take CUDA tensors (there is no CPU implementation)")
-        if not t.is_contiguous():
+        if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+                and v_scale.is_contiguous() and table.is_contiguous() and lens.is_contiguous()
+                and start.is_contiguous()):
             raise RuntimeError("bolt ops take contiguous tensors")
+    except AttributeError:
+        raise RuntimeError("bolt ops take CUDA tensors (there is no CPU implementation)") from None
     if not (k_cache.dtype is v_cache.dtype is torch.uint8 and k_scale.dtype is v_scale.dtype is torch.float32):
         raise RuntimeError(f"{op}: caches are u8, scales f32")
     shape, pages = k_cache.shape, k_scale.shape
@@ -332,6 +337,21 @@ def _kv_rows(op, t, what):
         raise RuntimeError(f"{op}: {what} must be dense over its heads and values")
     # an axis of one entry has no step
     return shape_arg(shape)[0], shape_arg((seq if S > 1 else 0, row if R > 1 else 0))[0]
+
+
+_WORKSPACES: dict = {}
+
+
+def _kv_workspace(like, nbytes):
+    """Scratch memory of a call.  Calls of one stream follow one another, so they share a tensor (an
+    allocation costs two microseconds); a captured call, which may be replayed on any stream, has its own."""
+    if torch.cuda.is_current_stream_capturing():
+        return like.new_empty((nbytes,))
+    key = like.device.index, _stream(like)
+    ws = _WORKSPACES.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _WORKSPACES[key] = like.new_empty((nbytes,))
+    return ws
 
 
 def KvAppend(k, v, k_cache, v_cache, k_scale, v_scale, table, start, lens, fmt: int = KV_INT8):
@@ -366,7 +386,7 @@ def KvAttention(q, k_cache, v_cache, k_scale, v_scale, table, start, lens, scale
     # new_empty of a tensor of the type: half the host time of torch.empty with a type and a device
     o = q.new_empty(q.shape)
     lse = k_scale.new_empty(q.shape[:3])
-    ws = k_cache.new_empty((max(0, lib().bolt_kv_attention_workspace(shape, cs)),))
+    ws = _kv_workspace(k_cache, max(0, lib().bolt_kv_attention_workspace(shape, cs)))
     _check(lib().bolt_kv_attention(_ptr(q), shape, st, _ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
                                    _ptr(table), ts, _ptr(start), _ptr(lens), float(scale), int(window), int(sinks),
                                    int(fmt), _ptr(o), _ptr(lse), _ptr(ws), ws.numel(), _stream(k_cache)))

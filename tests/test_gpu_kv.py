@@ -495,3 +495,121 @@ def test_refusals():
     o, lse = att(q=q[:, :0])
     assert o.shape == (2, 0, 4, 64) and lse.shape == (2, 0, 4)
     assert ops.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# sizes at which a block goes through many steps of several items: 64-bit form on the device
+# ---------------------------------------------------------------------------------------------
+def _large(S, R, Hq, Hkv, D, T, fmt, lens, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    need = [-(-n // T) for n in lens]
+    pool = sum(need) + 1
+    perm = torch.randperm(pool - 1, generator=g, device=DEV).int()
+    table = torch.full((S, max(need)), pool - 1, dtype=torch.int32, device=DEV)
+    at = 0
+    for s, n in enumerate(need):
+        table[s, :n] = perm[at:at + n]
+        at += n
+    caches = []
+    for _ in range(2):
+        x = torch.randn(pool, Hkv, T, D, generator=g, device=DEV) * (O.KV_QMAX[fmt] / 3)
+        x = x.clamp(-O.KV_QMAX[fmt], O.KV_QMAX[fmt])
+        caches.append((x.round() + 128).to(torch.uint8) if fmt == 0 else x.to(torch.float8_e4m3fn).view(torch.uint8))
+    scales = [(torch.rand(pool, Hkv, generator=g, device=DEV) + 0.5) * 3 / O.KV_QMAX[fmt] for _ in range(2)]
+    q = torch.randn(S, R, Hq, D, generator=g, device=DEV).bfloat16()
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    return q, caches, scales, table, n
+
+
+def _check_large(q, caches, scales, table, lens, start, o, lse, score, window, sinks, fmt, samples):
+    """Some (sequence, head) pairs against fp64; bounds as in the module's head."""
+    S, R, Hq, D = q.shape
+    T = caches[0].shape[2]
+    G = Hq // caches[0].shape[1]
+    for s, h in samples:
+        n = int(lens[s])
+        if n == 0:
+            continue
+        idx = torch.arange(n, device=DEV)
+        page = table[s].long()[idx // T]
+        k, v = ((c[page, h, idx % T].double() - 128 if fmt == 0 else c[page, h, idx % T].view(torch.float8_e4m3fn).double())
+                * sc[page, h].double()[:, None] for c, sc in zip(caches, scales))
+        a = int(start[s])
+        qs = q[s, :n - a, h * G:(h + 1) * G].double()
+        x = torch.einsum("rgd,jd->rgj", qs, k) * D ** -0.5
+        ql = torch.einsum("rgd,jd->rgj", qs.abs(), k.abs()).amax(-1) * D ** -0.5
+        pos = a + torch.arange(n - a, device=DEV)[:, None, None]
+        hidden = idx > pos
+        if window:
+            hidden |= (idx <= pos - window) & (idx >= sinks)
+        x = x.masked_fill(hidden, -torch.inf)
+        z = torch.logsumexp(x, -1)
+        p = torch.exp(x - z[..., None])
+        dl = (2 * D + 16) * U * ql
+        rows, heads = slice(0, n - a), slice(h * G, (h + 1) * G)
+        assert bool(((lse[s, rows, heads].double() - z).abs() <= dl + 2.0 ** -20 * (1 + z.abs())).all())
+        want, av = p @ v, p @ v.abs()
+        bound = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -18 + 2 * dl[..., None]) * av
+        assert bool(((o[s, rows, heads].double() - want).abs() <= bound).all())
+        if score is not None:
+            w = p.sum((0, 1))
+            assert bool(((score[s, h, :n].double() - w).abs() <= 2 * (dl.max() + 4 * U * z.abs().max() + 2.0 ** -18) * w
+                         + 2 * U * w).all())
+            assert not score[s, h, n:].any()
+
+
+@pytest.mark.parametrize("S,R,Hq,Hkv,D,T,fmt,longest,window,sinks", [
+    (40, 8, 64, 4, 128, 16, 0, 6000, 0, 0),    # 128 rows a head, more than 32 tiles an item
+    (3, 700, 4, 2, 64, 64, 1, 9000, 0, 0),     # a prompt's chunk behind a long prefix
+    (2, 300, 16, 4, 128, 32, 1, 9000, 700, 33),
+    (24, 1, 16, 8, 128, 32, 0, 20000, 0, 0),   # one row: hundreds of steps a warp
+    (24, 1, 24, 2, 64, 16, 1, 20000, 0, 0),
+    (5, 4, 16, 2, 128, 128, 0, 70000, 0, 0),   # 32 rows a head
+    (6, 7, 16, 2, 64, 16, 0, 30000, 5000, 4),  # 56 rows a head
+    (300, 1, 4, 4, 64, 16, 0, 90, 0, 0),       # more sequences than blocks take at once
+])
+def test_long_items(S, R, Hq, Hkv, D, T, fmt, longest, window, sinks):
+    lens = [max(R, longest * ((s * 7) % S + 1) // S) for s in range(S)]
+    if S > 2:
+        lens[1] = 0
+    q, caches, scales, table, n = _large(S, R, Hq, Hkv, D, T, fmt, lens, seed=S + R)
+    start = (n - R).clamp(min=0)
+    o, lse = ops.KvAttention(q, *caches, *scales, table, start, n, D ** -0.5, window=window, sinks=sinks, fmt=fmt)
+    score = ops.KvScore(q, caches[0], scales[0], table, start, n, lse,
+                        torch.zeros(S, Hkv, table.shape[1] * T, device=DEV), D ** -0.5, window=window, sinks=sinks, fmt=fmt)
+    longest_s = max(range(S), key=lambda s: lens[s])
+    samples = [(longest_s, h) for h in range(Hkv)] + [(s, s % Hkv) for s in range(0, S, max(1, S // 6))]
+    _check_large(q, caches, scales, table, n, start, o, lse, score, window, sinks, fmt, samples)
+    if S > 2:
+        assert not o[1].any() and bool(torch.isneginf(lse[1]).all())
+    assert ops.device_status() == 0
+
+
+def test_calls_on_other_streams():
+    # two streams at once, each with its own inputs: results as one after the other
+    inputs = [_large(4, 2, 16, 2, 128, 32, 0, [3000, 900, 0, 50], seed=90 + i) for i in range(2)]
+    want = []
+    for q, caches, scales, table, n in inputs:
+        want.append(ops.KvAttention(q, *caches, *scales, table, (n - 2).clamp(min=0), n, 0.1))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    starts = [(x[4] - 2).clamp(min=0) for x in inputs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (q, caches, scales, table, n) in enumerate(inputs):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.KvAttention(q, *caches, *scales, table, starts[i], n, 0.1))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, lse in got[i]:
+            assert torch.equal(o, want[i][0]) and torch.equal(lse, want[i][1])
+
+
+def test_a_negative_scale():
+    for R, Hq in ((1, 4), (40, 8)):
+        c = Cache([300], 2, 64, 32, 0, seed=95)
+        q = _rows(1, R, Hq, 64, seed=96)
+        start = c.lens - R
+        o, lse = _attention(c, q, start, -0.125)
+        _check_attention(o, lse, O.kv_attention(q, *c.host(), c.table, start, c.lens, -0.125), 64)
