@@ -613,3 +613,24 @@ def test_a_negative_scale():
         start = c.lens - R
         o, lse = _attention(c, q, start, -0.125)
         _check_attention(o, lse, O.kv_attention(q, *c.host(), c.table, start, c.lens, -0.125), 64)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_the_example_runs(fmt):
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "long_context_decode.py")
+    spec = importlib.util.spec_from_file_location("long_context_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    o, cache = example.main(["--steps", "90", "--prompt", "150", "--budget", "200", "--fmt", fmt])
+    assert bool(torch.isfinite(o).all())
+    # 150 + 50 tokens reach the budget of 200, 100 are kept, 40 more come
+    assert cache.lens.tolist() == cache.length == [140] * 4
+    # every page has one owner
+    pages = cache.free + [p for own in cache.owned for p in own]
+    assert sorted(pages) == list(range(cache.k.shape[0]))
+    # a row's weights sum to 1, and what was evicted left with its sums
+    assert float(cache.score.sum()) > 0 and not cache.score[:, :, 140:].any()
+    assert ops.device_status() == 0
