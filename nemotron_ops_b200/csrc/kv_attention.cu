@@ -489,8 +489,8 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(co
 struct Plan {
   int rows, round, per_sm;
 };
-Plan plan_of(int64_t M) {
-  if (M <= 8) return Plan{8, 4, 3};
+Plan plan_of(int64_t M, int D) {
+  if (M <= 8) return Plan{8, 4, D == 64 ? 4 : 3};
   if (M <= 16) return Plan{16, 4, 2};
   if (M <= 32) return Plan{32, 8, 1};
   if (M <= 64) return Plan{64, 4, 1};
@@ -512,7 +512,7 @@ cudaError_t launch(const KvAttnParams& p, const Work& w, unsigned blocks, const 
 template <int D, int FMT>
 cudaError_t launch_rows(const KvAttnParams& p, const Work& w, int rows, unsigned blocks, const LaunchCfg& cfg) {
   switch (rows) {
-    case 8: return launch<D, FMT, 1, 1, 4, 1, 4, 3>(p, w, blocks, cfg);
+    case 8: return launch<D, FMT, 1, 1, 4, 1, 4, D == 64 ? 4 : 3>(p, w, blocks, cfg);
     case 16: return launch<D, FMT, 2, 1, 4, 1, 4, 2>(p, w, blocks, cfg);
     case 32: return launch<D, FMT, 4, 1, 8, 1, 4, 1>(p, w, blocks, cfg);
     case 64: return launch<D, FMT, 4, 2, 4, 1, 4, 1>(p, w, blocks, cfg);
@@ -525,7 +525,7 @@ int64_t align16(int64_t n) { return (n + 15) & ~int64_t(15); }
 }  // namespace
 
 int64_t kv_attention_workspace(int64_t rows, int D, int sms) {
-  const Plan t = plan_of(rows);
+  const Plan t = plan_of(rows, D);
   const int64_t blocks = static_cast<int64_t>(sms) * t.per_sm;
   return align16(blocks * 2 * t.rows * D * 4) + align16(blocks * 2 * t.rows * 8) + blocks * static_cast<int64_t>(sizeof(Split));
 }
@@ -533,7 +533,7 @@ int64_t kv_attention_workspace(int64_t rows, int D, int sms) {
 cudaError_t launch_kv_attention(const KvAttnParams& params, void* workspace, const LaunchCfg& cfg) {
   KvAttnParams p = params;
   const int64_t M = static_cast<int64_t>(p.rows.R) * p.G;
-  const Plan t = plan_of(M);
+  const Plan t = plan_of(M, p.c.D);
   const int64_t row_blocks = (M + t.rows - 1) / t.rows, items = p.c.S * row_blocks * p.c.heads;
   if (M > 0x7fffffff || p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   p.few_steps = items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16 + kMostItemCost) <= 0x7fffffff;
