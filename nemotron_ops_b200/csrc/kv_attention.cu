@@ -5,18 +5,25 @@
 //
 // One pass with the running maximum and sum of a softmax (kv_mma.cuh has the operands).  The rows of a
 // sequence that read one kv head -- R rows times G query heads -- are the M axis of the products, so
-// the codes are read once for all of them.  A block holds MW x MR tiles of 16 rows and splits their
-// steps over TW warps; the blocks share all steps evenly (kv_share), a segment being one
-// (sequence, row block, head)'s consecutive steps in one block.  At its end the TW partial results
-// are joined through shared memory.  A segment that is a whole item writes the result; the others
-// leave (max, sum, values) in the workspace for kv_combine_kernel, which joins them in block order, so
-// results do not depend on scheduling.
+// the codes are read once for all of them.  A block holds NT tiles of 8 rows and splits their steps over
+// four warps; the blocks share all steps evenly (kv_share), a segment being one (sequence, row block,
+// head)'s consecutive steps in one block.  At its end the four partial results are joined through shared
+// memory.  A segment that is a whole item writes the result; the others leave (max, sum, values) in the
+// workspace for kv_combine_kernel, which joins them in block order, so results do not depend on scheduling.
+// More than 16 rows go to the tensor-memory kernel (kv_attention_umma.cu).
 //
 // Rounding: logits, maxima, sums and values are fp32; a weight is rounded to fp16 (11 bits) once, as
 // the second product's operand.  A row's weights are 2^(x - m + 8) for its logits x (in units of log 2)
 // and a reference m that is raised to the row's maximum only when some x passes m + 7: weights stay
 // below 2^15, those down to 2^-22 of the reference keep all 11 bits, and most steps need neither the
 // maximum over the row's lanes nor a rescaling.
+//
+// HBM bounds it where there is enough to read: 64 sequences of up to 8,192 positions, 8 heads, 4 rows a head
+// take 95 us with the joining, 5.7 TB/s.  Tensor copies into a ring, because the codes must be on their way well
+// ahead of their use and 16-byte copies by the lanes do not get there: with the arithmetic taken out they read
+// 3.8 TB/s at any ring depth, tensor copies 5.9.  One sequence of 131,001 positions (16 rows a head, 2 heads)
+// takes 30 us, 22 of them here: the way from the length to the first product, 37 steps a warp, and the parts'
+// 2.4 MB.  Short items (48 sequences, 16 heads of 64 values, 68 steps an item: 36 us) are bound by their set-up.
 #include "kv_split.cuh"
 
 namespace bolt {
@@ -26,18 +33,19 @@ namespace {
 // Of an item's set-up, in steps: about 6 us, measured in a batch of 64 sequences of up to 8,192 positions.
 constexpr int kItemCost = 16;
 
-// NT tiles of 8 rows a warp, MW warps along the rows, TW along the steps; a warp takes NP steps at a
-// time, from a ring of STAGES steps.
-template <int D, int NT, int MW, int TW, int NP, int STAGES>
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kStages = 4;  // steps of a warp's ring
+
+// NT tiles of 8 rows.
+template <int D, int NT>
 struct Tile {
-  static constexpr int kRows = NT * MW * 8, kWarps = MW * TW, kThreads = kWarps * 32;
-  static constexpr int kStep = D * 2;                    // uint4 of a warp's step: 16 positions, K and V
-  static constexpr int kRing = kWarps * STAGES * kStep;  // uint4
-  static constexpr int kJoin = TW * kRows * D / 4;       // uint4, in the ring's place
-  static constexpr bool kQRegs = NT <= 2;                // query operands in registers, else in shared memory
-  static constexpr int kQ = kQRegs ? 0 : MW * NT * (D / 16) * 32;  // uint2
-  static constexpr size_t kSmem = (kRing > kJoin ? kRing : kJoin) * 16 + kQ * 8 + kWarps * (64 * 20 + STAGES * 8) +
-                                  TW * kRows * 8 + 1024;  // the ring starts on a 1,024-byte boundary
+  static constexpr int kRows = NT * 8;
+  static constexpr int kStep = 32 * D;                       // bytes of a warp's step: 16 positions, K and V
+  static constexpr int kRing = kWarps * kStages * kStep;
+  static constexpr int kJoin = kWarps * kRows * D * 4;       // in the ring's place
+  static_assert(kJoin <= kRing, "the joining buffer takes the ring's place");
+  static constexpr size_t kSmem = kRing + kWarps * (64 * 20 + kStages * 8) + kWarps * kRows * 8 +
+                                  1024;  // the ring starts on a 1,024-byte boundary
 };
 
 // float4 index f of a row's values in the joining buffer, spread over the banks
@@ -79,32 +87,30 @@ struct VCodes {
   }
 };
 
-template <int D, int FMT, int NT, int MW, int TW, int NP, int STAGES, int CPS>
-__global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
+template <int D, int FMT, int NT, int CPS>
+__global__ void __launch_bounds__(kThreads, CPS) kv_attention_kernel(
     const KvAttnParams p, const Work w, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-  using L = Tile<D, NT, MW, TW, NP, STAGES>;
+  using L = Tile<D, NT>;
   extern __shared__ uint4 smem_raw[];
-  uint4* smem = reinterpret_cast<uint4*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float4* so = reinterpret_cast<float4*>(smem);                            // [TW][rows][D / 4]
-  uint4* tail = smem + (L::kRing > L::kJoin ? L::kRing : L::kJoin);
-  uint2* sq = reinterpret_cast<uint2*>(tail);                              // [MW * NT][D / 16][32]
-  float4* s_scale = reinterpret_cast<float4*>(sq + L::kQ);                 // [warps][64]: K scale, log2 and 1 / V scale, position and flags
-  int* s_row = reinterpret_cast<int*>(s_scale + L::kWarps * 64);           // [warps][64]: first line of the codes, or -1
-  uint64_t* s_full = reinterpret_cast<uint64_t*>(s_row + L::kWarps * 64);  // [warps][STAGES]: barriers of the ring
-  float* sm = reinterpret_cast<float*>(s_full + L::kWarps * STAGES);       // [TW][rows]
-  float* sl = sm + TW * L::kRows;                                          // [TW][rows]
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float4* so = reinterpret_cast<float4*>(smem);                         // [warps][rows][D / 4]
+  float4* s_scale = reinterpret_cast<float4*>(smem + L::kRing);         // [warps][64]: K scale, log2 and 1 / V scale, position and flags
+  int* s_row = reinterpret_cast<int*>(s_scale + kWarps * 64);           // [warps][64]: first line of the codes, or -1
+  uint64_t* s_full = reinterpret_cast<uint64_t*>(s_row + kWarps * 64);  // [warps][kStages]: barriers of the ring
+  float* sm = reinterpret_cast<float*>(s_full + kWarps * kStages);      // [warps][rows]
+  float* sl = sm + kWarps * L::kRows;                                   // [warps][rows]
   pdl_wait();
   pdl_trigger();
   const KvCache& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
-  const int mw = warp % MW, tk = warp / MW;
-  uint8_t* ring = reinterpret_cast<uint8_t*>(smem + warp * STAGES * L::kStep);
+  uint8_t* ring = smem + warp * kStages * L::kStep;
+  const uint32_t ring_at = smem_u32(ring);
   const unsigned M = static_cast<unsigned>(p.rows.R) * p.G, G = p.G;
   s_scale += warp * 64;
   s_row += warp * 64;
-  s_full += warp * STAGES;
+  s_full += warp * kStages;
   if (lane == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(s_full + i), 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(smem_u32(s_full + i), 1);
     fence_barrier_init();
     asm volatile("fence.proxy.async;" ::: "memory");
   }
@@ -113,9 +119,9 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
   bool stuck = false;   // a copy did not arrive in time: the rest of the work is left
   const int k_at = kv_at<D>(place<D>(g), 16 * q4);  // the codes 64 i + 16 q4 .. are at k_at ^ 64 i
   const int v_at[2] = {kv_at<D>(place<D>(2 * q4), D / 8 * g), kv_at<D>(place<D>(2 * q4 + 1), D / 8 * g)};
-  const KvShare share = kv_share<L::kThreads>(p, w.row_blocks, L::kRows, TW * NP, kItemCost);
+  const KvShare share = kv_share<kThreads>(p, w.row_blocks, L::kRows, kWarps, kItemCost);
 
-  kv_empty_items<D, L::kRows, L::kThreads>(p, w);
+  kv_empty_items<D, L::kRows, kThreads>(p, w);
 
   KvWalk walk;
   walk.start(share);
@@ -125,63 +131,57 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
     const KvSeq& seq = seg.seq;
     const KvSpan& span = seg.span;
 
-    // ---- the segment: steps i0 .. i1 - 1; this warp's k-th is the k % NP-th of the group k / NP * TW + tk
-    const unsigned m1 = m0 + mw * NT * 8;  // this warp's first row
-    const KvSpan mine = kv_span(p, seq, min(m1, M), NT * 8);
-    const int rounds = mine.n > 0 && !stuck ? max(0, (i1 - i0 - tk * NP + TW * NP - 1) / (TW * NP)) : 0;
-    const auto step_of = [&](int k) { return i0 + (k / NP * TW + tk) * NP + k % NP; };
+    // ---- the segment: steps i0 .. i1 - 1; this warp's k-th is i0 + k kWarps + warp
+    const int steps = max(0, (i1 - i0 - warp + kWarps - 1) / kWarps) * !stuck;
+    const auto step_of = [&](int k) { return i0 + k * kWarps + warp; };
     uint4 raw_q[NT][D / 64][2];
 #pragma unroll
-    for (int r = 0; r < NT; ++r) kv_fetch_q<D>(p, seq, s, h, m1 + r * 8, raw_q[r]);
+    for (int r = 0; r < NT; ++r) kv_fetch_q<D>(p, seq, s, h, m0 + r * 8, raw_q[r]);
     // offsets and scales of 32 steps, one a lane, made in three stages so that the loads of one are under way
     // while steps are computed
     KvPages meta;
     const auto look_up_page = [&](int k) {
-      const int i = step_of(k);
-      meta.load_page(c, s, k < rounds * NP && i < i1, span.base(min(i, i1 - 1)));
+      meta.load_page(c, s, k < steps, span.base(min(step_of(k), i1 - 1)));
     };
     const auto look_up_scales = [&](int k) {
       meta.check_page(c);
       meta.load_scales<true>(c, h);
       s_row[k & 63] = meta.page < 0 ? -1 : ((meta.page * c.heads + h) * c.T + (span.base(step_of(k)) & (c.T - 1))) / (128 / D);
     };
-    constexpr int kDead = 1, kWhole = 2;  // none of the warp's rows sees the step, or all see all of it
+    constexpr int kDead = 1, kWhole = 2;  // none of the rows sees the step, or all see all of it
     const auto keep = [&](int k) {
       const int j0 = span.base(min(step_of(k), i1 - 1));
       int flags = 0;
-      if (meta.page < 0 || j0 > mine.last)
+      if (meta.page < 0 || j0 > span.last)
         flags = kDead;
-      else if (j0 + 15 <= mine.first &&
-               (p.mask.window == 0 || j0 > mine.last - p.mask.window || j0 + 15 < p.mask.sinks))
+      else if (j0 + 15 <= span.first &&
+               (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
         flags = kWhole;
       const float vs = fmaxf(meta.vs, 0x1p-96f);
       s_scale[k & 63] = make_float4(meta.ks, log2f(vs), 1.f / vs, __int_as_float(j0 | flags));
     };
-    const auto fetch = [&](int n) {  // round n into its places in the ring
+    const auto fetch = [&](int k) {  // step k into its place in the ring
       __syncwarp();  // which no lane reads any more
-      if (lane != 0 || n >= rounds) return;
-#pragma unroll
-      for (int u = 0; u < NP; ++u) {
-        const unsigned slot = (taken + n * NP + u) % STAGES;
-        const int row = s_row[(n * NP + u) & 63];
-        const uint32_t bar = smem_u32(s_full + slot), to = smem_u32(ring + slot * L::kStep * 16);
-        if (row >= 0) {
-          mbar_arrive_expect_tx(bar, 32 * D);
-          tma_load_3d(to, &map_k, 0, row, 0, bar);
-          tma_load_3d(to + 16 * D, &map_v, 0, row, 0, bar);
-        } else {
-          mbar_arrive(bar);
-        }
+      if (lane != 0 || k >= steps) return;
+      const unsigned slot = (taken + k) % kStages;
+      const int row = s_row[k & 63];
+      const uint32_t bar = smem_u32(s_full + slot), to = ring_at + slot * L::kStep;
+      if (row >= 0) {
+        mbar_arrive_expect_tx(bar, 32 * D);
+        tma_load_3d(to, &map_k, 0, row, 0, bar);
+        tma_load_3d(to + 16 * D, &map_v, 0, row, 0, bar);
+      } else {
+        mbar_arrive(bar);
       }
     };
-    constexpr int kAhead = STAGES / NP - 1;
+    constexpr int kAhead = kStages - 1;
     look_up_page(lane);
     look_up_scales(lane);
     __syncwarp();
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) fetch(n);
+    for (int k = 0; k < kAhead; ++k) fetch(k);
     keep(lane);
-    uint2 q[L::kQRegs ? NT : 1][D / 16];
+    uint2 q[NT][D / 16];
     float qf[NT][2], qt[NT][2];  // of the rows 2 q4 and 2 q4 + 1 of each tile, as all that follow
     int pos[NT][2];
     float o[NT][D / 16][4], l_run[NT][2];
@@ -189,15 +189,12 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
       float f, t;
-      kv_make_q<D, FMT>(p, raw_q[r], q[L::kQRegs ? r : 0], f, t);
-      if (!L::kQRegs && tk == 0)
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) sq[((mw * NT + r) * (D / 16) + kk) * 32 + lane] = q[0][kk];
+      kv_make_q<D, FMT>(p, raw_q[r], q[r], f, t);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         qf[r][e] = __shfl_sync(0xffffffffu, f, (2 * q4 + e) * 4);
         qt[r][e] = __shfl_sync(0xffffffffu, t, (2 * q4 + e) * 4);
-        const unsigned m = m1 + r * 8 + 2 * q4 + e;
+        const unsigned m = m0 + r * 8 + 2 * q4 + e;
         const int row = seq.start + static_cast<int>(m / G);
         pos[r][e] = m < M && row < seq.len ? row : -1;
         m_ref[r][e] = 0.f;
@@ -209,90 +206,67 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[r][t2][x] = 0.f;
     }
-    if constexpr (L::kQRegs)
-      __syncwarp();
-    else
-      __syncthreads();
-    const auto q_of = [&](int r, int kk) {
-      return L::kQRegs ? q[L::kQRegs ? r : 0][kk] : sq[((mw * NT + r) * (D / 16) + kk) * 32 + lane];
-    };
+    __syncwarp();
 
-    for (int n = 0; n < rounds; ++n) {
-      const int k0 = n * NP;
-      if ((k0 & 7) == 0) {
-        const int later = (k0 & ~31) + 32 + lane;
+    for (int k = 0; k < steps; ++k) {
+      if ((k & 7) == 0) {
+        const int later = (k & ~31) + 32 + lane;
         __syncwarp();  // no lane reads the entries of 32 steps ago any more
-        if ((k0 & 31) == 0) look_up_page(later);
-        if ((k0 & 31) == 8) look_up_scales(later);
-        if ((k0 & 31) == 16) keep(later);
+        if ((k & 31) == 0) look_up_page(later);
+        if ((k & 31) == 8) look_up_scales(later);
+        if ((k & 31) == 16) keep(later);
         __syncwarp();
       }
-      fetch(n + kAhead);
-#pragma unroll
-      for (int u = 0; u < NP; ++u) {
-        const unsigned i = taken + k0 + u;
-        stuck |= !mbar_wait(smem_u32(s_full + i % STAGES), (i / STAGES) & 1, kStatusFullWait);
-      }
+      fetch(k + kAhead);
+      const unsigned at = taken + k;
+      stuck |= !mbar_wait(smem_u32(s_full + at % kStages), (at / kStages) & 1, kStatusFullWait);
       if (__any_sync(0xffffffffu, stuck)) {
         // wait, within limits, for what else is on its way into the ring
-        for (int k = k0; k < min(n + kAhead + 1, rounds) * NP; ++k)
-          mbar_wait(smem_u32(s_full + (taken + k) % STAGES), ((taken + k) / STAGES) & 1, kStatusDrainWait);
+        for (int i = k; i < min(k + kAhead + 1, steps); ++i)
+          mbar_wait(smem_u32(s_full + (taken + i) % kStages), ((taken + i) / kStages) & 1, kStatusDrainWait);
         stuck = true;
         break;
       }
 
-      const uint8_t* b[NP];
-      float4 sc[NP];
-      int j0[NP];
-      int all = kDead | kWhole;
-#pragma unroll
-      for (int u = 0; u < NP; ++u) {
-        b[u] = ring + (taken + k0 + u) % STAGES * L::kStep * 16;
-        sc[u] = s_scale[(k0 + u) & 63];
-        j0[u] = __float_as_int(sc[u].w);
-        all &= j0[u];
-      }
-      if (all & kDead) continue;
-      const bool whole = all & kWhole;
+      const uint8_t* b = ring + at % kStages * L::kStep;
+      const float4 sc = s_scale[k & 63];
+      const int j0 = __float_as_int(sc.w) & ~15, flags = __float_as_int(sc.w);
+      if (flags & kDead) continue;
+      const bool whole = flags & kWhole;
       // logits in units of log 2, with the value scale's logarithm added, less the reference: lane (g, q4) has
       // the positions place(g) and 8 + place(g) (index 2 i) and the rows 2 q4 and 2 q4 + 1 (index e)
-      float x[NT][NP][4];
+      float x[NT][4];
 #pragma unroll
-      for (int u = 0; u < NP; ++u)
+      for (int i = 0; i < D / 64; ++i) {
+        const uint4 lo = lds128(b + (k_at ^ (64 * i))), hi = lds128(b + (kv_next_tile<D>(k_at) ^ (64 * i)));
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const uint4 lo = lds128(b[u] + (k_at ^ (64 * i))), hi = lds128(b[u] + (kv_next_tile<D>(k_at) ^ (64 * i)));
+        for (int y = 0; y < 4; ++y) {
+          uint32_t a0, a1, a2, a3;
+          k_to_half<FMT>(word_of(lo, y), a0, a2);
+          k_to_half<FMT>(word_of(hi, y), a1, a3);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            uint32_t a0, a1, a2, a3;
-            k_to_half<FMT>(word_of(lo, y), a0, a2);
-            k_to_half<FMT>(word_of(hi, y), a1, a3);
-#pragma unroll
-            for (int r = 0; r < NT; ++r) {
-              const uint2 qb = q_of(r, 4 * i + y);
-              if (i + y == 0)
-                mma16816_first(x[r][u], a0, a1, a2, a3, qb.x, qb.y);
-              else
-                mma16816(x[r][u], a0, a1, a2, a3, qb.x, qb.y);
-            }
+          for (int r = 0; r < NT; ++r) {
+            const uint2 qb = q[r][4 * i + y];
+            if (i + y == 0)
+              mma16816_first(x[r], a0, a1, a2, a3, qb.x, qb.y);
+            else
+              mma16816(x[r], a0, a1, a2, a3, qb.x, qb.y);
           }
         }
+      }
       bool over = false;
 #pragma unroll
       for (int r = 0; r < NT; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float top = -INFINITY;
+          const float f = qf[r][e] * sc.x, d = sc.y - m_ref[r][e] - qt[r][e] * sc.x;
 #pragma unroll
-          for (int u = 0; u < NP; ++u) {
-            const float f = qf[r][e] * sc[u].x, d = sc[u].y - m_ref[r][e] - qt[r][e] * sc[u].x;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& z = x[r][u][2 * i + e];
-              z = z * f + d;
-              if (!whole && ((j0[u] & kDead) || !kv_sees(p.mask, pos[r][e], (j0[u] & ~15) + 8 * i + place<D>(g)))) z = -INFINITY;
-              top = fmaxf(top, z);
-            }
+          for (int i = 0; i < 2; ++i) {
+            float& z = x[r][2 * i + e];
+            z = z * f + d;
+            if (!whole && !kv_sees(p.mask, pos[r][e], j0 + 8 * i + place<D>(g))) z = -INFINITY;
+            top = fmaxf(top, z);
           }
           over |= top > m_top[r][e];
         }
@@ -301,9 +275,7 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
         for (int r = 0; r < NT; ++r)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < NP; ++u) top = fmaxf(top, fmaxf(x[r][u][e], x[r][u][2 + e]));
+            float top = fmaxf(x[r][e], x[r][2 + e]);
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -311,11 +283,8 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
             // a row that sees nothing new keeps its reference
             if (top == -INFINITY) continue;
             const float up = fresh ? top - kWeightLog : fmaxf(0.f, top - kWeightLog), f = fresh ? 0.f : ex2(-up);
-#pragma unroll
-            for (int u = 0; u < NP; ++u) {
-              x[r][u][e] -= up;
-              x[r][u][2 + e] -= up;
-            }
+            x[r][e] -= up;
+            x[r][2 + e] -= up;
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
               o[r][t][e] *= f;
@@ -327,52 +296,45 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
           }
       }
       // weights, as the second product's B operand: positions and rows change places
-      uint32_t w0[NT][NP], w1[NT][NP];
+      uint32_t w0[NT], w1[NT];
 #pragma unroll
-      for (int r = 0; r < NT; ++r)
+      for (int r = 0; r < NT; ++r) {
+        float y[4];
 #pragma unroll
-        for (int u = 0; u < NP; ++u) {
-          float y[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = ex2(x[r][u][e]);
-          l_run[r][0] += (y[0] + y[2]) * sc[u].z;
-          l_run[r][1] += (y[1] + y[3]) * sc[u].z;
-          w0[r][u] = transpose8(__floats2half2_rn(y[0], y[1]));
-          w1[r][u] = transpose8(__floats2half2_rn(y[2], y[3]));
-        }
-#pragma unroll
-      for (int u = 0; u < NP; ++u) {
-        VCodes<D> v;
-        v.load(b[u] + 16 * D, v_at);
-        if (!whole) {
-          // weights of 0 must not meet NaN: a step that was not copied, or a stale e4m3 code that no row of the warp sees
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = (j0[u] & ~15) + (i >> 1) * 8 + place<D>(2 * q4 + (i & 1));
-            if ((j0[u] & kDead) || (FMT == kKvE4m3 && (j > mine.last || (p.mask.window && j <= mine.first - p.mask.window &&
-                                                                 j >= p.mask.sinks))))
-#pragma unroll
-              for (int wd = 0; wd < D / 32; ++wd) v.w[i][wd] = 0;
-          }
-        }
-        // the value axis: rows g and 8 + g of tile t are the values (D / 8) g + 2 t and + 1.  Lifted int8 codes
-        // are the subnormals 2^-24 code; a second product with -2^-17 takes their offset of 128 off in every step
-#pragma unroll
-        for (int wd = 0; wd < D / 32; ++wd)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t sel = i ? 0x7362u : 0x5140u;
-            uint32_t a0, a1, a2, a3;
-            codes_to_half<FMT>(prmt(v.w[0][wd], v.w[1][wd], sel), a0, a1);
-            codes_to_half<FMT>(prmt(v.w[2][wd], v.w[3][wd], sel), a2, a3);
-#pragma unroll
-            for (int r = 0; r < NT; ++r) mma16816(o[r][2 * wd + i], a0, a1, a2, a3, w0[r][u], w1[r][u]);
-          }
+        for (int e = 0; e < 4; ++e) y[e] = ex2(x[r][e]);
+        l_run[r][0] += (y[0] + y[2]) * sc.z;
+        l_run[r][1] += (y[1] + y[3]) * sc.z;
+        w0[r] = transpose8(__floats2half2_rn(y[0], y[1]));
+        w1[r] = transpose8(__floats2half2_rn(y[2], y[3]));
       }
+      VCodes<D> v;
+      v.load(b + 16 * D, v_at);
+      if (FMT == kKvE4m3 && !whole) {
+        // weights of 0 must not meet NaN: a stale e4m3 code that no row of the block sees
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = j0 + (i >> 1) * 8 + place<D>(2 * q4 + (i & 1));
+          if (j > span.last || (p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks))
+#pragma unroll
+            for (int wd = 0; wd < D / 32; ++wd) v.w[i][wd] = 0;
+        }
+      }
+      // the value axis: rows g and 8 + g of tile t are the values (D / 8) g + 2 t and + 1
+#pragma unroll
+      for (int wd = 0; wd < D / 32; ++wd)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t sel = i ? 0x7362u : 0x5140u;
+          uint32_t a0, a1, a2, a3;
+          codes_to_half<FMT>(prmt(v.w[0][wd], v.w[1][wd], sel), a0, a1);
+          codes_to_half<FMT>(prmt(v.w[2][wd], v.w[3][wd], sel), a2, a3);
+#pragma unroll
+          for (int r = 0; r < NT; ++r) mma16816(o[r][2 * wd + i], a0, a1, a2, a3, w0[r], w1[r]);
+        }
     }
-    taken += rounds * NP;
+    taken += steps;
 
-    // ---- join the TW warps of each row
+    // ---- join the warps of each row
 #pragma unroll
     for (int r = 0; r < NT; ++r)
 #pragma unroll
@@ -384,9 +346,9 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
         // the maximum's place takes the reference; none for rows that do not exist
         m_ref[r][e] = pos[r][e] < 0 || m_top[r][e] == -INFINITY ? -INFINITY : m_ref[r][e] + kWeightLog;
         if (g == 0) {
-          const int row = (mw * NT + r) * 8 + 2 * q4 + e;
-          sm[tk * L::kRows + row] = m_ref[r][e];
-          sl[tk * L::kRows + row] = l;
+          const int row = r * 8 + 2 * q4 + e;
+          sm[warp * L::kRows + row] = m_ref[r][e];
+          sl[warp * L::kRows + row] = l;
         }
       }
     __syncthreads();  // and all rings are idle
@@ -394,12 +356,12 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
     for (int r = 0; r < NT; ++r)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = (mw * NT + r) * 8 + 2 * q4 + e;
+        const int row = r * 8 + 2 * q4 + e;
         float top = sm[row];
 #pragma unroll
-        for (int k = 1; k < TW; ++k) top = fmaxf(top, sm[k * L::kRows + row]);
+        for (int k = 1; k < kWarps; ++k) top = fmaxf(top, sm[k * L::kRows + row]);
         const float f = m_ref[r][e] == -INFINITY ? 0.f : ex2(m_ref[r][e] - top);
-        float4* to = so + (tk * L::kRows + row) * (D / 4);
+        float4* to = so + (warp * L::kRows + row) * (D / 4);
 #pragma unroll
         for (int t = 0; t < D / 16; t += 2) {
           float4 v = make_float4(o[r][t][e] * f, o[r][t][2 + e] * f, o[r][t + 1][e] * f, o[r][t + 1][2 + e] * f);
@@ -408,13 +370,14 @@ __global__ void __launch_bounds__(MW * TW * 32, CPS) kv_attention_kernel(
         }
       }
     __syncthreads();
-    kv_finish<D, L::kRows, TW, L::kThreads>(p, w, share, seg, sm, sl, so, Swizzle<D>());
+    kv_finish<D, L::kRows, kWarps, kThreads>(p, w, share, seg, sm, sl, so, Swizzle<D>());
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next segment's copies come after these reads and writes
     __syncthreads();
   }
 }
 
-// Joins the parts of the items that lie in several blocks: WPR warps a row, a lane D / 32 values.
+// Joins the parts of the items that lie in several blocks: WPR warps a row, a lane D / 32 values.  Latency bounds
+// it (the item, the parts' maxima, the parts), so that a row of many parts has 32 warps: 6 us for 148 parts.
 template <int D, int WPR>
 __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(const KvAttnParams p, const Work w, int rows) {
   constexpr int E = D / 32, W = WPR > 8 ? WPR : 8, RPB = W / WPR;
@@ -483,39 +446,38 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(co
   if (lane == 0) p.lse[out] = l > 0.f ? (top - kWeightLog + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// The tiling for M = R * G rows a kv head.  Up to 16 rows: tiles of 8 or 16 rows whose steps four warps
-// share, several blocks an SM.  More: 32 rows a warp, so that a converted operand serves four tiles, one
-// block an SM; beyond 64 rows the tensor-memory kernel (kv_attention_umma.cu).
+// The tiling for M = R * G rows a kv head.  Up to 16 rows: tiles of 8 or 16 rows whose steps four warps share,
+// several blocks an SM.  More: 128 rows, the tensor-memory kernel, one block an SM.  It costs the same for 17 rows
+// as for 128, the other the more the more rows it has.  Both sides, in us, heads of 128 values (tiles of 32 and
+// 64 rows for the first, which it had before): 32 sequences of 8,192 positions, 8 heads: 76 with 16 rows here,
+// 153 : 136 with 24, 158 : 137 with 32 and 244 : 144 with 64; 8 sequences of 16,384, 1 head: 30 : 31 with 32,
+// 45 : 32 with 64; one of 4,000: 17.5 : 17.9 with 32, 18.0 : 18.6 with 64.  Registers set the blocks an SM.
 struct Plan {
   int rows, round, per_sm;
 };
 Plan plan_of(int64_t M, int D) {
-  if (M <= 8) return Plan{8, 4, D == 64 ? 4 : 3};
-  if (M <= 16) return Plan{16, 4, 2};
-  if (M <= 32) return Plan{32, 8, 1};
-  if (M <= 64) return Plan{64, 4, 1};
+  if (M <= 8) return Plan{8, kWarps, D == 64 ? 4 : 3};
+  if (M <= 16) return Plan{16, kWarps, 2};
   return Plan{128, 8, 1};
 }
 
-template <int D, int FMT, int NT, int MW, int TW, int NP, int STAGES, int CPS>
+template <int D, int FMT, int NT, int CPS>
 cudaError_t launch(const KvAttnParams& p, const Work& w, unsigned blocks, const LaunchCfg& cfg) {
-  using L = Tile<D, NT, MW, TW, NP, STAGES>;
+  using L = Tile<D, NT>;
   static SmemOptIn opt;
-  auto kern = kv_attention_kernel<D, FMT, NT, MW, TW, NP, STAGES, CPS>;
+  auto kern = kv_attention_kernel<D, FMT, NT, CPS>;
   const cudaError_t e = allow_smem(kern, L::kSmem, opt);
   if (e != cudaSuccess) return e;
   CUtensorMap map_k, map_v;
   if (!kv_code_map(&map_k, p.c, p.c.k) || !kv_code_map(&map_v, p.c, p.c.v)) return cudaErrorInvalidValue;
-  return launch_kernel(kern, dim3(blocks), dim3(L::kThreads), L::kSmem, cfg, p, w, map_k, map_v);
+  return launch_kernel(kern, dim3(blocks), dim3(kThreads), L::kSmem, cfg, p, w, map_k, map_v);
 }
 
 template <int D, int FMT>
 cudaError_t launch_rows(const KvAttnParams& p, const Work& w, int rows, unsigned blocks, const LaunchCfg& cfg) {
   switch (rows) {
-    case 8: return launch<D, FMT, 1, 1, 4, 1, 4, D == 64 ? 4 : 3>(p, w, blocks, cfg);
-    case 16: return launch<D, FMT, 2, 1, 4, 1, 4, 2>(p, w, blocks, cfg);
-    case 32: return launch<D, FMT, 4, 1, 8, 1, 4, 1>(p, w, blocks, cfg);
-    case 64: return launch<D, FMT, 4, 2, 4, 1, 4, 1>(p, w, blocks, cfg);
+    case 8: return launch<D, FMT, 1, D == 64 ? 4 : 3>(p, w, blocks, cfg);
+    case 16: return launch<D, FMT, 2, 2>(p, w, blocks, cfg);
     default: return launch_kv_attention_umma(p, w, blocks, cfg);
   }
 }

@@ -12,7 +12,9 @@
 //
 // Both are streams of HBM bytes (append 2 in, 1 out a value; read 1 in, 2 out).  KvAppend gives a block the
 // new rows of one (page, head), which it holds in registers between the maximum and the rounding, so each
-// value is read once.
+// value is read once.  2 sequences of 6,000 rows, 8 heads of 128 values, K and V: 38 us to write and read them
+// back.  KvAppend by itself takes 24, bound by the instructions of the rounding (2.7 issued a cycle; 29 us with a
+// division a value); KvRead goes at HBM's rate.  One row of each of 64 sequences: 10 us, latency.
 namespace bolt {
 
 namespace {

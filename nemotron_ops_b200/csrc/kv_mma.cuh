@@ -303,8 +303,7 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
-// Four K codes as fp16 pairs: an int8 code's byte alone is the
-// subnormal 2^-24 code, and its offset of 128 comes off the logit as 128 times the sum of the query row
+// Four K codes as fp16 pairs: an int8 code's byte alone is the subnormal 2^-24 code, and its offset of 128 comes off the logit as 128 times the sum of the query row
 // (kv_make_q), which costs one operation a row instead of one a pair.
 template <int FMT>
 __device__ __forceinline__ void k_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {

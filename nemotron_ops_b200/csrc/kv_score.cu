@@ -5,7 +5,10 @@
 // 16 positions belong to one warp, which copies their K codes into a ring of its own ahead of time and
 // keeps them as fp16 operands in registers while it goes through the row tiles: a sum is made by one warp
 // in one order and added to the score once for each kRowTiles * 8 rows, by a reduction in memory that
-// nothing waits for and no other warp makes for these positions.
+// nothing waits for and no other warp makes for these positions.  Instruction issue bounds it where there is
+// enough to do: 32 sequences of up to 8,192 positions, 8 heads of 64 values, 16 rows a head take 41 us, 290
+// instructions a KB of codes.  One sequence of 65,536 positions, 2 heads of 128, 16 rows: 11 us, of which the
+// bytes are 2.7 and the way from the length to the first codes most of the rest.
 #include "kv_mma.cuh"
 
 namespace bolt {
@@ -16,7 +19,8 @@ constexpr int kWarps = 8;
 constexpr int kItemCost = 16;  // of an item's set-up, in steps (kv_attention.cu has the measurement)
 constexpr int kRowTiles = 16;  // tiles of 8 query rows in shared memory at a time
 // Steps that a warp takes at a time and steps of its ring.  Steps of 64 values are too short for one alone
-// (32 sequences of up to 8,192 positions, 8 heads: 54 us one at a time, 42 us two); two of 128 values leave one block an SM (65,536 positions, 2 heads: 12 us one at a time, 18 us two).
+// (32 sequences of up to 8,192 positions, 8 heads: 54 us one at a time, 42 us two); two of 128 values leave one
+// block an SM (65,536 positions, 2 heads: 12 us one at a time, 18 us two).
 template <int D>
 constexpr int kTogether = D == 64 ? 2 : 1;
 template <int D>

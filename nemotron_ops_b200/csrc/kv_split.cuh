@@ -5,6 +5,8 @@
 
 namespace bolt {
 
+// Weights are 2^(x - reference + kWeightLog) of their logits x, fp16 operands: at most 2^kWeightTop, and a row's
+// largest at least 2^kWeightLog when its reference was last raised.
 constexpr float kWeightLog = 8.f, kWeightTop = 15.f;
 
 struct Split {  // segments of one item: the first in block `block`'s slot 2 block + 1, the i-th in 2 (block + i)
@@ -110,7 +112,7 @@ __device__ __forceinline__ void kv_empty_items(const KvAttnParams& p, const Work
   }
 }
 
-// The kernel for more than 64 rows a kv head (kv_attention_umma.cu): 128 rows a block, one block an SM.
+// The kernel for more than 16 rows a kv head (kv_attention_umma.cu): 128 rows a block, one block an SM.
 cudaError_t launch_kv_attention_umma(const KvAttnParams& p, const Work& w, unsigned blocks, const LaunchCfg& cfg);
 
 }  // namespace bolt
