@@ -307,7 +307,9 @@ BOLT_API int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const
  * Rows that do not exist give o = 0 and lse = -inf.
  *   workspace  scratch device memory of bolt_kv_attention_workspace(q_shape, cache_shape) bytes on the
  *              current device (-1: bad shapes), 16-byte aligned; nothing has to be in it, and nothing
- *              of it is read by a later call
+ *              of it is read by a later call.  The call enqueues two kernels that meet in it, so only calls
+ *              that one host thread makes on one stream may share it: calls of two threads may be enqueued
+ *              kernel by kernel in turn, even on one stream
  */
 BOLT_API int64_t bolt_kv_attention_workspace(const int64_t* q_shape, const int64_t* cache_shape);
 BOLT_API int bolt_kv_attention(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,

@@ -9,6 +9,7 @@ reference's message (the reference returns ORT_FAIL with the same text).
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -339,18 +340,21 @@ def _kv_rows(op, t, what):
     return shape_arg(shape)[0], shape_arg((seq if S > 1 else 0, row if R > 1 else 0))[0]
 
 
-_WORKSPACES: dict = {}
+_WORKSPACES = threading.local()
 
 
 def _kv_workspace(like, nbytes):
-    """Scratch memory of a call.  Calls of one stream follow one another, so they share a tensor (an
-    allocation costs two microseconds); a captured call, which may be replayed on any stream, has its own."""
+    """Scratch memory of a call, whose two kernels meet in it.  The calls that one host thread makes on one
+    stream follow one another, kernel by kernel, so they share a tensor (an allocation costs two microseconds).
+    Two threads may enqueue their kernels on one stream in turn, so each has its own; and so has a captured
+    call, which may be replayed on any stream."""
     if torch.cuda.is_current_stream_capturing():
         return like.new_empty((nbytes,))
+    held = _WORKSPACES.__dict__  # this thread's
     key = like.device.index, _stream(like)
-    ws = _WORKSPACES.get(key)
+    ws = held.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _WORKSPACES[key] = like.new_empty((nbytes,))
+        ws = held[key] = like.new_empty((nbytes,))
     return ws
 
 
