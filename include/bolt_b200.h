@@ -304,7 +304,8 @@ BOLT_API int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const
  * the positions j <= p and, with window > 0, only those with j > p - window or j < sinks.
  *   o    bf16 [S, R, Hq, D] = sum_j softmax_j(scale * q . k_j) v_j
  *   lse  f32  [S, R, Hq]    = log sum_j exp(scale * q . k_j)
- * Rows that do not exist give o = 0 and lse = -inf.
+ * Rows that do not exist give o = 0 and lse = -inf.  A row whose q holds an infinity or NaN, or that sees a
+ * logit of NaN (a K scale of NaN), gives NaN for o and lse; other rows are not touched by it.
  *   workspace  scratch device memory of bolt_kv_attention_workspace(q_shape, cache_shape) bytes on the
  *              current device (-1: bad shapes), 16-byte aligned; nothing has to be in it, and nothing
  *              of it is read by a later call.  The call enqueues two kernels that meet in it, so only calls
@@ -322,7 +323,8 @@ BOLT_API int bolt_kv_attention(const void* q, const int64_t* q_shape, const int6
  * KvScore: score f32 [S, heads, score_width] (score_width >= width * T) += each position's attention
  * weight, sum over the rows and over the query heads of its cache head of exp(scale * q . k_j - lse),
  * with q, the mask and lse as bolt_kv_attention took and gave them.  In place; positions that no row
- * sees keep their sums.  The result does not depend on scheduling.
+ * sees keep their sums; those that a row of NaN (bolt_kv_attention) sees become NaN.  The result does not
+ * depend on scheduling.
  */
 BOLT_API int bolt_kv_score(const void* q, const int64_t* q_shape, const int64_t* q_strides, const void* k_cache,
                            const int64_t* cache_shape, const void* k_scale, const void* table,

@@ -1,7 +1,8 @@
 // KvAttention over the paged 8-bit key/value cache (layout in kv.h).
 //
 //   l_j = scale * q . k_j over the positions j that the row sees;  lse = log sum_j exp(l_j)
-//   o = sum_j exp(l_j - lse) v_j (bf16) and lse (f32); a row that sees nothing gives 0 and -inf
+//   o = sum_j exp(l_j - lse) v_j (bf16) and lse (f32); a row that sees nothing gives 0 and -inf,
+//   one with a logit of NaN gives NaN
 //
 // One pass with the running maximum and sum of a softmax (kv_mma.cuh has the operands).  The rows of a
 // sequence that read one kv head -- R rows times G query heads -- are the M axis of the products, so
@@ -343,8 +344,12 @@ __global__ void __launch_bounds__(kThreads, CPS) kv_attention_kernel(
         l += __shfl_xor_sync(0xffffffffu, l, 4);
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
-        // the maximum's place takes the reference; none for rows that do not exist
-        m_ref[r][e] = pos[r][e] < 0 || m_top[r][e] == -INFINITY ? -INFINITY : m_ref[r][e] + kWeightLog;
+        // the maximum's place takes the reference; none for rows that do not exist.  NaN among the logits passed
+        // by the maximum and is in the sum, also of a row that has no reference.
+        m_ref[r][e] = pos[r][e] < 0                  ? -INFINITY
+                      : l != l                       ? NAN
+                      : m_top[r][e] == -INFINITY     ? -INFINITY
+                                                     : m_ref[r][e] + kWeightLog;
         if (g == 0) {
           const int row = r * 8 + 2 * q4 + e;
           sm[warp * L::kRows + row] = m_ref[r][e];
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(co
     }
   }
   if (!live) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t out = (static_cast<int64_t>(t.s) * p.rows.R + m / p.G) * p.Hq + t.h * p.G + m % p.G;
   uint32_t u[E / 2];
 #pragma unroll
@@ -443,7 +448,7 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(co
     *reinterpret_cast<uint2*>(p.o + out * D + lane * E) = make_uint2(u[0], u[1]);
   else
     *reinterpret_cast<uint32_t*>(p.o + out * D + lane * E) = u[0];
-  if (lane == 0) p.lse[out] = l > 0.f ? (top - kWeightLog + log2f(l)) * kLn2 : -INFINITY;
+  if (lane == 0) p.lse[out] = l == 0.f ? -INFINITY : (top - kWeightLog + log2f(l)) * kLn2;
 }
 
 // The tiling for M = R * G rows a kv head.  Up to 16 rows: tiles of 8 or 16 rows whose steps four warps share,

@@ -493,7 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
       }
       if (ok && n_tiles > 0) ok = wait(o_full(i), (i ? done1 : done0) + n_tiles - 1);
       tc_after();
-      ref = pos < 0 || top_off == -INFINITY || !ok ? -INFINITY : ref + kWeightLog;
+      // NaN among the logits passed by the maximum and is in the sum, also of a row that has no reference
+      ref = pos < 0 || !ok ? -INFINITY : l != l ? NAN : top_off == -INFINITY ? -INFINITY : ref + kWeightLog;
       sm[i * kRows + row] = ref;
       sl[i * kRows + row] = l;
     }

@@ -343,24 +343,24 @@ __device__ __forceinline__ void kv_fetch_q(const KvAttnParams& p, const KvSeq& s
 
 // ... and as B operands: for the contraction step 4 i + y the lane holds the values 64 i + 16 c + 4 y .. + 3
 // of row g -- the order in which a lane's 16 loaded K codes lie.  logit / log 2 = (sum of products) * f - t,
-// times the page's K scale; f and t are those of row g.
+// times the page's K scale; f and t are those of row g.  A row with a value that is not finite has a t of NaN,
+// so that all its logits are.
 template <int D, int FMT>
 __device__ __forceinline__ void kv_make_q(const KvAttnParams& p, const uint4 (&raw)[D / 64][2], uint2 (&q)[D / 16],
                                           float& f, float& t) {
-  float amax = 0.f;
+  uint32_t amax = 0;  // the largest magnitude's bits: those of infinities and NaN are the largest of all
 #pragma unroll
   for (int i = 0; i < D / 64; ++i)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const uint32_t w[4] = {raw[i][k].x, raw[i][k].y, raw[i][k].z, raw[i][k].w};
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xFFFF0000u))));
+      for (int x = 0; x < 4; ++x) amax = max(amax, max((w[x] << 16) & 0x7FFF0000u, w[x] & 0x7FFF0000u));
     }
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   // 2^-x brings the largest value into [1, 2); the power is kept within fp32's normal range
-  const int x = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 120);
+  const int x = min(max(static_cast<int>(amax >> 23) - 127, -100), 120);
   const float down = __uint_as_float(static_cast<uint32_t>(127 - x) << 23);
   float sum = 0.f;
 #pragma unroll
@@ -386,6 +386,7 @@ __device__ __forceinline__ void kv_make_q(const KvAttnParams& p, const uint4 (&r
     t = 128.f * f * sum;
     f *= 0x1p24f;
   }
+  if (amax >= 0x7F800000u) t = NAN;
 }
 
 // The same with sums that start at 0.

@@ -66,7 +66,7 @@ __device__ __forceinline__ void kv_finish(const KvAttnParams& p, const Work& w, 
       }
     }
     if (item) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       const unsigned r = m / G;
       const int64_t out = (static_cast<int64_t>(seg.s) * p.rows.R + r) * p.Hq + seg.h * G + (m - r * G);
       uint4 u;
@@ -79,7 +79,7 @@ __device__ __forceinline__ void kv_finish(const KvAttnParams& p, const Work& w, 
       u.z = *reinterpret_cast<uint32_t*>(&y2);
       u.w = *reinterpret_cast<uint32_t*>(&y3);
       *reinterpret_cast<uint4*>(p.o + out * D + 4 * f) = u;
-      if (f == 0) p.lse[out] = l > 0.f ? (top - kWeightLog + log2f(l)) * kLn2 : -INFINITY;
+      if (f == 0) p.lse[out] = l == 0.f ? -INFINITY : (top - kWeightLog + log2f(l)) * kLn2;
     } else {
       float4* to = reinterpret_cast<float4*>(w.part + (static_cast<int64_t>(slot) * ROWS + row) * D) + f;
       to[0] = v[0];

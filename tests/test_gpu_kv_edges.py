@@ -7,14 +7,28 @@ and it stays below the term of 2^-18 for the numbers of positions of these cases
 """
 import threading
 
-import torch
+import numpy as np
 import pytest
+import torch
 
+import oracle as O
 import test_gpu_kv as kv
 from nemotron_ops_b200 import ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+
+ROWS = [(1, 1), (1, 8), (2, 8), (1, 17), (3, 8), (65, 2)]  # R, G: tiles of 8, of 16, and the tensor-memory kernel
+
+
+def _check(o, lse, ref, D, bad):
+    """The rows of `bad` [S, R, Hq] are NaN throughout, the others right."""
+    o, lse = o.cpu().clone(), lse.cpu().clone()
+    bad = torch.from_numpy(bad)
+    assert bool(o[bad].isnan().all()) and bool(lse[bad].isnan().all())
+    o[bad] = torch.from_numpy(ref["o"])[bad].to(o.dtype)
+    lse[bad] = torch.from_numpy(ref["lse"])[bad].to(lse.dtype)
+    kv._check_attention(o, lse, ref, D)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -46,4 +60,60 @@ def test_host_threads_on_one_stream():
     for (o, lse), results in zip(want, got):
         assert len(results) == 200
         assert all(torch.equal(o, a) and torch.equal(lse, b) for a, b in results)
+    assert ops.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# values that are not finite
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("value", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R,G", ROWS)
+def test_a_query_row_that_is_not_finite(R, G, D, fmt, value):
+    # its o and lse are NaN, its neighbours' are as they were; rows that do not exist stay empty
+    lens = [1500, 0, 90]
+    c = kv.Cache(lens, 2, D, 16, fmt, seed=201)
+    q = kv._rows(3, R, 2 * G, D, seed=202)
+    start = (c.lens - R).clamp(min=0)
+    if R > 1:
+        start[2] = c.lens[2] - 1  # one row of R
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, D ** -0.5, fmt=fmt)
+    dirty, bad = q.clone(), np.zeros(q.shape[:3], dtype=bool)
+    for s, r, i, d in ((0, R // 2, G, D - 1), (1, 0, 0, 3), (2, 0, G - 1, 0), (2, R - 1, G, 5)):
+        dirty[s, r, i, d] = float(value)
+        bad[s, r, i] = int(start[s]) + r < lens[s]
+    o, lse = kv._attention(c, dirty, start, D ** -0.5)
+    _check(o, lse, ref, D, bad)
+    # the weights of such a row are NaN where it looks; other heads and positions have theirs
+    width = c.width * 16
+    scale = D ** -0.5
+    score = ops.KvScore(dirty.to(DEV), c.k.to(DEV), c.ks.to(DEV), c.table.to(DEV), start.to(DEV), c.lens.to(DEV), lse,
+                        torch.ones(3, 2, width, device=DEV), scale, fmt=fmt).cpu()
+    clean = torch.from_numpy(ref["lse"]).float()
+    want, added = O.kv_score(q, c.k, c.ks, c.table, start, c.lens, clean, torch.ones(3, 2, width), scale, fmt=fmt)
+    nan = np.zeros(want.shape, dtype=bool)
+    for s, r, i in np.argwhere(bad):
+        nan[s, i // G, :int(start[s]) + r + 1] = True
+    assert np.array_equal(np.isnan(score.numpy()), nan)
+    dl = (2 * D + 16) * kv.U * ref["ql"].max() + 4 * kv.U * 30 + 2.0 ** -18
+    assert (np.abs(score.double().numpy() - want)[~nan] <= (2 * dl * added + 2 * kv.U * np.abs(want))[~nan]).all()
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R,G", [(4, 2), (8, 2), (20, 3)])
+def test_a_page_whose_k_scale_is_nan(R, G, D, fmt):
+    # rows that see one of its positions are NaN, those before it are not touched
+    n = 288 + R // 2  # the last page begins inside the call's rows
+    c = kv.Cache([n], 2, D, 16, fmt, seed=203)
+    q = kv._rows(1, R, 2 * G, D, seed=204)
+    start = c.lens - R
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, 0.1, fmt=fmt)
+    c.ks[c.table[0, 18].long(), 1] = float("nan")
+    bad = np.zeros(q.shape[:3], dtype=bool)
+    bad[0, R // 2:, G:] = True
+    o, lse = kv._attention(c, q, start, 0.1)
+    _check(o, lse, ref, D, bad)
     assert ops.device_status() == 0
