@@ -235,8 +235,11 @@ struct KvPages {
   int page;
   float ks, vs;
   __device__ __forceinline__ void load_page(const KvCache& c, int s, bool live, int base) {
+    // -1 stands for no page; an entry that is negative is one past every cache's last
     page = -1;
-    if (live) page = c.table[static_cast<int64_t>(s) * c.width + (base >> c.tshift)] & 0x7fffffff;
+    if (live)
+      page = static_cast<int>(
+          min(static_cast<unsigned>(c.table[static_cast<int64_t>(s) * c.width + (base >> c.tshift)]), 0x7fffffffu));
   }
   __device__ __forceinline__ void check_page(const KvCache& c) {
     if (page >= c.pages) {

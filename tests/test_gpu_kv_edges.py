@@ -117,3 +117,40 @@ def test_a_page_whose_k_scale_is_nan(R, G, D, fmt):
     o, lse = kv._attention(c, q, start, 0.1)
     _check(o, lse, ref, D, bad)
     assert ops.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# page tables
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("entry", [-1, -12345, -2 ** 31, -2 ** 31 + 1, 2 ** 31 - 1])
+@pytest.mark.parametrize("R,G", [(1, 2), (1, 16), (1, 20)])
+def test_page_numbers_that_the_cache_does_not_have(R, G, entry):
+    # the page's positions are left out, whatever the entry's low bits name, and the status word says so
+    c = kv.Cache([40], 1, 64, 16, 0, seed=211)
+    q = kv._rows(1, 1, G, 64, seed=212)
+    start = c.lens - 1
+    table = c.table.clone()
+    table[0, 1] = entry
+    dev = c.dev()
+    args = table.to(DEV), start.to(DEV), c.lens.to(DEV)
+    ops.device_status()
+    o, lse = ops.KvAttention(q.to(DEV), *dev, *args, 0.1)
+    assert ops.device_status() == 1 << 8
+    idx = np.r_[0:16, 32:40]
+    k, v = (O.kv_tokens(x, s, c.table, 0, idx, 0)[:, 0] for x, s in ((c.k, c.ks), (c.v, c.vs)))
+    x = q[0, 0].double().numpy() @ k.T * 0.1
+    z = np.log(np.exp(x).sum(1))
+    p = np.exp(x - z[:, None])
+    ref = dict(o=(p @ v)[None, None], lse=z[None, None], av=(p @ np.abs(v))[None, None],
+               ql=(np.abs(q[0, 0].double().numpy()) @ np.abs(k).T * 0.1).max(1)[None, None])
+    kv._check_attention(o, lse, ref, 64)
+    score = ops.KvScore(q.to(DEV), dev[0], dev[2], *args, lse, torch.ones(1, 1, 48, device=DEV), 0.1).cpu()
+    assert ops.device_status() == 1 << 8
+    want = np.ones(48)
+    want[idx] += p.sum(0)
+    dl = (2 * 64 + 16) * kv.U * ref["ql"].max() + 4 * kv.U * np.abs(z).max() + 2.0 ** -18
+    assert (np.abs(score[0, 0].double().numpy() - want) <= 2 * dl * want + 2 * kv.U * want).all()
+    # the other ops leave it out too
+    rk, _ = ops.KvRead(*dev, args[0], torch.zeros_like(start).to(DEV), args[2], 40)
+    assert ops.device_status() == 1 << 8
+    assert not rk[0, 16:32].any() and bool(rk[0, :16].any())
