@@ -513,6 +513,8 @@ KvAttnParams kv_attn(const std::string& op, const KvCache& c, const void* q, con
     throw std::invalid_argument(op + ": query heads must be a multiple of the cache's heads");
   p.rows = KvRows{static_cast<const int*>(start), static_cast<const int*>(lens),
                   kv_row_shape(op, c, q_shape, q_strides, Hq)};
+  if (p.rows.R * (Hq / c.heads) > INT32_MAX)
+    throw std::invalid_argument(op + ": rows times query heads of a cache head must be fewer than 2^31");
   if (window < 0 || sinks < 0) throw std::invalid_argument(op + ": window and sinks must not be negative");
   const int64_t most = int64_t(1) << 30;  // no position is larger
   p.mask = KvMask{static_cast<int>(std::min(window, most)), static_cast<int>(std::min(sinks, most))};

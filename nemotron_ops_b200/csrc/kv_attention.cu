@@ -502,7 +502,7 @@ cudaError_t launch_kv_attention(const KvAttnParams& params, void* workspace, con
   const int64_t M = static_cast<int64_t>(p.rows.R) * p.G;
   const Plan t = plan_of(M, p.c.D);
   const int64_t row_blocks = (M + t.rows - 1) / t.rows, items = p.c.S * row_blocks * p.c.heads;
-  if (M > 0x7fffffff || p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (p.c.S * row_blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
   p.few_steps = items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16 + kMostItemCost) <= 0x7fffffff;
   // no more blocks than the longest sequences could fill
   const int64_t steps = std::max<int64_t>(items * (((static_cast<int64_t>(p.c.width) << p.c.tshift) + 15) / 16), 1);

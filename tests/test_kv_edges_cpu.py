@@ -1,9 +1,10 @@
 """CPU checks of the host side of the key/value cache ops where calls meet: threads, devices, sizes."""
+import ctypes
 import threading
 
 import torch
 
-from nemotron_ops_b200 import ops
+from nemotron_ops_b200 import _lib, ops
 
 
 def test_host_threads_do_not_share_scratch_memory(monkeypatch):
@@ -30,3 +31,20 @@ def test_host_threads_do_not_share_scratch_memory(monkeypatch):
     # calls of one thread and one stream follow one another and have one buffer, which grows
     one = ops._kv_workspace(like, 100)
     assert one.numel() == 100 and ops._kv_workspace(like, 10) is one
+
+
+def test_more_rows_than_32_bits_count():
+    # rows x query heads of a cache head: the kernels count them in 32 bits
+    def sh(*dims):
+        return _lib.shape_arg(dims)[0]
+
+    lib, some = _lib.lib(), ctypes.c_void_p(4096)  # aligned; never dereferenced on the host
+    cache, table, strides = sh(5, 2, 16, 128), sh(3, 4), sh(1024, 0)
+    for rows, heads in ((1 << 29, 8), (1 << 29, 16), (65536, 2 << 15), (1 << 20, 2 << 12)):
+        q = sh(3, rows, heads, 128)
+        assert lib.bolt_kv_score(some, q, strides, some, cache, some, some, table, some, some, some, 0.1, 0, 0, 0, some,
+                                 64, None) == 1
+        assert "KvScore: rows times query heads of a cache head must be fewer than 2^31" in _lib.last_error()
+        assert lib.bolt_kv_attention(some, q, strides, some, cache, some, some, some, some, table, some, some, 0.1, 0, 0,
+                                     0, some, some, some, 1 << 40, None) == 1
+        assert "KvAttention: rows times query heads of a cache head must be fewer than 2^31" in _lib.last_error()
