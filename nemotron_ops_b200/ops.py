@@ -322,16 +322,22 @@ def _kv_args(op, k_cache, v_cache, k_scale, v_scale, table, lens, start=None):
         raise RuntimeError(f"{op}: page table must be [sequences, pages of a sequence]")
     if lens.shape != tables[:1] or start.shape != tables[:1]:
         raise RuntimeError(f"{op}: starts and lengths must be [sequences]")
+    # the library launches on the current device, which has to have every tensor
+    if not (torch._C._cuda_getDevice() == k_cache.get_device() == v_cache.get_device() == k_scale.get_device()
+            == v_scale.get_device() == table.get_device() == lens.get_device() == start.get_device()):
+        raise RuntimeError(f"{op}: tensors must be on the current device")
     return shape_arg(shape)[0], shape_arg(tables)[0]
 
 
-def _kv_rows(op, t, what):
+def _kv_rows(op, t, what, cache):
     """Shape argument of rows [S, R, heads, D] whose last two axes are dense, and that of the strides of the
-    sequence and row axes."""
+    sequence and row axes.  They are on the cache's device."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise RuntimeError("bolt ops take CUDA tensors (there is no CPU implementation)")
     if t.dtype != torch.bfloat16 or t.dim() != 4:
         raise RuntimeError(f"{op}: {what} must be bf16 [sequences, rows, heads, head size]")
+    if t.get_device() != cache.get_device():
+        raise RuntimeError(f"{op}: tensors must be on the current device")
     seq, row, head, one = t.stride()
     S, R, H, D = shape = t.shape
     if (one != 1 and D != 1) or (head != D and H != 1):
@@ -362,8 +368,8 @@ def KvAppend(k, v, k_cache, v_cache, k_scale, v_scale, table, start, lens, fmt: 
     """Quantise the rows k, v bf16 [S, R, heads, D] into their pages, in place: a page's scale grows to
     max|x| / 127 (KV_INT8) or / 448 (KV_E4M3) where a row needs it, and its older codes with it."""
     cs, ts = _kv_args("KvAppend", k_cache, v_cache, k_scale, v_scale, table, lens, start)
-    shape, ks = _kv_rows("KvAppend", k, "k")
-    _, vs = _kv_rows("KvAppend", v, "v")
+    shape, ks = _kv_rows("KvAppend", k, "k", k_cache)
+    _, vs = _kv_rows("KvAppend", v, "v", k_cache)
     if v.shape != k.shape:
         raise RuntimeError("KvAppend: k and v must have the same shape")
     _check(lib().bolt_kv_append(_ptr(k), shape, ks, _ptr(v), vs, _ptr(k_cache), cs, _ptr(v_cache), _ptr(k_scale),
@@ -386,7 +392,7 @@ def KvAttention(q, k_cache, v_cache, k_scale, v_scale, table, start, lens, scale
     """Returns (o bf16 [S, R, Hq, D], lse f32 [S, R, Hq]) of the rows q bf16 [S, R, Hq, D]: the row at
     position p sees the positions j <= p and, with a window, only j > p - window or j < sinks."""
     cs, ts = _kv_args("KvAttention", k_cache, v_cache, k_scale, v_scale, table, lens, start)
-    shape, st = _kv_rows("KvAttention", q, "q")
+    shape, st = _kv_rows("KvAttention", q, "q", k_cache)
     # new_empty of a tensor of the type: half the host time of torch.empty with a type and a device
     o = q.new_empty(q.shape)
     lse = k_scale.new_empty(q.shape[:3])
@@ -403,7 +409,9 @@ def KvScore(q, k_cache, k_scale, table, start, lens, lse, score, scale: float, w
     returns it); q, the mask and lse as in the KvAttention call whose weights are taken."""
     cs, ts = _kv_args("KvScore", k_cache, k_cache, k_scale, k_scale, table, lens, start)
     _need(lse, score)
-    shape, st = _kv_rows("KvScore", q, "q")
+    if not lse.get_device() == score.get_device() == k_cache.get_device():
+        raise RuntimeError("KvScore: tensors must be on the current device")
+    shape, st = _kv_rows("KvScore", q, "q", k_cache)
     if lse.dtype != torch.float32 or lse.shape != q.shape[:3]:
         raise RuntimeError("KvScore: lse must be f32 [sequences, rows, query heads]")
     if score.dtype != torch.float32 or score.dim() != 3 or score.shape[:2] != (table.shape[0], k_cache.shape[1]):
@@ -421,6 +429,8 @@ def KvEvict(k_cache, v_cache, k_scale, v_scale, table, lens, score, new_table, k
     (kept i32 [S, heads, keep], new_lens i32 [S], new_score f32 [S, heads, keep])."""
     cs, ts = _kv_args("KvEvict", k_cache, v_cache, k_scale, v_scale, table, lens)
     _need(score, new_table)
+    if not score.get_device() == new_table.get_device() == k_cache.get_device():
+        raise RuntimeError("KvEvict: tensors must be on the current device")
     S, heads = table.shape[0], k_cache.shape[1]
     if new_table.dtype != torch.int32 or new_table.dim() != 2 or new_table.shape[0] != S:
         raise RuntimeError("KvEvict: the new page table must be i32 [sequences, pages of a sequence]")
