@@ -268,7 +268,7 @@ BOLT_API int bolt_mamba_verify(const void* proj, const int64_t* proj_shape, int 
  *                                                page table[s][j / T]; entries past a sequence's end are not read
  *   start, lens       i32 [S]                    row r of a call is position start[s] + r and exists while that
  *                                                is below lens[s] (the length with the call's rows); a sequence
- *                                                may be empty
+ *                                                may be empty, and a table without columns (width 0) holds empty ones alone
  *   fmt               0: value = scale * (code - 128), codes 1..255;  1: value = scale * e4m3(code)
  * Rows (q, k, v) are bf16 [S, R, heads, D] with dense head and value axes; the sequence and row
  * strides (elements, multiples of 8) are given, so parts of a fused projection can be passed as they

@@ -501,6 +501,9 @@ void kv_pointers(const std::string& op, std::initializer_list<const void*> ps) {
     if (p == nullptr) throw std::invalid_argument(op + ": null buffer");
 }
 
+// The page table, or (not dereferenced) `any` for one without columns, which needs no memory.
+const void* kv_table(const KvCache& c, const void* any) { return c.width > 0 ? c.table : any; }
+
 // The arguments that KvAttention and KvScore share.
 KvAttnParams kv_attn(const std::string& op, const KvCache& c, const void* q, const int64_t* q_shape,
                      const int64_t* q_strides, const void* start, const void* lens, float scale, int64_t window,
@@ -555,7 +558,7 @@ int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const void* v_
     const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
     require(rows >= 0 && rows <= (int64_t(1) << 29), "KvRead: bad row count");
     if (c.S == 0 || rows == 0) return;
-    kv_pointers(op, {k_cache, v_cache, k_scale, v_scale, table, start, lens, k, v});
+    kv_pointers(op, {k_cache, v_cache, k_scale, v_scale, kv_table(c, lens), start, lens, k, v});
     require_aligned({k, v, k_cache, v_cache}, op);
     check_launch(launch_kv_read(c, KvRows{static_cast<const int*>(start), static_cast<const int*>(lens),
                                           static_cast<int>(rows)},
@@ -584,7 +587,7 @@ int bolt_kv_attention(const void* q, const int64_t* q_shape, const int64_t* q_st
     const KvCache c = kv_cache(op, k_cache, cache_shape, v_cache, k_scale, v_scale, table, table_shape, fmt);
     KvAttnParams p = kv_attn(op, c, q, q_shape, q_strides, start, lens, scale, window, sinks);
     if (c.S == 0 || p.rows.R == 0) return;
-    kv_pointers(op, {q, k_cache, v_cache, k_scale, v_scale, table, start, lens, o, lse, workspace});
+    kv_pointers(op, {q, k_cache, v_cache, k_scale, v_scale, kv_table(c, lens), start, lens, o, lse, workspace});
     require_aligned({q, k_cache, v_cache, o, workspace}, op);
     p.o = static_cast<bf16*>(o);
     p.lse = static_cast<float*>(lse);
@@ -627,7 +630,8 @@ int bolt_kv_evict(void* k_cache, const int64_t* cache_shape, void* v_cache, void
     require(new_width * c.T >= keep && new_width <= INT32_MAX, "KvEvict: the new page table must hold keep positions");
     require(score_width >= static_cast<int64_t>(c.width) * c.T, "KvEvict: score must cover the page table");
     if (c.S == 0) return;
-    kv_pointers(op, {k_cache, v_cache, k_scale, v_scale, table, lens, score, new_table, kept, new_lens, new_score});
+    kv_pointers(op, {k_cache, v_cache, k_scale, v_scale, kv_table(c, lens), lens, score_width > 0 ? score : lens, new_table,
+                     kept, new_lens, new_score});
     require_aligned({k_cache, v_cache}, op);
     KvEvictParams p{};
     p.c = c;

@@ -154,3 +154,29 @@ def test_page_numbers_that_the_cache_does_not_have(R, G, entry):
     rk, _ = ops.KvRead(*dev, args[0], torch.zeros_like(start).to(DEV), args[2], 40)
     assert ops.device_status() == 1 << 8
     assert not rk[0, 16:32].any() and bool(rk[0, :16].any())
+
+
+@pytest.mark.parametrize("R,G", [(1, 4), (2, 8), (9, 4)])
+def test_tables_of_no_pages(R, G):
+    # sequences that hold nothing and a table without columns: nothing to see, nothing to keep
+    c = kv.Cache([16, 16], 2, 64, 16, 0, seed=213)
+    dev = c.dev()
+    table = torch.zeros(2, 0, dtype=torch.int32, device=DEV)
+    zero = torch.zeros(2, dtype=torch.int32, device=DEV)
+    q = kv._rows(2, R, 2 * G, 64, seed=214).to(DEV)
+    o, lse = ops.KvAttention(q, *dev, table, zero, zero, 0.1)
+    assert not o.any() and bool(torch.isneginf(lse).all())
+    k, v = ops.KvRead(*dev, table, zero, zero, 3)
+    assert k.shape == (2, 3, 2, 64) and not k.any() and not v.any()
+    score = torch.zeros(2, 2, 0, device=DEV)
+    assert ops.KvScore(q, dev[0], dev[2], table, zero, zero, lse, score, 0.1) is score
+    new = torch.tensor([[0], [1]], dtype=torch.int32, device=DEV)
+    kept, lens, sums = ops.KvEvict(*dev, table, zero, score, new, 5)
+    assert bool((kept == -1).all()) and not lens.any() and not sums.any()
+    ops.KvAppend(q[:, :, :2], q[:, :, :2], *dev, table, zero, zero)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(dev, c.host()))
+    assert ops.device_status() == 0
+    # a length that such a table cannot hold is left out
+    o, lse = ops.KvAttention(q, *dev, table, zero, zero + 1, 0.1)
+    assert ops.device_status() == 1 << 7
+    assert not o.any() and bool(torch.isneginf(lse).all())
