@@ -6,8 +6,9 @@
 // positions (for logits) or the value axis (for outputs) as the 16 and the query rows as the 8: a
 // sequence's rows that share a head are few, and tiles of 8 leave the least of the unit idle.  fp16
 // holds every int8 and e4m3 value exactly, and a permutation of the contraction index, applied to both
-// operands, lets every lane load 16 consecutive bytes.  Query rows are scaled by a power of two into
-// fp16's range (their 8 significant bits fit) and the power goes into the row's logit factor.
+// operands, lets every lane load 16 consecutive bytes.  Query rows are scaled by a power of two to the top of
+// fp16's range and the power goes into the row's logit factor: a value's 8 significant bits fit down to 2^-31 of the
+// row's largest, and smaller ones err by at most 2^-39 of it (of 2^-112, if that is more).
 #pragma once
 
 #include "kv.cuh"
@@ -362,8 +363,8 @@ __device__ __forceinline__ void kv_make_q(const KvAttnParams& p, const uint4 (&r
     }
   amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  // 2^-x brings the largest value into [1, 2); the power is kept within fp32's normal range
-  const int x = min(max(static_cast<int>(amax >> 23) - 127, -100), 120);
+  // 2^-x brings the largest value into [2^14, 2^15); the power is kept within fp32's normal range
+  const int x = max(static_cast<int>(amax >> 23) - 127 - 14, -126);
   const float down = __uint_as_float(static_cast<uint32_t>(127 - x) << 23);
   float sum = 0.f;
 #pragma unroll

@@ -180,3 +180,22 @@ def test_tables_of_no_pages(R, G):
     o, lse = ops.KvAttention(q, *dev, table, zero, zero + 1, 0.1)
     assert ops.device_status() == 1 << 7
     assert not o.any() and bool(torch.isneginf(lse).all())
+
+
+# ---------------------------------------------------------------------------------------------
+# precision
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("small", [2.0 ** -16, 2.0 ** -20, 2.0 ** -22])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R,G", [(1, 2), (2, 8), (3, 8)])
+def test_query_values_far_below_the_rows_largest(R, G, D, small):
+    # the largest meets keys of 0 and the others decide
+    c = kv.Cache([200], 2, D, 16, 1, seed=221)
+    c.k[..., 7] = 0
+    q = kv._rows(1, R, 2 * G, D, seed=222).float() * small
+    q[..., 7] = 1.0
+    q = q.bfloat16()
+    start = c.lens - R
+    scale = D ** -0.5 / small
+    o, lse = kv._attention(c, q, start, scale)
+    kv._check_attention(o, lse, O.kv_attention(q, *c.host(), c.table, start, c.lens, scale, fmt=1), D)
