@@ -305,7 +305,8 @@ BOLT_API int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const
  *   o    bf16 [S, R, Hq, D] = sum_j softmax_j(scale * q . k_j) v_j
  *   lse  f32  [S, R, Hq]    = log sum_j exp(scale * q . k_j)
  * Rows that do not exist give o = 0 and lse = -inf.  A row whose q holds an infinity or NaN, or that sees a
- * logit of NaN (a K scale of NaN), gives NaN for o and lse; other rows are not touched by it.
+ * logit of NaN (a K scale of NaN) or a page whose V scale is not finite, gives NaN for o and lse; other rows are
+ * not touched by it.
  *   workspace  scratch device memory of bolt_kv_attention_workspace(q_shape, cache_shape) bytes on the
  *              current device (-1: bad shapes), 16-byte aligned; nothing has to be in it, and nothing
  *              of it is read by a later call.  The call enqueues two kernels that meet in it, so only calls

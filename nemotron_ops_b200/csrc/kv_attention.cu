@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, CPS) kv_attention_kernel(
       else if (j0 + 15 <= span.first &&
                (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
         flags = kWhole;
-      const float vs = fmaxf(meta.vs, 0x1p-96f);
-      s_scale[k & 63] = make_float4(meta.ks, log2f(vs), 1.f / vs, __int_as_float(j0 | flags));
+      const float2 vs = kv_v_scale(meta.vs);
+      s_scale[k & 63] = make_float4(meta.ks, vs.x, vs.y, __int_as_float(j0 | flags));
     };
     const auto fetch = [&](int k) {  // step k into its place in the ring
       __syncwarp();  // which no lane reads any more

@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
         flags = kDead;
       else if (j0 + 15 <= span.first && (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
         flags = kWhole;
-      const float vs = fmaxf(meta.vs, 0x1p-96f);
-      s_meta[t % kMetaTiles * kSteps + cw] = make_float4(meta.ks, log2f(vs), 1.f / vs, __int_as_float(j0 | flags));
+      const float2 vs = kv_v_scale(meta.vs);
+      s_meta[t % kMetaTiles * kSteps + cw] = make_float4(meta.ks, vs.x, vs.y, __int_as_float(j0 | flags));
       reinterpret_cast<int*>(smem + L::kLine)[cw * kMetaTiles + t % kMetaTiles] =
           meta.page < 0 ? -1 : ((meta.page * c.heads + s_seg.h) * c.T + (j0 & (c.T - 1))) / (128 / D);
     };

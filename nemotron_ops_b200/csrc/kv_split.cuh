@@ -9,6 +9,14 @@ namespace bolt {
 // largest at least 2^kWeightLog when its reference was last raised.
 constexpr float kWeightLog = 8.f, kWeightTop = 15.f;
 
+// A page's V scale is part of its positions' weights: its logarithm, to add to their logits, and the factor that
+// takes it off again in the sums.  A scale of 0 counts as 2^-96 (its values are far below any others'); one that is
+// not finite makes the logits NaN and leaves the factor finite, for the rows that do not see the page.
+__device__ __forceinline__ float2 kv_v_scale(float scale) {
+  const float s = fmaxf(scale, 0x1p-96f);
+  return make_float2(scale < INFINITY ? log2f(s) : NAN, 1.f / s);
+}
+
 struct Split {  // segments of one item: the first in block `block`'s slot 2 block + 1, the i-th in 2 (block + i)
   int s, mb, h, block, parts;
 };

@@ -119,6 +119,22 @@ def test_a_page_whose_k_scale_is_nan(R, G, D, fmt):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("value", ["nan", "inf"])
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("R,G", [(4, 2), (8, 2), (20, 3)])
+def test_a_page_whose_v_scale_is_not_finite(R, G, fmt, value):
+    n = 288 + R // 2
+    c = kv.Cache([n], 2, 128, 16, fmt, seed=205)
+    q = kv._rows(1, R, 2 * G, 128, seed=206)
+    start = c.lens - R
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, 0.1, fmt=fmt)
+    c.vs[c.table[0, 18].long(), 1] = float(value)
+    bad = np.zeros(q.shape[:3], dtype=bool)
+    bad[0, R // 2:, G:] = True
+    o, lse = kv._attention(c, q, start, 0.1)
+    _check(o, lse, ref, 128, bad)
+
+
 # ---------------------------------------------------------------------------------------------
 # page tables
 # ---------------------------------------------------------------------------------------------
