@@ -215,3 +215,29 @@ def test_query_values_far_below_the_rows_largest(R, G, D, small):
     scale = D ** -0.5 / small
     o, lse = kv._attention(c, q, start, scale)
     kv._check_attention(o, lse, O.kv_attention(q, *c.host(), c.table, start, c.lens, scale, fmt=1), D)
+
+
+# ---------------------------------------------------------------------------------------------
+# sizes that take the branches off the common way
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,keep,sinks,recent,kind", [
+    (48 * 1024, 30000, 4, 100, "ties"),       # the most whose weights are held in shared memory
+    (48 * 1024 + 1, 30000, 4, 100, "ties"),   # ... and one more
+    (100003, 777, 0, 0, "even"),
+    (100003, 60001, 16, 30000, "special"),
+])
+def test_evict_of_sequences_longer_than_shared_memory(n, keep, sinks, recent, kind):
+    kv.test_evict_matches_the_definition([n, 300], keep, sinks, recent, 1, 64, 256, kind, 0)
+
+
+@pytest.mark.parametrize("S,R,Hq,Hkv,D,T,fmt,longest,window,sinks", [
+    # more than 32 (sequence, row block) pairs, but at most a quarter as many items as blocks
+    (40, 1, 4, 1, 128, 32, 0, 5000, 0, 0),
+    (70, 2, 8, 1, 64, 16, 1, 4000, 0, 0),
+    (33, 2, 8, 1, 128, 16, 1, 3000, 500, 9),
+    (37, 3, 8, 1, 128, 64, 0, 3000, 0, 0),     # 24 rows a head
+    (34, 20, 1, 1, 64, 16, 0, 5000, 1000, 4),
+    (3, 1500, 1, 1, 64, 16, 0, 6000, 0, 0),    # 12 row blocks a sequence
+])
+def test_many_sequences_of_one_head(S, R, Hq, Hkv, D, T, fmt, longest, window, sinks):
+    kv.test_long_items(S, R, Hq, Hkv, D, T, fmt, longest, window, sinks)
