@@ -7,14 +7,14 @@
 // A page's scale never shrinks, so its older codes are rewritten only when a new value is larger
 // than all before it.  Infinities and NaN do not count towards the scale: they are stored as
 // +-Q * s' and 0, and leave the rest of the page as it is.
-#include "kv.cuh"
-
 //
 // Both are streams of HBM bytes (append 2 in, 1 out a value; read 1 in, 2 out).  KvAppend gives a block the
 // new rows of one (page, head), which it holds in registers between the maximum and the rounding, so each
 // value is read once.  2 sequences of 6,000 rows, 8 heads of 128 values, K and V: 38 us to write and read them
 // back.  KvAppend by itself takes 24, bound by the instructions of the rounding (2.7 issued a cycle; 29 us with a
 // division a value); KvRead goes at HBM's rate.  One row of each of 64 sequences: 10 us, latency.
+#include "kv.cuh"
+
 namespace bolt {
 
 namespace {
@@ -175,8 +175,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendParams 
   }
 }
 
-// Block y: a sequence.  A thread takes vectors of 16 values of a (row, head), kReadVecs of them.
-constexpr int kReadVecs = 1;
+// Block y: a sequence.  A thread takes 16 values of a (row, head), of K and of V.
 template <int FMT>
 __global__ void __launch_bounds__(kThreads, 8) kv_read_kernel(const KvCache c, const KvRows rows, bf16* k, bf16* v) {
   pdl_wait();
@@ -184,51 +183,40 @@ __global__ void __launch_bounds__(kThreads, 8) kv_read_kernel(const KvCache c, c
   const int s = blockIdx.y, shift = c.D == 128 ? 3 : 2;
   const KvSeq q = kv_seq(c, rows.start, rows.lens, s);
   const int64_t n = static_cast<int64_t>(rows.R) * c.heads << shift;  // vectors of the sequence
-  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (kThreads * kReadVecs) + threadIdx.x;
-  uint4 x[kReadVecs][2];
-  float sc[kReadVecs][2];
-#pragma unroll
-  for (int i = 0; i < kReadVecs; ++i) {
-    const int64_t at = i0 + i * kThreads;
-    x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
-    sc[i][0] = sc[i][1] = 0.f;
-    if (at >= n) break;
-    const int64_t rh = at >> shift;
-    const int r = rh <= 0x7fffffff ? static_cast<int>(static_cast<unsigned>(rh) / static_cast<unsigned>(c.heads))
-                                   : static_cast<int>(rh / c.heads);
-    const int h = static_cast<int>(rh - static_cast<int64_t>(r) * c.heads);
-    const int64_t pos = static_cast<int64_t>(q.start) + r;
-    if (pos >= q.len) continue;
-    const int page = kv_page(c.table, c.width, c.pages, s, static_cast<int>(pos >> c.tshift));
-    if (page < 0) continue;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (at >= n) return;
+  const int64_t rh = at >> shift;
+  const int r = rh <= 0x7fffffff ? static_cast<int>(static_cast<unsigned>(rh) / static_cast<unsigned>(c.heads))
+                                 : static_cast<int>(rh / c.heads);
+  const int h = static_cast<int>(rh - static_cast<int64_t>(r) * c.heads);
+  const int64_t pos = static_cast<int64_t>(q.start) + r;
+  uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  float sc[2] = {0.f, 0.f};  // also where there is nothing to read
+  const int page = pos < q.len ? kv_page(c.table, c.width, c.pages, s, static_cast<int>(pos >> c.tshift)) : -1;
+  if (page >= 0) {
     const int64_t unit = static_cast<int64_t>(page) * c.heads + h;
     const int64_t from = ((unit << c.tshift) + (pos & (c.T - 1))) * c.D + (at & ((1 << shift) - 1)) * 16;
-    x[i][0] = *reinterpret_cast<const uint4*>(c.k + from);
-    x[i][1] = *reinterpret_cast<const uint4*>(c.v + from);
-    sc[i][0] = c.ks[unit];
-    sc[i][1] = c.vs[unit];
+    x[0] = *reinterpret_cast<const uint4*>(c.k + from);
+    x[1] = *reinterpret_cast<const uint4*>(c.v + from);
+    sc[0] = c.ks[unit];
+    sc[1] = c.vs[unit];
   }
 #pragma unroll
-  for (int i = 0; i < kReadVecs; ++i) {
-    const int64_t at = i0 + i * kThreads;
-    if (at >= n) break;
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint32_t w[4] = {x[kv].x, x[kv].y, x[kv].z, x[kv].w};
+    uint32_t y[8];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      const uint32_t w[4] = {x[i][kv].x, x[i][kv].y, x[i][kv].z, x[i][kv].w};
-      uint32_t y[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float z[4];
-        kv_decode4<FMT>(w[e], z);
-        const __nv_bfloat162 a = __floats2bfloat162_rn(z[0] * sc[i][kv], z[1] * sc[i][kv]);
-        const __nv_bfloat162 b = __floats2bfloat162_rn(z[2] * sc[i][kv], z[3] * sc[i][kv]);
-        y[2 * e] = *reinterpret_cast<const uint32_t*>(&a);
-        y[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&b);
-      }
-      uint4* out = reinterpret_cast<uint4*>((kv ? v : k) + (static_cast<int64_t>(s) * n + at) * 16);
-      __stcs(out, make_uint4(y[0], y[1], y[2], y[3]));
-      __stcs(out + 1, make_uint4(y[4], y[5], y[6], y[7]));
+    for (int e = 0; e < 4; ++e) {
+      float z[4];
+      kv_decode4<FMT>(w[e], z);
+      const __nv_bfloat162 a = __floats2bfloat162_rn(z[0] * sc[kv], z[1] * sc[kv]);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(z[2] * sc[kv], z[3] * sc[kv]);
+      y[2 * e] = *reinterpret_cast<const uint32_t*>(&a);
+      y[2 * e + 1] = *reinterpret_cast<const uint32_t*>(&b);
     }
+    uint4* out = reinterpret_cast<uint4*>((kv ? v : k) + (static_cast<int64_t>(s) * n + at) * 16);
+    __stcs(out, make_uint4(y[0], y[1], y[2], y[3]));
+    __stcs(out + 1, make_uint4(y[4], y[5], y[6], y[7]));
   }
 }
 
@@ -258,7 +246,7 @@ cudaError_t launch_kv_append(const KvCache& c, const KvRows& rows, const bf16* k
 
 cudaError_t launch_kv_read(const KvCache& c, const KvRows& rows, bf16* k, bf16* v, const LaunchCfg& cfg) {
   const int64_t n = static_cast<int64_t>(rows.R) * c.heads * (c.D >> 4);
-  const int64_t grid = (n + kThreads * kReadVecs - 1) / (kThreads * kReadVecs);
+  const int64_t grid = (n + kThreads - 1) / kThreads;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
   return launch_kernel(c.fmt == kKvInt8 ? kv_read_kernel<kKvInt8> : kv_read_kernel<kKvE4m3>,
                        dim3(static_cast<unsigned>(grid), static_cast<unsigned>(c.S)), dim3(kThreads), 0, cfg, c, rows, k, v);
