@@ -307,6 +307,10 @@ BOLT_API int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const
  * Rows that do not exist give o = 0 and lse = -inf.  A row whose q holds an infinity or NaN, or that sees a
  * logit of NaN (a K scale of NaN) or a page whose V scale is not finite, gives NaN for o and lse; other rows are
  * not touched by it.
+ * Logits, sums and values are fp32.  A position's weight is rounded to fp16 (11 bits) once; where weight times V
+ * scale is below 2^-22 of the row's largest such product, it errs by at most 2^-33 of that instead, and below 2^-134
+ * it is left out of o and lse (a scale of 0 counts as 2^-96).  q's values keep their bits down to 2^-31 of the row's
+ * largest; an int8 logit errs by fp32 roundings of scale * sum|q_d| * 128 * s.
  *   workspace  scratch device memory of bolt_kv_attention_workspace(q_shape, cache_shape) bytes on the
  *              current device (-1: bad shapes), 16-byte aligned; nothing has to be in it, and nothing
  *              of it is read by a later call.  The call enqueues two kernels that meet in it, so only calls

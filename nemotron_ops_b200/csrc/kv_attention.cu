@@ -452,11 +452,23 @@ __global__ void __launch_bounds__(WPR > 8 ? WPR * 32 : 256) kv_combine_kernel(co
 }
 
 // The tiling for M = R * G rows a kv head.  Up to 16 rows: tiles of 8 or 16 rows whose steps four warps share,
-// several blocks an SM.  More: 128 rows, the tensor-memory kernel, one block an SM.  It costs the same for 17 rows
-// as for 128, the other the more the more rows it has.  Both sides, in us, heads of 128 values (tiles of 32 and
-// 64 rows for the first, which it had before): 32 sequences of 8,192 positions, 8 heads: 76 with 16 rows here,
-// 153 : 136 with 24, 158 : 137 with 32 and 244 : 144 with 64; 8 sequences of 16,384, 1 head: 30 : 31 with 32,
-// 45 : 32 with 64; one of 4,000: 17.5 : 17.9 with 32, 18.0 : 18.6 with 64.  Registers set the blocks an SM.
+// several blocks an SM.  More: 128 rows, the tensor-memory kernel, one block an SM.  It costs much the same for 17
+// rows as for 128, the other the more the more rows it has.  Both sides, in us, with tiles of 32 and 64 rows for the
+// first, which it had before ("window": 1,024 positions and 4 sinks of 48 sequences of up to 20,000):
+//   heads of 128 values           16 rows     24         32         48         64
+//     32 x 8,192 positions, 8 heads  76   154 : 137  159 : 137  239 : 141  244 : 144
+//     8 x 16,384, 2 heads            22              29 : 31    44 : 31    45 : 32
+//     window, 16 heads               75   155 : 151  159 : 154  232 : 161  234 : 165
+//     window, 4 heads                29    52 : 51    53 : 52    71 : 55    73 : 57
+//   heads of 64 values
+//     32 x 8,192 positions, 8 heads  61   111 : 121  114 : 123  171 : 124  173 : 126
+//     8 x 16,384, 2 heads            19              24 : 27    34 : 28    34 : 28
+//     window, 16 heads               61   113 : 134  115 : 135  173 : 139  172 : 141
+//     window, 4 heads                23    38 : 44    39 : 44    53 : 46    54 : 47
+// One rule for both head sizes: with 17 to 32 rows it costs heads of 64 values 7 to 19% (their weights' exponentials
+// are as many as those of 128 values, over half the bytes), and a window of 256 positions in 4 sequences, where
+// set-up is all, 10 to 20% for either; tiles of 32 rows for them alone would be a third form of this kernel.
+// Registers set the blocks an SM.
 struct Plan {
   int rows, round, per_sm;
 };

@@ -18,7 +18,7 @@
 // floor (128 x 128 a tile at 16 a cycle and SM are 1,024 cycles, the tile's two products 512), but the latency of
 // a stream's chain S -> weights -> O bounds it: about 4,000 cycles a tile with two streams, products and
 // exponentials a quarter of the time each.  Two sequences of 4,000 positions, 1,500 rows, 16 query heads on 4:
-// 182 us with the joining, 440 TFLOP/s; 8 sequences of up to 16,384, 128 rows a head, 2 heads: 34 us.
+// 184 us with the joining, 440 TFLOP/s; 8 sequences of up to 16,384, 128 rows a head, 2 heads: 34 us.
 #include <type_traits>
 
 #include "kv_split.cuh"

@@ -12,10 +12,10 @@
 // kSelKeys positions), the cut is found eleven bits at a time by histograms, and the kept positions are
 // written in order.  Then the codes move, one block per (sequence, head, 128 positions or one page of 256):
 // look-ups of positions, pages and scales serve K and V, and the copies are 16 bytes a thread.  32 sequences of
-// 4,096 positions cut to 1,000, 8 heads of 128 values: 20 us for the selection (passes over shared
-// memory) and 31 for the moves, which HBM bounds.  One of 20,000, cut to
-// 8,192, 2 heads: the selection takes most of 36 us, on two SMs; a split of it over more would need an exchange
-// of histograms in each pass.
+// 4,096 positions cut to 1,000, 8 heads of 128 values: 22 us for the selection (passes over shared memory) and 31
+// for the moves, 116 MB at 3.7 TB/s, which the instructions of the requantising bound (2.3 issued a cycle, the ALU
+// busy half the time).  One of 20,000, cut to 8,192, 2 heads: the selection takes 29 us, on two SMs, and the moves
+// 13, latency; a split of the selection over more SMs would need an exchange of histograms in each pass.
 #include "kv.cuh"
 
 namespace bolt {

@@ -19,8 +19,10 @@ constexpr int kWarps = 8;
 constexpr int kItemCost = 16;  // of an item's set-up, in steps (kv_attention.cu has the measurement)
 constexpr int kRowTiles = 16;  // tiles of 8 query rows in shared memory at a time
 // Steps that a warp takes at a time and steps of its ring.  Steps of 64 values are too short for one alone
-// (32 sequences of up to 8,192 positions, 8 heads: 54 us one at a time, 42 us two); two of 128 values leave one
-// block an SM (65,536 positions, 2 heads: 12 us one at a time, 18 us two).
+// (32 sequences of up to 8,192 positions, 8 heads, 16 rows a head: 47 us one at a time, with a ring of 3, 4 or 6, and
+// 41 us two; 4 rows a head 41 and 36; one sequence of 65,536, 2 heads, 9.9 and 9.3).  Two of 128 values spill, and
+// gain little (54 and 51 us for the batch, 28 and 28 for 8 sequences, 11.2 and 11.0 for one) with a ring of 4; one of
+// 6 leaves one block an SM (83, 43 and 18 us).
 template <int D>
 constexpr int kTogether = D == 64 ? 2 : 1;
 template <int D>
