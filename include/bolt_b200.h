@@ -305,8 +305,9 @@ BOLT_API int bolt_kv_read(const void* k_cache, const int64_t* cache_shape, const
  *   o    bf16 [S, R, Hq, D] = sum_j softmax_j(scale * q . k_j) v_j
  *   lse  f32  [S, R, Hq]    = log sum_j exp(scale * q . k_j)
  * Rows that do not exist give o = 0 and lse = -inf.  A row whose q holds an infinity or NaN, or that sees a
- * logit of NaN (a K scale of NaN) or a page whose V scale is not finite, gives NaN for o and lse; other rows are
- * not touched by it.
+ * logit of NaN (a K scale of NaN) or a page whose V scale is not finite, gives NaN for o and lse.  A NaN among V's
+ * codes (fmt 1; bolt_kv_append writes none) gives at least its place of o NaN for the rows that see it.  Other rows
+ * are not touched by these.
  * Logits, sums and values are fp32.  A position's weight is rounded to fp16 (11 bits) once; where weight times V
  * scale is below 2^-22 of the row's largest such product, it errs by at most 2^-33 of that instead, and below 2^-134
  * it is left out of o and lse (a scale of 0 counts as 2^-96).  q's values keep their bits down to 2^-31 of the row's

@@ -311,13 +311,32 @@ __global__ void __launch_bounds__(kThreads, CPS) kv_attention_kernel(
       VCodes<D> v;
       v.load(b + 16 * D, v_at);
       if (FMT == kKvE4m3 && !whole) {
-        // weights of 0 must not meet NaN: a stale e4m3 code that no row of the block sees
+        // weights of 0 must not meet a NaN code (a stale one that no row sees, or one that some rows see): it becomes
+        // 0, and the rows that see its position get a sum of NaN
+        uint32_t nan = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int j = j0 + (i >> 1) * 8 + place<D>(2 * q4 + (i & 1));
-          if (j > span.last || (p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks))
+          uint32_t any = 0;
 #pragma unroll
-            for (int wd = 0; wd < D / 32; ++wd) v.w[i][wd] = 0;
+          for (int wd = 0; wd < D / 32; ++wd) {
+            const uint32_t bytes = kv_nan_bytes(v.w[i][wd]);
+            any |= bytes;
+            v.w[i][wd] &= ~bytes;
+          }
+          if (any) nan |= 1u << ((i >> 1) * 8 + place<D>(2 * q4 + (i & 1)));
+        }
+        nan = __reduce_or_sync(0xffffffffu, nan);
+        if (nan) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = 8 * i + place<D>(g);
+            if (nan >> at & 1)
+#pragma unroll
+              for (int r = 0; r < NT; ++r)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (kv_sees(p.mask, pos[r][e], j0 + at)) l_run[r][e] = NAN;
+          }
         }
       }
       // the value axis: rows g and 8 + g of tile t are the values (D / 8) g + 2 t and + 1

@@ -128,6 +128,11 @@ __device__ __forceinline__ uint32_t seen_bits(const KvMask& m, int pos, int j0) 
   return seen;
 }
 
+// Every row of the span sees all of the step from j0 on.
+__device__ __forceinline__ bool sees_whole(const KvMask& m, const KvSpan& span, int j0) {
+  return j0 + 15 <= span.first && (m.window == 0 || j0 > span.last - m.window || j0 + 15 < m.sinks);
+}
+
 // 16 codes as 16 halves in order: exact V codes, or K's (k_to_half).
 template <int FMT, bool V>
 __device__ __forceinline__ void convert16(const uint4& x, uint4& lo, uint4& hi) {
@@ -159,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
   __shared__ KvWalk s_walk;
   __shared__ KvSegment s_seg;
   __shared__ int s_more;
+  __shared__ unsigned s_nan[kRows / 32];  // the rows that see a NaN among V's codes of a step that not all rows see
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float4* s_meta = reinterpret_cast<float4*>(smem + L::kMeta);  // [tile % 64][step]: K scale, log2 and 1 / V scale, position and flags
   float2* sf = reinterpret_cast<float2*>(smem + L::kFactor);    // [row]: logit factor and shift (kv_make_q)
@@ -217,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
 
   while (true) {
     if (tid == 0) s_more = s_walk.next(p, w.row_blocks, kRows, s_seg);
+    if (FMT == kKvE4m3 && tid < kRows / 32) s_nan[tid] = 0;
     __syncthreads();
     if (!s_more) break;
     const int i0 = s_seg.i0, i1 = s_seg.i1, tiles = (i1 - i0 + kSteps - 1) / kSteps;
@@ -232,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
       int flags = 0;
       if (meta.page < 0)
         flags = kDead;
-      else if (j0 + 15 <= span.first && (p.mask.window == 0 || j0 > span.last - p.mask.window || j0 + 15 < p.mask.sinks))
+      else if (sees_whole(p.mask, span, j0))
         flags = kWhole;
       const float2 vs = kv_v_scale(meta.vs);
       s_meta[t % kMetaTiles * kSteps + cw] = make_float4(meta.ks, vs.x, vs.y, __int_as_float(j0 | flags));
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
       uint64_t* empty = full + kConvWarps * kSlots;
       const int* lines = reinterpret_cast<const int*>(smem + L::kLine) + cw * kMetaTiles;
       const int from_at = kv_at<D>(r, chunk * 16), to_at = 2 * cw * L::kGroup + 2 * chunk * 128 + r * 16;
-      const auto convert = [&](int u, auto is_v, bool dead, int j0, uint8_t* tile) {
+      const auto convert = [&](int u, auto is_v, bool dead, bool whole, int j0, uint8_t* tile) {
         constexpr bool V = decltype(is_v)::value;
         const unsigned n = taken + u, slot = n % kSlots;
         if (!wait(smem_u32(full + slot), n / kSlots)) return false;
@@ -339,13 +346,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
         if (dead) {  // no codes
 #pragma unroll
           for (int v = 0; v < D / 32; ++v) x[v] = make_uint4(kZero, kZero, kZero, kZero);
-        } else if (FMT == kKvE4m3 && V && (j0 + 15 > span.first || p.mask.window)) {
-          // what no row of the block sees may be a NaN code, which a weight of 0 must not meet
+        } else if (FMT == kKvE4m3 && V && !whole) {
+          // weights of 0 must not meet a NaN code (a stale one that no row sees, or one that some rows see): it
+          // becomes 0, and the rows that see its position are marked
+          uint32_t nan = 0;
 #pragma unroll
           for (int v = 0; v < D / 32; ++v) {
-            const int j = j0 + (v & 1) * 8 + r;
-            if (j > span.last || (p.mask.window && j <= span.first - p.mask.window && j >= p.mask.sinks))
-              x[v] = make_uint4(kZero, kZero, kZero, kZero);
+            const uint4 b = make_uint4(kv_nan_bytes(x[v].x), kv_nan_bytes(x[v].y), kv_nan_bytes(x[v].z), kv_nan_bytes(x[v].w));
+            if (b.x | b.y | b.z | b.w) nan |= 1u << ((v & 1) * 8 + r);
+            x[v] = make_uint4(x[v].x & ~b.x, x[v].y & ~b.y, x[v].z & ~b.z, x[v].w & ~b.w);
+          }
+          nan = __reduce_or_sync(0xffffffffu, nan);
+          if (nan) {
+#pragma unroll 1
+            for (int k = 0; k < kRows / 32; ++k) {
+              const int at_row = s_seg.seq.start + static_cast<int>((s_seg.m0 + 32 * k + lane) / static_cast<unsigned>(p.G));
+              const unsigned rows = __ballot_sync(0xffffffffu, seen_bits(p.mask, at_row, j0) & nan);
+              if (lane == 0) atomicOr(&s_nan[k], rows);
+            }
           }
         }
 #pragma unroll
@@ -370,10 +388,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
         if (n > 0 && !wait(s_full(i), n - 1)) break;
         const bool dead = lines[t % kMetaTiles] < 0;
         const int j0 = span.base(min(i0 + t * kSteps + cw, i1 - 1));
-        if (!convert(2 * t, std::false_type(), dead, j0, smem + L::kK + i * L::kTile)) break;
+        const bool whole = sees_whole(p.mask, span, j0);
+        if (!convert(2 * t, std::false_type(), dead, whole, j0, smem + L::kK + i * L::kTile)) break;
         if (lane == 0) mbar_arrive(k_full(i));
         if (n > 0 && !wait(o_full(i), n - 1)) break;
-        if (!convert(2 * t + 1, std::true_type(), dead, j0, smem + L::kV + i * L::kTile)) break;
+        if (!convert(2 * t + 1, std::true_type(), dead, whole, j0, smem + L::kV + i * L::kTile)) break;
         if (lane == 0) mbar_arrive(v_full(i));
       }
     } else {
@@ -511,6 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv_attention_umma_kernel(
       const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
       const float ref = sm[i * kRows + row], top = fmaxf(sm[row], sm[kRows + row]);
       const float f = ref == -INFINITY ? 0.f : ex2(ref - top);
+      if (FMT == kKvE4m3 && (s_nan[row >> 5] >> (row & 31) & 1)) sl[i * kRows + row] = NAN;
 #pragma unroll 1
       for (int q = 0; q < D / 16; ++q) {
         float x[16];

@@ -307,6 +307,9 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
+// The bytes of a word of e4m3 codes that are NaN, all ones.
+__device__ __forceinline__ uint32_t kv_nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu); }
+
 // Four K codes as fp16 pairs: an int8 code's byte alone is the subnormal 2^-24 code, and its offset of 128 comes off the logit as 128 times the sum of the query row
 // (kv_make_q), which costs one operation a row instead of one a pair.
 template <int FMT>

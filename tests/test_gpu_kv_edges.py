@@ -135,6 +135,27 @@ def test_a_page_whose_v_scale_is_not_finite(R, G, fmt, value):
     _check(o, lse, ref, 128, bad)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("R,G,window,at", [(4, 2, 0, 2), (8, 1, 0, 7), (8, 2, 3, 2), (16, 1, 20, 0), (20, 3, 0, 11),
+                                           (30, 1, 20, 3), (130, 2, 0, 64), (150, 1, 40, 60), (40, 1, 0, -200)])
+def test_a_nan_among_the_v_codes(R, G, window, at, D):
+    # the call's row `at` is the first that sees it: a NaN in o for that row and those after it that still do, and
+    # nothing of it in the others'
+    c = kv.Cache([300 + R, 40 + R], 2, D, 16, 1, seed=207)
+    q = kv._rows(2, R, 2 * G, D, seed=208)
+    start = c.lens - R
+    ref = O.kv_attention(q, *c.host(), c.table, start, c.lens, 0.1, window=window, sinks=2 if window else 0, fmt=1)
+    j = 300 + at
+    c.v[c.table[0, j // 16].long(), 1, j % 16, 5] = 0x7F
+    o, lse = kv._attention(c, q, start, 0.1, window=window, sinks=2 if window else 0)
+    bad = np.zeros(q.shape[:3], dtype=bool)
+    bad[0, max(at, 0):(at + window if window else R), G:] = True
+    assert bool(o[0, :, G:, 5].cpu()[torch.from_numpy(bad[0, :, G:])].isnan().all())
+    o[torch.from_numpy(bad).to(DEV)], lse[torch.from_numpy(bad).to(DEV)] = float("nan"), float("nan")
+    _check(o, lse, ref, D, bad)
+    assert ops.device_status() == 0
+
+
 # ---------------------------------------------------------------------------------------------
 # page tables
 # ---------------------------------------------------------------------------------------------
