@@ -24,7 +24,7 @@
 // ahead of their use and 16-byte copies by the lanes do not get there: with the arithmetic taken out they read
 // 3.8 TB/s at any ring depth, tensor copies 5.9.  One sequence of 131,001 positions (16 rows a head, 2 heads)
 // takes 30 us, 22 of them here: the way from the length to the first product, 37 steps a warp, and the parts'
-// 2.4 MB.  Short items (48 sequences, 16 heads of 64 values, 68 steps an item: 36 us) are bound by their set-up.
+// 2.4 MB.  Short items (48 sequences, 16 heads of 64 values, 68 steps an item: 37 us) are bound by their set-up.
 #include "kv_split.cuh"
 
 namespace bolt {
