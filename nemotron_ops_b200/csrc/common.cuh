@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <atomic>
+#include <mutex>
 #include <stdint.h>
 
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ < 1000)
@@ -160,6 +161,7 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 struct SmemOptIn {
   static constexpr int kMaxDevices = 64;
   std::atomic<size_t> bytes[kMaxDevices];
+  std::mutex mu;  // the call and the note of it go together: a later smaller size must not undo a larger one
 };
 
 template <typename Kern>
@@ -168,13 +170,11 @@ inline cudaError_t allow_smem(Kern kern, size_t bytes, SmemOptIn& s) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= SmemOptIn::kMaxDevices)
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
   std::atomic<size_t>& cur = s.bytes[dev];
-  if (bytes <= cur.load(std::memory_order_relaxed)) return cudaSuccess;
+  if (bytes <= cur.load()) return cudaSuccess;
+  std::lock_guard<std::mutex> lock(s.mu);
+  if (bytes <= cur.load()) return cudaSuccess;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  if (e == cudaSuccess) {
-    size_t c = cur.load();
-    while (c < bytes && !cur.compare_exchange_weak(c, bytes)) {
-    }
-  }
+  if (e == cudaSuccess) cur.store(bytes);
   return e;
 }
 
